@@ -22,6 +22,10 @@ EINVAL = 22
 HIP_BASE = 1000
 ROPE_NEOX = 0
 ROPE_INTERLEAVED = 1
+F32 = 0  # FENCE_F32
+F16 = 1
+KV_INT8 = 0  # FENCE_KV_INT8
+KV_E4M3 = 1
 ARRIVE_WORDS_PER_HEAD = 64  # FENCE_ARRIVE_WORDS_PER_HEAD
 QK8_0 = 32
 Q8_0_BLOCK_BYTES = 34
@@ -72,6 +76,12 @@ SIGNATURES = {
     "fence_softmax_causal": (_P, _L, _I, _I, _P),
     "fence_embed_q8_0_gather": (_P, _P, _L, _P, _L, _I, _P),
     "fence_embed_q8_0_gather_rms_norm": (_P, _P, _L, _P, _L, _I, _P, _F, _P),
+    "fence_kv_plan": (_P, _P, _P, _I, _P, _I, _I, _P, _P, _P, _I, _P, _P, _P, _L, _P, _P),
+    "fence_store_kv_q8": (_P, _P, _P, _I, _L, _P, _L, _P),
+    "fence_gqa_attention_q8": (_P, _P, _I, _L, _L, _P, _P, _I, _P, _P, _I, _I, _I, _P, _L, _P),
+    "fence_gqa_attention_q8_workspace": (_I, _I, _I, _I, _I),
+    "fence_sample": (_P, _P, _L, _I, _L, _P, _P, _P, _P, _P, _P, _L, _P),
+    "fence_sample_workspace": (_L, _I),
     "fence_rope_inv_freq": (_P, _I, _F),
     "fence_time_next_launch": (_P, _P),
     "fence_time_next_launches": (_P, _P, _I),
@@ -80,7 +90,8 @@ SIGNATURES = {
     "fence_status_string": (_I,),
     "fence_version": (),
 }
-_RESTYPES = {"fence_status_string": ctypes.c_char_p, "fence_version": ctypes.c_char_p}
+_RESTYPES = {"fence_status_string": ctypes.c_char_p, "fence_version": ctypes.c_char_p,
+             "fence_gqa_attention_q8_workspace": _L, "fence_sample_workspace": _L}
 
 _lib = None
 
@@ -89,6 +100,12 @@ class RmsInput(ctypes.Structure):
     """fence_rms_input: h = hidden + residual, x_f16 = binary16(rms_norm(h))."""
     _fields_ = [("hidden", _P), ("residual", _P), ("hidden_out", _P), ("weight", _P), ("x_f16", _P),
                 ("eps", _F)]
+
+
+class KvPages(ctypes.Structure):
+    """fence_kv_pages: one layer's pages of an 8-bit KV cache."""
+    _fields_ = [("k", _P), ("v", _P), ("k_scale", _P), ("v_scale", _P), ("n_pages", _I), ("page_size", _I),
+                ("n_kv_heads", _I), ("head_dim", _I), ("type", _I)]
 
 
 class FenceError(RuntimeError):
@@ -315,6 +332,42 @@ def embed_q8_0_gather(out, table, vocab, ids, tokens, dim, stream=None):
 
 def embed_q8_0_gather_rms_norm(out, table, vocab, ids, tokens, dim, w, eps, stream=None):
     _call("fence_embed_q8_0_gather_rms_norm", out, table, vocab, ids, tokens, dim, w, eps, stream)
+
+
+def kv_pages(k, v, k_scale, v_scale, n_pages, page_size, n_kv_heads, head_dim, type):
+    return KvPages(k, v, k_scale, v_scale, n_pages, page_size, n_kv_heads, head_dim, type)
+
+
+def kv_plan(lens_out, lens, new_lens, batch, block_table, max_blocks, page_size, free_pages, free_count_out,
+            free_count, n_pages, q_start, positions, slots, max_tokens, admitted, stream=None):
+    _call("fence_kv_plan", lens_out, lens, new_lens, batch, block_table, max_blocks, page_size, free_pages,
+          free_count_out, free_count, n_pages, q_start, positions, slots, max_tokens, admitted, stream)
+
+
+def store_kv_q8(cache, k, v, type, ld, slots, tokens, stream=None):
+    """cache: a KvPages; type: F32 or F16 of k and v."""
+    _call("fence_store_kv_q8", ctypes.byref(cache), k, v, type, ld, slots, tokens, stream)
+
+
+def gqa_attention_q8(out, q, type, ldq, ldo, cache, block_table, max_blocks, kv_lens, q_start, batch, max_q_len,
+                     n_q_heads, workspace, workspace_bytes, stream=None):
+    """cache: a KvPages; type: F32 or F16 of q and out."""
+    _call("fence_gqa_attention_q8", out, q, type, ldq, ldo, ctypes.byref(cache), block_table, max_blocks, kv_lens,
+          q_start, batch, max_q_len, n_q_heads, workspace, workspace_bytes, stream)
+
+
+def gqa_attention_q8_workspace(batch, max_q_len, n_q_heads, n_kv_heads, head_dim) -> int:
+    return lib().fence_gqa_attention_q8_workspace(batch, max_q_len, n_q_heads, n_kv_heads, head_dim)
+
+
+def sample(out, logits, rows, vocab, ld, temperature, top_k, top_p, min_p, u, workspace, workspace_bytes,
+           stream=None):
+    _call("fence_sample", out, logits, rows, vocab, ld, temperature, top_k, top_p, min_p, u, workspace,
+          workspace_bytes, stream)
+
+
+def sample_workspace(rows, vocab) -> int:
+    return lib().fence_sample_workspace(rows, vocab)
 
 
 def time_next_launch(start, stop) -> None:

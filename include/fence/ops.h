@@ -325,6 +325,136 @@ int fence_embed_q8_0_gather_rms_norm(float* out, const void* table,
                                      float eps, hipStream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Batched serving over a paged 8-bit KV cache.  No counterparts in the
+ * reference, which decodes one sequence over a contiguous binary16 cache and
+ * samples on the host.  A step is: fence_kv_plan (once), then per layer
+ * fence_qk_norm_rope with the plan's positions, fence_store_kv_q8 with its
+ * slots and fence_gqa_attention_q8, and fence_sample on the logits.
+ * ------------------------------------------------------------------------ */
+
+/* Element types of q, k, v and outputs. */
+enum {
+    FENCE_F32 = 0,
+    FENCE_F16 = 1 /* binary16 */
+};
+
+/* Code types of an 8-bit cache: whole numbers -127..127, or OCP e4m3 (largest
+ * value 448, no infinities). */
+enum {
+    FENCE_KV_INT8 = 0,
+    FENCE_KV_E4M3 = 1
+};
+
+/* One layer's cache pages.  Position j of a sequence lives in page
+ * block_table[seq][j / page_size] at offset j % page_size; what it holds is
+ * code * scale, with one scale per page and kv head (K and V each).
+ * page_size 16, 32, 64, 128 or 256; head_dim a multiple of 16 up to 256;
+ * n_pages * page_size <= INT32_MAX; k and v 16-byte aligned. */
+typedef struct {
+    void* k;        /* codes [n_pages][n_kv_heads][page_size][head_dim] */
+    void* v;        /* the same */
+    float* k_scale; /* [n_pages][n_kv_heads] */
+    float* v_scale; /* the same */
+    int n_pages;
+    int page_size;
+    int n_kv_heads;
+    int head_dim;
+    int type;       /* FENCE_KV_INT8 or FENCE_KV_E4M3 */
+} fence_kv_pages;
+
+/* Plans a step of `batch` sequences: which page and slot each new token gets.
+ * Device arrays throughout.  lens[b]: cached tokens; new_lens[b]: tokens this
+ * step, 0 for none, negative for a sequence that has ended.  free_pages
+ * [n_pages] is a stack of free page ids, free_count[0] of them.
+ *   1. The pages of ended sequences, in batch and block order, go onto the
+ *      stack; their length becomes 0.
+ *   2. Sequence b is admitted if its tokens end within max_tokens, its new
+ *      length fits max_blocks pages, and either it needs no new page or the
+ *      pages needed by the sequences up to and including it (those that the
+ *      first two conditions let pass) are on the stack.  Its pages come off
+ *      the top of the stack and into its row of block_table
+ *      [batch][max_blocks]; admitted[b] = 1 (also if it ended), else 0.
+ *   3. lens_out[b]: the new length (the old one if not admitted);
+ *      free_count_out[0]: pages left.  Both may equal their inputs.
+ *   4. q_start[0..batch]: the first row of each sequence's tokens, in batch
+ *      order, admitted or not.  For row t of them positions[t] is its
+ *      position and slots[t] = page * page_size + offset, -1 if it was not
+ *      admitted.  Rows behind the last, up to max_tokens: position 0, slot -1,
+ *      so that a step captured at a fixed number of rows can run padded.
+ * The entries of block_table behind a sequence's pages, and those of ended
+ * sequences, are left as they were.  Released ids that would not fit the
+ * stack are dropped.  page_size as in fence_kv_pages; max_blocks *
+ * page_size, n_pages * page_size and max_tokens <= INT32_MAX. */
+int fence_kv_plan(int32_t* lens_out, const int32_t* lens, const int32_t* new_lens, int batch,
+                  int32_t* block_table, int max_blocks, int page_size, int32_t* free_pages,
+                  int32_t* free_count_out, const int32_t* free_count, int n_pages, int32_t* q_start,
+                  int32_t* positions, int32_t* slots, int64_t max_tokens, int32_t* admitted,
+                  hipStream_t stream);
+
+/* Stores the k and v of `tokens` rows into their slots, rounded to 8 bits: the
+ * paged form of fence_store_kv.  k and v [tokens][n_kv_heads][head_dim] of
+ * `type` FENCE_F32 or FENCE_F16, ld >= n_kv_heads * head_dim elements from row
+ * to row (so they may be parts of one q/k/v row).  Rows with a slot outside
+ * [0, n_pages * page_size) are skipped.  The rows of one page must follow one
+ * another with slots that rise by one, as fence_kv_plan gives them.  For each
+ * page and head that receives rows,
+ *   scale = max(old, max|new values| / 127)   (448 for e4m3), in fp32,
+ * where old is the page's scale, or 0 if the rows begin at offset 0 (what the
+ * page held before is of no account then).  New codes are the values divided
+ * by scale, rounded to nearest, ties to even (0 where scale is 0); if the
+ * scale grew, the codes at the offsets before the rows are rounded again to
+ * the new scale.  A value that is not finite makes the scale so, and with it
+ * everything that is read from that page and head. */
+int fence_store_kv_q8(const fence_kv_pages* cache, const void* k, const void* v, int type, int64_t ld,
+                      const int32_t* slots, int64_t tokens, hipStream_t stream);
+
+/* Attention of a batch over an 8-bit cache: the batched, paged form of
+ * fence_gqa_attention, for single tokens, drafted tokens and prompts alike.
+ * Sequence b has the rows q_start[b] .. q_start[b+1] of q and out
+ * [rows][n_q_heads][head_dim] (`type` FENCE_F32 or FENCE_F16 for both, ldq and
+ * ldo elements from row to row, at least n_q_heads * head_dim); its last row
+ * is position kv_lens[b] - 1, so row i sees the positions below kv_lens[b] -
+ * (q_start[b+1] - q_start[b]) + i + 1.  A row that sees none is zeros; rows
+ * that are no sequence's are left as they were.  max_q_len bounds the rows of
+ * a sequence; rows past it are not computed.  Positions past max_blocks *
+ * page_size, and those in pages with an id outside [0, n_pages), count as not
+ * there.  scale = 1/sqrt(head_dim); the softmax and all sums are held in
+ * fp32.  FENCE_F32 agrees with fp32 arithmetic to fp32 rounding; FENCE_F16
+ * rounds the probabilities to binary16.  n_q_heads % n_kv_heads == 0.
+ * workspace: fence_gqa_attention_q8_workspace(...) bytes, 16-byte aligned;
+ * calls that overlap must not share it. */
+int fence_gqa_attention_q8(void* out, const void* q, int type, int64_t ldq, int64_t ldo,
+                           const fence_kv_pages* cache, const int32_t* block_table, int max_blocks,
+                           const int32_t* kv_lens, const int32_t* q_start, int batch, int max_q_len,
+                           int n_q_heads, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* Workspace bytes of fence_gqa_attention_q8 (host; 0 for bad arguments). */
+int64_t fence_gqa_attention_q8_workspace(int batch, int max_q_len, int n_q_heads, int n_kv_heads,
+                                         int head_dim);
+
+/* Samples a token per row of logits [rows][vocab] (ld >= vocab floats from
+ * row to row) with the random number u[row] in [0, 1).  In descending order of
+ * the logits, the lowest index first among equals, with the weights
+ * exp((x - max) / temperature): kept are the first top_k; of these the
+ * shortest beginning that holds at least top_p of their weight; of these the
+ * ones whose weight is at least min_p (the first one's is 1).  out[row] is the
+ * first kept token at which the running sum of weights passes u times the
+ * kept weight.  Sums are held in 64 bits.  temperature, top_k, top_p, min_p
+ * and u are device arrays of one entry per row; NULL temperature: 1, NULL or
+ * out-of-range filters (top_k outside 1..vocab-1, top_p not below 1, min_p
+ * not above 0): off.  temperature <= 0: the largest logit, the lowest index
+ * first.  NaN logits count as -inf; +inf ones share all the weight; a row
+ * with nothing above -inf gives 0.
+ * workspace: fence_sample_workspace(rows, vocab) bytes, 16-byte aligned;
+ * calls that overlap must not share it. */
+int fence_sample(int32_t* out, const float* logits, int64_t rows, int vocab, int64_t ld,
+                 const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                 const float* u, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
+/* Workspace bytes of fence_sample (host; 0 for bad arguments). */
+int64_t fence_sample_workspace(int64_t rows, int vocab);
+
+/* ---------------------------------------------------------------------------
  * Host-side helpers (no device work).
  * ------------------------------------------------------------------------ */
 
