@@ -39,9 +39,8 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 def _fence():
     """The framework's binding."""
-    pkg = glob.glob(os.path.join(glob.escape(ROOT), "*_amd"))[0]
-    if pkg not in sys.path:
-        sys.path.insert(0, pkg)
+    if "fence_ops" not in sys.modules:
+        sys.path.insert(0, glob.glob(os.path.join(glob.escape(ROOT), "*_amd"))[0])
     import fence_ops
 
     return fence_ops
