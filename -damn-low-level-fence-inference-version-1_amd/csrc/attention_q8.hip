@@ -18,15 +18,29 @@ namespace {
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float f16v __attribute__((ext_vector_type(16)));
 
-constexpr int kCols = 16;          // columns of a product: (row, head of the group) pairs
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
-constexpr int kUnit = 32 * kWaves; // positions a workgroup takes at a time, 32 a wave
+// Columns of the products are the (row, head of the group) pairs of one kv
+// head; a sequence's are taken kCols or kBigCols at a time.
+constexpr int kCols = 16;              // attention_q8_kernel: each wave all of them, its own positions
+constexpr int kUnit = 32 * kWaves;     // and the positions its workgroup takes at a time
+constexpr int kBigCols = 32 * kWaves;  // prompt_q8_kernel: each wave 32 of them, all positions
+constexpr int kBigUnit = 64;
+// Up to this many columns a sequence goes to attention_q8_kernel.
+#ifndef FENCE_ATTN_Q8_SMALL
+#define FENCE_ATTN_Q8_SMALL 32
+#endif
+constexpr int kSmall = FENCE_ATTN_Q8_SMALL;
 #ifndef FENCE_ATTN_Q8_GRID
 #define FENCE_ATTN_Q8_GRID 1024
 #endif
-constexpr int kMaxGrid = FENCE_ATTN_Q8_GRID;
+constexpr int kGrid = FENCE_ATTN_Q8_GRID;
+#ifndef FENCE_ATTN_Q8_BIG_GRID
+#define FENCE_ATTN_Q8_BIG_GRID 512
+#endif
+constexpr int kBigGrid = FENCE_ATTN_Q8_BIG_GRID;
 
 struct Q8Args {
     void* out;
@@ -42,51 +56,67 @@ struct Q8Args {
     float* ws;
     int n_pages, page_shift, n_kv_heads, head_dim, group;
     int max_blocks, batch, max_q_len;
-    int part_cols;  // columns of a partial in the workspace
+    int part_cols;  // columns of a part in the workspace
     float scale_log2;
 };
 
-// A sequence as the products see it.
+// A sequence as one of the two kernels sees it: rows = 0 if it is the other's.
+template <bool BIG>
 struct Seq {
+    static constexpr int COLS = BIG ? kBigCols : kCols;
+    static constexpr int UNIT = BIG ? kBigUnit : kUnit;
     int row0, rows, q_len, kv;  // first row, rows computed, rows there are, positions
-    __device__ __forceinline__ int tiles(int group) const { return (rows * group + kCols - 1) / kCols; }
-    // positions that the last column of a tile sees
-    __device__ __forceinline__ int sees(int tile, int group) const {
-        int i = (tile * kCols + kCols - 1) / group;
-        if (i > q_len - 1) i = q_len - 1;
+
+    __device__ __forceinline__ Seq(const Q8Args& a, int b) {
+        row0 = a.q_start[b];
+        const int n = a.q_start[b + 1] - row0;
+        q_len = n < 0 ? 0 : n;
+        rows = q_len < a.max_q_len ? q_len : a.max_q_len;
+        if ((rows * a.group > kSmall) != BIG) rows = 0;
+        const int cap = a.max_blocks << a.page_shift;
+        const int len = a.kv_lens[b];
+        kv = len < 0 ? 0 : len > cap ? cap : len;
+    }
+    __device__ __forceinline__ int tiles(int group) const { return (rows * group + COLS - 1) / COLS; }
+    // positions that row i sees, i at most q_len - 1
+    __device__ __forceinline__ int row_sees(int i) const {
         const int n = kv - q_len + i + 1;
         return n < 0 ? 0 : n;
     }
-    // workgroup units of one kv head's tile: one at least, which writes the zeros of rows that see nothing
+    // positions that the last column of a tile sees
+    __device__ __forceinline__ int sees(int tile, int group) const {
+        const int i = (tile * COLS + COLS - 1) / group;
+        return row_sees(i < q_len - 1 ? i : q_len - 1);
+    }
+    // units of one kv head's tile: one at least, which writes the zeros of rows that see nothing
     __device__ __forceinline__ int units(int tile, int group) const {
-        const int n = (sees(tile, group) + kUnit - 1) / kUnit;
+        const int n = (sees(tile, group) + UNIT - 1) / UNIT;
         return n < 1 ? 1 : n;
+    }
+    // f(tile, units) for every tile until it returns false
+    template <class F>
+    __device__ __forceinline__ void each_tile(int group, F f) const {
+        const int n = tiles(group), whole = COLS / group, part = COLS % group;
+        int i = (COLS - 1) / group, over = (COLS - 1) % group;  // sees() without its division
+        for (int t = 0; t < n; ++t) {
+            const int sees = row_sees(i < q_len - 1 ? i : q_len - 1);
+            if (!f(t, sees > UNIT ? (sees + UNIT - 1) / UNIT : 1)) return;
+            i += whole;
+            over += part;
+            if (over >= group) over -= group, ++i;
+        }
+    }
+    // of all kv heads and tiles
+    __device__ __forceinline__ int64_t all_units(const Q8Args& a) const {
+        int64_t n = 0;
+        each_tile(a.group, [&](int, int u) { return n += u, true; });
+        return n * a.n_kv_heads;
     }
 };
 
-__device__ __forceinline__ Seq sequence(const Q8Args& a, int b) {
-    Seq s;
-    s.row0 = a.q_start[b];
-    const int n = a.q_start[b + 1] - s.row0;
-    s.q_len = n < 0 ? 0 : n;
-    s.rows = s.q_len < a.max_q_len ? s.q_len : a.max_q_len;
-    const int cap = a.max_blocks << a.page_shift;
-    const int kv = a.kv_lens[b];
-    s.kv = kv < 0 ? 0 : kv > cap ? cap : kv;
-    return s;
-}
-
-// Units of a whole sequence.
-__device__ __forceinline__ int64_t seq_units(const Q8Args& a, int b) {
-    const Seq s = sequence(a, b);
-    int64_t n = 0;
-    for (int t = 0; t < s.tiles(a.group); ++t) n += s.units(t, a.group);
-    return n * a.n_kv_heads;
-}
-
 // Prefix sums of the sequences' units over the workgroup: the total, and the
 // sequence that unit `find(total)` belongs to with the units before it.
-template <class F>
+template <bool BIG, class F>
 __device__ __forceinline__ int64_t locate(const Q8Args& a, F find, int* seq, int64_t* before) {
     __shared__ int64_t waves[kWaves];
     __shared__ int64_t found_before;
@@ -97,7 +127,7 @@ __device__ __forceinline__ int64_t locate(const Q8Args& a, F find, int* seq, int
         int64_t at = 0;
         const int64_t target = pass ? find(total) : -1;
         for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
-            if (!pass || a.batch > kThreads) mine = b0 + tid < a.batch ? seq_units(a, b0 + tid) : 0;
+            if (!pass || a.batch > kThreads) mine = b0 + tid < a.batch ? Seq<BIG>(a, b0 + tid).all_units(a) : 0;
             int64_t v = mine;
 #pragma unroll
             for (int d = 1; d < kWave; d *= 2) {
@@ -132,10 +162,65 @@ __device__ __forceinline__ int sharers(int64_t total, int grid) {
     return total < 1 ? 1 : total < grid ? static_cast<int>(total) : grid;
 }
 
-// The workgroup of `grid` that unit u of `total` falls to, when workgroup w
-// takes the units from w * total / grid to (w + 1) * total / grid.
-__device__ __forceinline__ int owner(int64_t u, int64_t total, int grid) {
-    return static_cast<int>(((u + 1) * grid - 1) / total);
+// A workgroup's place in the units, in the order of sequences, tiles, kv heads
+// and positions.
+template <bool BIG>
+struct Place {
+    int64_t u, u_end;
+    int seq, tile, head, unit, units;
+
+    // Of unit `at(total, grid)`; false if there is none for this workgroup.
+    template <class F>
+    __device__ __forceinline__ bool find(const Q8Args& a, int me, int* grid, int64_t* total, F at) {
+        int64_t before;
+        *total = locate<BIG>(a, [&](int64_t n) { return at(n, sharers(n, *grid)); }, &seq, &before);
+        *grid = sharers(*total, *grid);
+        if (me >= *grid || *total == 0) return false;
+        u = at(*total, *grid);
+        const Seq<BIG> s(a, seq);
+        int64_t rest = u - before;
+        s.each_tile(a.group, [&](int t, int n) {
+            tile = t;
+            units = n;
+            if (rest < static_cast<int64_t>(n) * a.n_kv_heads) return false;
+            rest -= static_cast<int64_t>(n) * a.n_kv_heads;
+            return true;
+        });
+        head = static_cast<int>(rest / units);
+        unit = static_cast<int>(rest % units);
+        seq = __builtin_amdgcn_readfirstlane(seq);
+        tile = __builtin_amdgcn_readfirstlane(tile);
+        head = __builtin_amdgcn_readfirstlane(head);
+        unit = __builtin_amdgcn_readfirstlane(unit);
+        units = __builtin_amdgcn_readfirstlane(units);
+        return true;
+    }
+    // Past the item (a sequence's tile and kv head); u < u_end says that there is another one.
+    __device__ __forceinline__ void next(const Q8Args& a) {
+        unit = 0;
+        if (++head < a.n_kv_heads) return;
+        head = 0;
+        Seq<BIG> s(a, seq);
+        if (++tile == s.tiles(a.group)) {
+            tile = 0;
+            do s = Seq<BIG>(a, ++seq);
+            while (s.rows == 0);
+        }
+        units = s.units(tile, a.group);
+    }
+};
+
+// Where a workgroup leaves its part of an item that it shares: the one that
+// it ends (or passes through) and the one that it begins.  A part: per column
+// the running maximum, the sum and the unnormalised output.
+__device__ __forceinline__ float* part_at(const Q8Args& a, int wg, bool begins, int hd) {
+    return a.ws + static_cast<int64_t>(wg * 2 + (begins ? 1 : 0)) * a.part_cols * (hd + 2);
+}
+
+template <int QT>
+__device__ __forceinline__ void put(void* out, int64_t at, float v) {
+    if constexpr (QT == FENCE_F32) static_cast<float*>(out)[at] = v;
+    else static_cast<uint16_t*>(out)[at] = f32_to_f16_bits(v);
 }
 
 // Codes to binary16, four bytes to two pairs.  int8: with the sign bit
@@ -186,36 +271,24 @@ __global__ __launch_bounds__(kThreads) void attention_q8_kernel(Q8Args a) {
     const int r = lane % 16, g = lane / 16;
     const int hd = a.head_dim, page_mask = (1 << a.page_shift) - 1;
 
-    int b;
-    int64_t before;
     const int me = blockIdx.x;
-    const int64_t total = locate(a, [&](int64_t n) { return me * n / sharers(n, gridDim.x); }, &b, &before);
-    const int grid = sharers(total, gridDim.x);
-    if (me >= grid || total == 0) return;
-    int64_t u = me * total / grid;
-    const int64_t u_end = (me + 1) * total / grid;
-    Seq s = sequence(a, b);
-    // the tile and head in which u lies, in the order of tiles and then heads
-    int tile = 0, units = s.units(0, a.group);
-    int64_t rest = u - before;
-    while (rest >= static_cast<int64_t>(units) * a.n_kv_heads) {
-        rest -= static_cast<int64_t>(units) * a.n_kv_heads;
-        units = s.units(++tile, a.group);
-    }
-    int head = static_cast<int>(rest / units);
-    int unit = static_cast<int>(rest % units);
+    int grid = gridDim.x;
+    int64_t total;
+    Place<false> at_;
+    if (!at_.find(a, me, &grid, &total, [&](int64_t n, int g) { return me * n / g; })) return;
+    at_.u_end = (me + 1) * total / grid;
 
-    while (u < u_end) {
-        const int first = unit;
-        const int last = u_end - u < units - unit ? unit + static_cast<int>(u_end - u) : units;
+    while (at_.u < at_.u_end) {
+        const Seq<false> s(a, at_.seq);
+        const int tile = at_.tile, head = at_.head, first = at_.unit, units = at_.units;
+        const int last = at_.u_end - at_.u < units - first ? first + static_cast<int>(at_.u_end - at_.u) : units;
         const int cols = s.rows * a.group - tile * kCols < kCols ? s.rows * a.group - tile * kCols : kCols;
         // this lane's column
         const int col = tile * kCols + r;
         const int row = col / a.group;
         const bool mine = r < cols;
         const int qhead = head * a.group + col % a.group;
-        int sees = mine ? s.kv - s.q_len + row + 1 : 0;  // of its row
-        if (sees < 0) sees = 0;
+        const int sees = mine ? s.row_sees(row) : 0;
         const int end = s.sees(tile, a.group);
 
         h8 qf[PARTS][PIECES][2];
@@ -278,7 +351,7 @@ __global__ __launch_bounds__(kThreads) void attention_q8_kernel(Q8Args a) {
         float m = -__builtin_inff(), l = 0.0f;
         float vref = 0.0f;  // the largest V scale so far: o is in units of it times 2^-14
 
-        const int32_t* row_of_table = a.table + static_cast<int64_t>(b) * a.max_blocks;
+        const int32_t* row_of_table = a.table + static_cast<int64_t>(at_.seq) * a.max_blocks;
         for (int un = first; un < last; ++un) {
             const int pos0 = un * kUnit + wave * 32;
             if (pos0 >= end) break;
@@ -401,7 +474,7 @@ __global__ __launch_bounds__(kThreads) void attention_q8_kernel(Q8Args a) {
         }
         __syncthreads();
         const bool whole = first == 0 && last == units;
-        float* part = a.ws + static_cast<int64_t>(me * 2 + (first == 0 ? 1 : 0)) * pc * (HD + 2);
+        float* part = part_at(a, me, first == 0, HD);
         for (int x = tid; x < cols * HD; x += kThreads) {
             const int c = x / HD, d = x % HD;
             float top = -__builtin_inff();
@@ -420,9 +493,7 @@ __global__ __launch_bounds__(kThreads) void attention_q8_kernel(Q8Args a) {
                     const int cc = tile * kCols + c;
                     const int64_t to = static_cast<int64_t>(s.row0 + cc / a.group) * a.ldo +
                                        static_cast<int64_t>(head * a.group + cc % a.group) * hd + d;
-                    const float res = sum != 0.0f ? val / sum : 0.0f;
-                    if constexpr (F32) static_cast<float*>(a.out)[to] = res;
-                    else static_cast<uint16_t*>(a.out)[to] = f32_to_f16_bits(res);
+                    put<QT>(a.out, to, sum != 0.0f ? val / sum : 0.0f);
                 }
             } else {
                 part[c * (HD + 2) + 2 + d] = val;
@@ -431,104 +502,466 @@ __global__ __launch_bounds__(kThreads) void attention_q8_kernel(Q8Args a) {
         }
         __syncthreads();
 
-        u += last - first;
-        unit = 0;
-        if (u >= u_end) break;
-        if (++head == a.n_kv_heads) {
-            head = 0;
-            if (++tile == s.tiles(a.group)) {
-                tile = 0;
-                do {
-                    s = sequence(a, ++b);
-                } while (s.rows == 0);
-            }
-            units = s.units(tile, a.group);
-        }
+        at_.u += last - first;
+        if (at_.u < at_.u_end) at_.next(a);
     }
 }
 
-// The parts of the items (a sequence's tile and kv head) that more than one
-// workgroup took, in workgroup order.
-template <int QT, int HD>
-__global__ __launch_bounds__(kThreads) void attention_q8_merge_kernel(Q8Args a, int grid) {
-    const int tile = blockIdx.x / a.n_kv_heads, head = blockIdx.x % a.n_kv_heads;
-    int seq = blockIdx.y;
-    const Seq s = sequence(a, seq);
-    if (tile >= s.tiles(a.group)) return;
-    // units before this sequence, and in all
-    __shared__ int64_t waves[2][kWaves];
-    int64_t pre = 0, all = 0;
-    for (int b = threadIdx.x; b < a.batch; b += kThreads) {
-        const int64_t n = seq_units(a, b);
-        all += n;
-        if (b < seq) pre += n;
-    }
+// Prompts: a workgroup takes kBigCols columns, 32 a wave, and 64 positions at
+// a time, whose codes it converts once into LDS for all of its columns:
+//   S' [32 positions x 32 columns] = K [32 x HD] Q' [HD x 32],  twice
+//   O' [HD x 32 columns] += V' [HD x 64 positions] P [64 x 32]
+// LDS holds the fragments as the products read them (16 bytes a lane, lanes in
+// a row, so reads and writes meet no bank twice).  The first product leaves
+// lane (column n, half g) with positions 8 q + 4 g + (0 .. 3) of 32, which
+// the second takes as its k index in that order, so P stays in registers; row
+// r of V' product t stands for dimension r * HD / 32 + t, so a thread that
+// converts 4 dimensions of 8 positions writes whole fragments, and a lane ends
+// with 16 consecutive dimensions of its column.
+//
+// The next 64 positions' codes are loaded before the products of these and
+// converted behind them into the other half of LDS, with one barrier a turn.
+//
+// binary16 (QT = FENCE_F16): with the page's V scale as a power of two in the
+// exponent, one fused multiply-add and one exponential make the probability
+// that the product takes, and its sum comes from the rounded values by dot
+// products.  The running maximum and the largest V scale are only moved when
+// a value would grow past 2^15 (kSlack), so O is rarely rescaled.
+template <int TYPE, int QT, int HD>
+__global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(Q8Args a) {
+    constexpr bool F32 = QT == FENCE_F32;
+    constexpr int PARTS = F32 ? 2 : 1;
+    constexpr int KS = HD / 16;               // k steps of the first product
+    constexpr int NT = HD / 32;               // products over V
+    constexpr int KJ = HD * 4 / kThreads;     // 16-byte pieces of K a thread converts
+    constexpr int VITEMS = HD * 2;            // 8 positions x 4 dimensions of V
+    constexpr int VJ = (VITEMS + kThreads - 1) / kThreads;
+    constexpr float kBase = F32 ? 14.0f : 10.0f;  // log2 of what stands for 1 times the largest V scale
+    constexpr float kSlack = F32 ? 0.0f : 4.0f;
+    __shared__ h8 kbuf[2][2][KS][kWave];
+    __shared__ h8 vbuf[2][NT][4][kWave];
+    const int tid = threadIdx.x, lane = tid % kWave;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    const int n = lane % 32, g = lane / 32;
+    const int hd = a.head_dim, page_mask = (1 << a.page_shift) - 1;
+
+    const int me = blockIdx.x;
+    int grid = gridDim.x;
+    int64_t total;
+    Place<true> at;
+    if (!at.find(a, me, &grid, &total, [&](int64_t units, int w) { return me * units / w; })) return;
+    at.u_end = (me + 1) * total / grid;
+
+    while (at.u < at.u_end) {
+        const Seq<true> s(a, at.seq);
+        const int tile = at.tile, head = at.head, first = at.unit, units = at.units;
+        const int last = at.u_end - at.u < units - first ? first + static_cast<int>(at.u_end - at.u) : units;
+        const int cols = s.rows * a.group - tile * kBigCols;
+        const int c = wave * 32 + n;  // this lane's column
+        const bool mine = c < cols;
+        const int row = (tile * kBigCols + c) / a.group;
+        const int qhead = head * a.group + (tile * kBigCols + c) % a.group;
+        const int sees = mine ? s.row_sees(row) : 0;
+        const int end = s.sees(tile, a.group);
+        // what every column of this wave sees, and what one of them sees at most
+        const int least = __builtin_amdgcn_readfirstlane(s.row_sees((tile * kBigCols + wave * 32) / a.group));
+        int most;
+        {
+            const int i = (tile * kBigCols + wave * 32 + 31) / a.group;
+            most = wave * 32 < cols ? s.row_sees(i < s.q_len - 1 ? i : s.q_len - 1) : 0;
+            most = __builtin_amdgcn_readfirstlane(most);
+        }
+
+        h8 qf[PARTS][KS];
+        float unscale = a.scale_log2;
+        {
+            const int64_t from = mine ? static_cast<int64_t>(s.row0 + row) * a.ldq + static_cast<int64_t>(qhead) * hd : 0;
+            if constexpr (F32) {
+                float biggest = 0.0f;
 #pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-        pre += __shfl_xor(pre, d);
-        all += __shfl_xor(all, d);
-    }
-    if (threadIdx.x % kWave == 0) {
-        waves[0][threadIdx.x / kWave] = pre;
-        waves[1][threadIdx.x / kWave] = all;
-    }
-    __syncthreads();
-    pre = all = 0;
+                for (int k = 0; k < KS; ++k)
+                    if (mine && k * 16 < hd) {
+                        const float* src = static_cast<const float*>(a.q) + from + k * 16 + g * 8;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) pre += waves[0][w], all += waves[1][w];
-    grid = sharers(all, grid);
-    for (int t = 0; t < tile; ++t) pre += static_cast<int64_t>(s.units(t, a.group)) * a.n_kv_heads;
-    const int units = s.units(tile, a.group);
-    pre += static_cast<int64_t>(units) * head;
-    const int w0 = owner(pre, all, grid), w1 = owner(pre + units - 1, all, grid);
-    if (w0 == w1) return;
-    const int cols = s.rows * a.group - tile * kCols < kCols ? s.rows * a.group - tile * kCols : kCols;
-    const int pc = a.part_cols, hd = a.head_dim;
-    const auto part = [&](int w) {
-        return a.ws + static_cast<int64_t>(w * 2 + (w == w0 ? 1 : 0)) * pc * (HD + 2);
-    };
-    for (int x = threadIdx.x; x < cols * HD; x += kThreads) {
+                        for (int i = 0; i < 8; ++i) biggest = fmaxf(biggest, fabsf(src[i]));
+                    }
+                biggest = fmaxf(biggest, __shfl_xor(biggest, 32));
+                uint32_t e = __builtin_bit_cast(uint32_t, biggest) >> 23;
+                e = e < 15 ? 15 : e > 254 ? 254 : e;
+                const float up = __builtin_bit_cast(float, (268 - e) << 23);
+                unscale *= __builtin_bit_cast(float, (e - 14) << 23);
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    const float* src = static_cast<const float*>(a.q) + from + k * 16 + g * 8;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float y = mine && k * 16 < hd ? src[i] * up : 0.0f;
+                        const _Float16 hi = static_cast<_Float16>(y);
+                        qf[0][k][i] = hi;
+                        qf[1][k][i] = static_cast<_Float16>(y - static_cast<float>(hi));
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    h8 x = {};
+                    if (mine && k * 16 < hd) {
+                        const _Float16* src = static_cast<const _Float16*>(a.q) + from + k * 16 + g * 8;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) x[i] = src[i];
+                    }
+                    qf[0][k] = x;
+                }
+            }
+        }
+
+        f16v o[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
+        float m = -__builtin_inff(), l = 0.0f, vref = 0.0f;
+        const int32_t* pages = a.table + static_cast<int64_t>(at.seq) * a.max_blocks;
+
+        // Lane i of a wave knows the page of position i of 64.
+        const auto page_of = [&](int un) {
+            const int pos = un * kBigUnit + lane;
+            return un < last && pos < end ? pages[pos >> a.page_shift] : -1;
+        };
+        const auto there = [&](int id) { return id >= 0 && id < a.n_pages; };
+        u4 kw[KJ];
+        uint32_t vw[VJ][8];
+        // this thread's codes of a unit, 0 for positions that are not there
+        const auto load = [&](int un, int id) {
+            const bool ok = there(id);
+            const int64_t base = (static_cast<int64_t>(ok ? id : 0) * a.n_kv_heads + head) << a.page_shift;
+            const int64_t krow = (base + ((un * kBigUnit + lane) & page_mask)) * hd;
+#pragma unroll
+            for (int j = 0; j < KJ; ++j) {
+                const int d = (wave + kWaves * j) * 16;
+                kw[j] = u4{0, 0, 0, 0};
+                if (ok && d < hd) kw[j] = *reinterpret_cast<const u4*>(a.k + krow + d);
+            }
+#pragma unroll
+            for (int j = 0; j < VJ; ++j) {
+                const int item = tid + j * kThreads;
+                const int d = item % (HD / 4) * 4, sg = item / (HD / 4);
+                const int p0 = (sg / 2) * 16 + (sg % 2) * 4;
+                const int64_t vbase = __shfl(base, p0 & 63);
+                const bool vok = __shfl(static_cast<int>(ok), p0 & 63) && item < VITEMS && d < hd;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int p = un * kBigUnit + p0 + (i / 4) * 8 + i % 4;
+                    vw[j][i] = 0;
+                    if (vok && p < end)
+                        vw[j][i] = *reinterpret_cast<const uint32_t*>(a.v + (vbase + (p & page_mask)) * hd + d);
+                }
+            }
+        };
+        const auto scales = [&](int id, float* ks, float* vs) {
+            const int64_t i = static_cast<int64_t>(there(id) ? id : 0) * a.n_kv_heads + head;
+            *ks = there(id) ? a.ks[i] : 0.0f;
+            *vs = there(id) ? a.vs[i] : 0.0f;
+        };
+        const auto convert = [&](int half, float vs) {
+#pragma unroll
+            for (int j = 0; j < KJ; ++j) {
+                const int k = wave + kWaves * j;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    h2 c0, c1, c2, c3;
+                    codes_h<TYPE>(kw[j][2 * i], &c0, &c1);
+                    codes_h<TYPE>(kw[j][2 * i + 1], &c2, &c3);
+                    kbuf[half][lane / 32][k][i * 32 + lane % 32] = join(c0, c1, c2, c3);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < VJ; ++j) {
+                const int item = tid + j * kThreads;
+                const int d = item % (HD / 4) * 4, sg = item / (HD / 4);
+                // a page whose scale is 0 holds zeros, whatever its codes
+                const bool none = !F32 && __shfl(vs, ((sg / 2) * 16) & 63) == 0.0f;
+                h2 x[4][4];
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    const uint32_t y = none ? 0 : vw[j][2 * p], z = none ? 0 : vw[j][2 * p + 1];
+                    codes_h<TYPE>(__builtin_amdgcn_perm(z, y, 0x05010400u), &x[p][0], &x[p][1]);
+                    codes_h<TYPE>(__builtin_amdgcn_perm(z, y, 0x07030602u), &x[p][2], &x[p][3]);
+                }
+                if (item < VITEMS) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        vbuf[half][(d + i) % NT][sg / 2][(sg % 2) * 32 + (d + i) / NT] =
+                            join(x[0][i], x[1][i], x[2][i], x[3][i]);
+                }
+            }
+        };
+
+        int id = page_of(first), id_next = page_of(first + 1);
+        float ks, vs, ks_next = 0.0f, vs_next = 0.0f;
+        load(first, id);
+        scales(id, &ks, &vs);
+        convert(first & 1, vs);
+        __syncthreads();
+        for (int un = first; un < last; ++un) {
+            const int half = un & 1, pos0 = un * kBigUnit;
+            const uint64_t ok = __ballot(there(id));
+            const int id_after = page_of(un + 2);
+            if (un + 1 < last) {
+                load(un + 1, id_next);
+                scales(id_next, &ks_next, &vs_next);
+            }
+            if (pos0 < most) {
+                f16v st[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) st[h][i] = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) {
+                        const h8 kf = kbuf[half][h][k][lane];
+#pragma unroll
+                        for (int x = 0; x < PARTS; ++x)
+                            st[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[x][k], st[h], 0, 0, 0);
+                    }
+                }
+                // scales of the four groups of 16 positions
+                float fk[4], fv[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    fk[q] = readlane(ks, 16 * q) * unscale;
+                    fv[q] = readlane(vs, 16 * q);
+                }
+                const bool open = pos0 + kBigUnit <= least && ok == ~0ull;
+                const auto seen = [&](int h, int i) {
+                    const int p = h * 32 + (i / 4) * 8 + g * 4 + i % 4;
+                    return pos0 + p < sees && (ok >> (h * 32 + (i / 8) * 16) & 1);
+                };
+                if (!open) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (!seen(h, i)) st[h][i] = -__builtin_inff();
+                }
+                float top = -__builtin_inff();
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    float t = st[q / 2][(q % 2) * 8];
+#pragma unroll
+                    for (int i = 1; i < 8; ++i) t = fmaxf(t, st[q / 2][(q % 2) * 8 + i]);
+                    if (t > -__builtin_inff()) top = fmaxf(top, t * fk[q]);
+                }
+                top = fmaxf(top, __shfl_xor(top, 32));
+                float vtop = vref;
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (fv[q] > vtop && fv[q] < __builtin_inff()) vtop = fv[q];
+                const bool grow_v = vtop > (F32 ? vref : 2.0f * vref);
+                if (__any(top > m + kSlack) || grow_v) {
+                    const float now = fmaxf(m, top);
+                    const float alpha = now == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - now);
+                    const float vnow = grow_v ? vtop : vref;
+                    const float beta = vnow > 0.0f ? alpha * (vref / vnow) : 0.0f;
+                    m = now;
+                    vref = vnow;
+                    l *= alpha;
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) o[t] *= beta;
+                }
+                const float ref = m == -__builtin_inff() ? 0.0f : m;
+                const float vone = vref > 0.0f ? 1.0f / vref : 0.0f;
+                h8 pf[PARTS][4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    if constexpr (F32) {
+                        const float to_v = fv[q] * vone * 16384.0f;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float x = st[q / 2][(q % 2) * 8 + i];
+                            float p = __builtin_amdgcn_exp2f(x * fk[q] - ref);
+                            if (!open && !seen(q / 2, (q % 2) * 8 + i)) p = 0.0f;
+                            l += p;
+                            const float y = p == 0.0f ? 0.0f : p * to_v;
+                            const _Float16 hi = static_cast<_Float16>(y);
+                            pf[0][q][i] = hi;
+                            pf[1][q][i] = static_cast<_Float16>(y - static_cast<float>(hi));
+                        }
+                    } else {
+                        const float ratio = fv[q] == 0.0f || vref == 0.0f ? 1.0f : fv[q] * vone;
+                        const float shift = __builtin_amdgcn_logf(ratio) + (kBase - ref);
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 8; i += 2) {
+                            float x[2];
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[q / 2][(q % 2) * 8 + i + j], fk[q], shift));
+                                if (!open && !seen(q / 2, (q % 2) * 8 + i + j)) x[j] = 0.0f;
+                            }
+                            const h2 y = {static_cast<_Float16>(x[0]), static_cast<_Float16>(x[1])};
+                            pf[0][q][i] = y[0];
+                            pf[0][q][i + 1] = y[1];
+                            const h2 ones = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
+                            sum = __builtin_amdgcn_fdot2(y, ones, sum, false);
+                        }
+                        l += sum * (0x1p-10f / ratio);
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const h8 vf = vbuf[half][t][q][lane];
+#pragma unroll
+                        for (int x = 0; x < PARTS; ++x)
+                            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[x][q], o[t], 0, 0, 0);
+                    }
+            }
+            if (un + 1 < last) convert((un + 1) & 1, vs_next);
+            __syncthreads();
+            id = id_next;
+            id_next = id_after;
+            ks = ks_next;
+            vs = vs_next;
+        }
+
+        // o[t][i] is dimension (8 (i / 4) + 4 g + i % 4) * NT + t of this lane's column.
+        l += __shfl_xor(l, 32);
+        const float unit_v = vref * (F32 ? 0x1p-14f : 0x1p-10f);
+        if (mine) {
+            if (first == 0 && last == units) {
+                const float f = l != 0.0f ? unit_v / l : 0.0f;
+                const int64_t to = static_cast<int64_t>(s.row0 + row) * a.ldo + static_cast<int64_t>(qhead) * hd;
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        const int d = (8 * (i / 4) + 4 * g + i % 4) * NT + t;
+                        if (d < hd) put<QT>(a.out, to + d, l != 0.0f ? o[t][i] * f : 0.0f);
+                    }
+            } else {
+                float* part = part_at(a, me, first == 0, HD) + c * (HD + 2);
+                if (g == 0) part[0] = m, part[1] = l;
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+                        part[2 + (8 * (i / 4) + 4 * g + i % 4) * NT + t] = o[t][i] * unit_v;
+            }
+        }
+        at.u += last - first;
+        if (at.u < at.u_end) at.next(a);
+    }
+}
+// Joins the parts of the items that more than one workgroup took, in workgroup
+// order.  Workgroup w here looks at the border before workgroup w + 1 of the
+// other kernel: if it is the first one inside an item, the item's columns
+// [y * kJoinCols, (y + 1) * kJoinCols) are its to join.
+constexpr int kJoinCols = 16;
+
+template <int QT, int HD, bool BIG>
+__global__ __launch_bounds__(kThreads) void join_q8_kernel(Q8Args a, int grid) {
+    const int w1 = blockIdx.x + 1;
+    int64_t total;
+    Place<BIG> p;
+    if (!p.find(a, w1, &grid, &total, [&](int64_t n, int g) { return (w1 < g ? w1 : 0) * n / g; })) return;
+    const int64_t u0 = p.u - p.unit;  // the item's first unit
+    if (p.unit == 0 || (w1 - 1) * total / grid > u0) return;
+    // the workgroup of the item's last unit
+    const int w_end = static_cast<int>(((u0 + p.units) * grid - 1) / total);
+    const Seq<BIG> s(a, p.seq);
+    const int col0 = p.tile * Seq<BIG>::COLS;
+    const int left = s.rows * a.group - col0;
+    const int c0 = blockIdx.y * kJoinCols;
+    int c1 = c0 + kJoinCols < left ? c0 + kJoinCols : left;
+    if (c1 > Seq<BIG>::COLS) c1 = Seq<BIG>::COLS;
+    const int hd = a.head_dim;
+    constexpr int AHEAD = 8;  // parts whose loads are in flight together
+    for (int x = c0 * HD + threadIdx.x; x < c1 * HD; x += kThreads) {
         const int c = x / HD, d = x % HD;
-        float top = -__builtin_inff();
-        for (int w = w0; w <= w1; ++w) top = fmaxf(top, part(w)[c * (HD + 2)]);
-        const float ref = top == -__builtin_inff() ? 0.0f : top;
-        float sum = 0.0f, val = 0.0f;
-        for (int w = w0; w <= w1; ++w) {
-            const float* p = part(w) + c * (HD + 2);
-            const float f = __builtin_amdgcn_exp2f(p[0] - ref);
-            sum += f * p[1];
-            val += f * p[2 + d];
+        float top = -__builtin_inff(), sum = 0.0f, val = 0.0f;
+        for (int w = w1 - 1; w <= w_end; w += AHEAD) {
+            float m[AHEAD], l[AHEAD], v[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const int ww = w + i <= w_end ? w + i : w_end;
+                const float* part = part_at(a, ww, ww == w1 - 1, HD) + c * (HD + 2);
+                m[i] = part[0];
+                l[i] = part[1];
+                v[i] = part[2 + d];
+            }
+            float most = top;
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) most = fmaxf(most, m[i]);
+            const float ref = most == -__builtin_inff() ? 0.0f : most;
+            const float f0 = __builtin_amdgcn_exp2f(top - ref);
+            sum *= f0;
+            val *= f0;
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                if (w + i > w_end) break;
+                const float f = __builtin_amdgcn_exp2f(m[i] - ref);
+                sum += f * l[i];
+                val += f * v[i];
+            }
+            top = most;
         }
         if (d < hd) {
-            const int cc = tile * kCols + c;
-            const int64_t to = static_cast<int64_t>(s.row0 + cc / a.group) * a.ldo +
-                               static_cast<int64_t>(head * a.group + cc % a.group) * hd + d;
-            const float res = sum != 0.0f ? val / sum : 0.0f;
-            if constexpr (QT == FENCE_F32) static_cast<float*>(a.out)[to] = res;
-            else static_cast<uint16_t*>(a.out)[to] = f32_to_f16_bits(res);
+            const int cc = col0 + c;
+            put<QT>(a.out,
+                    static_cast<int64_t>(s.row0 + cc / a.group) * a.ldo +
+                        static_cast<int64_t>(p.head * a.group + cc % a.group) * hd + d,
+                    sum != 0.0f ? val / sum : 0.0f);
         }
     }
 }
 
 int padded(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 
-int part_cols(int max_q_len, int group) {
-    return static_cast<int64_t>(max_q_len) * group < kCols ? max_q_len * group : kCols;
+bool big(int max_q_len, int group) { return static_cast<int64_t>(max_q_len) * group > kSmall; }
+
+int part_cols(int max_q_len, int group, bool is_big) {
+    const int64_t most = is_big ? kBigCols : kCols, n = static_cast<int64_t>(max_q_len) * group;
+    return static_cast<int>(n < most ? n : most);
+}
+
+// Floats of the parts that the workgroups of one kernel may leave.
+int64_t part_floats(int max_q_len, int group, int head_dim, bool is_big) {
+    return static_cast<int64_t>(is_big ? kBigGrid : kGrid) * 2 * part_cols(max_q_len, group, is_big) *
+           (padded(head_dim) + 2);
+}
+
+// Workgroups for at most `units` of work.
+unsigned grid_for(int64_t tiles, int64_t heads, int64_t positions, int unit, int batch, int most) {
+    const int64_t deep = (positions + unit - 1) / unit;
+    const int64_t each = tiles * heads > most ? most : tiles * heads * deep;
+    return static_cast<unsigned>(each > most / batch ? most : each * batch);
 }
 
 template <int TYPE, int QT, int HD>
-int attention_launch(const Q8Args& a, hipStream_t s) {
-    const int64_t tiles = (static_cast<int64_t>(a.max_q_len) * a.group + kCols - 1) / kCols;
-    const int64_t deep = (static_cast<int64_t>(a.max_blocks) << a.page_shift) + kUnit - 1;
-    const int64_t most = tiles * a.n_kv_heads * (deep / kUnit);
-    const int64_t grid = most > kMaxGrid / a.batch ? kMaxGrid : most * a.batch;
+int attention_launch(Q8Args a, hipStream_t s) {
+    const bool both = big(a.max_q_len, a.group);
+    const int64_t columns = static_cast<int64_t>(a.max_q_len) * a.group;
+    const int64_t positions = static_cast<int64_t>(a.max_blocks) << a.page_shift;
+    if (both) {
+        a.part_cols = part_cols(a.max_q_len, a.group, true);
+        const unsigned grid =
+            grid_for((columns + kBigCols - 1) / kBigCols, a.n_kv_heads, positions, kBigUnit, a.batch, kBigGrid);
+        if (const int st = launch(prompt_q8_kernel<TYPE, QT, HD>, dim3(grid), dim3(kThreads), 0, s, a)) return st;
+        if (grid > 1)
+            if (const int st = launch(join_q8_kernel<QT, HD, true>, dim3(grid - 1, (a.part_cols + kJoinCols - 1) / kJoinCols),
+                                      dim3(kThreads), 0, s, a, static_cast<int>(grid)))
+                return st;
+        a.ws += part_floats(a.max_q_len, a.group, a.head_dim, true);
+    }
+    const int64_t small = columns < kSmall ? columns : kSmall;
+    a.part_cols = part_cols(a.max_q_len, a.group, false);
+    const unsigned grid = grid_for((small + kCols - 1) / kCols, a.n_kv_heads, positions, kUnit, a.batch, kGrid);
     const size_t shmem = static_cast<size_t>(kWaves) * a.part_cols * (HD + 2) * sizeof(float);
-    if (const int st = launch(attention_q8_kernel<TYPE, QT, HD>, dim3(static_cast<unsigned>(grid)), dim3(kThreads),
-                              shmem, s, a))
-        return st;
-    if (deep / kUnit * grid == 0) return FENCE_SUCCESS;
-    return launch(attention_q8_merge_kernel<QT, HD>, dim3(static_cast<unsigned>(tiles * a.n_kv_heads), a.batch),
-                  dim3(kThreads), 0, s, a, static_cast<int>(grid));
+    if (const int st = launch(attention_q8_kernel<TYPE, QT, HD>, dim3(grid), dim3(kThreads), shmem, s, a)) return st;
+    if (grid == 1) return FENCE_SUCCESS;
+    return launch(join_q8_kernel<QT, HD, false>, dim3(grid - 1), dim3(kThreads), 0, s, a, static_cast<int>(grid));
 }
 
 template <int TYPE, int QT>
@@ -549,8 +982,9 @@ extern "C" int64_t fence_gqa_attention_q8_workspace(int batch, int max_q_len, in
     if (batch < 0 || max_q_len < 0 || n_q_heads < 1 || n_kv_heads < 1 || n_q_heads % n_kv_heads || head_dim < 16 ||
         head_dim > 256 || head_dim % 16)
         return 0;
-    const int64_t bytes = static_cast<int64_t>(kMaxGrid) * 2 * part_cols(max_q_len, n_q_heads / n_kv_heads) *
-                          (padded(head_dim) + 2) * 4;
+    const int group = n_q_heads / n_kv_heads;
+    int64_t bytes = 4 * part_floats(max_q_len, group, head_dim, false);
+    if (big(max_q_len, group)) bytes += 4 * part_floats(max_q_len, group, head_dim, true);
     return bytes < 16 ? 16 : bytes;
 }
 
@@ -585,7 +1019,7 @@ extern "C" int fence_gqa_attention_q8(void* out, const void* q, int type, int64_
     const Q8Args a{out, q, ldq, ldo, static_cast<const uint8_t*>(cache->k), static_cast<const uint8_t*>(cache->v),
                    cache->k_scale, cache->v_scale, block_table, kv_lens, q_start, static_cast<float*>(workspace),
                    cache->n_pages, __builtin_ctz(cache->page_size), cache->n_kv_heads, cache->head_dim, group,
-                   max_blocks, batch, max_q_len, part_cols(max_q_len, group),
+                   max_blocks, batch, max_q_len, 0,
                    static_cast<float>(scale * 1.4426950408889634)};
     if (cache->type == FENCE_KV_INT8)
         return type == FENCE_F32 ? attention_hd<FENCE_KV_INT8, FENCE_F32>(a, stream)
