@@ -60,153 +60,241 @@ struct Q8Args {
     float scale_log2;
 };
 
+// Read-only data at addresses that are the same in every lane, through the
+// scalar cache: it does not queue behind the codes that are being loaded.
+template <class T>
+__device__ __forceinline__ T uniform_load(const T* p, int64_t i) {
+    return reinterpret_cast<const __attribute__((address_space(4))) T*>(reinterpret_cast<uintptr_t>(p))[i];
+}
+
 // A sequence as one of the two kernels sees it: rows = 0 if it is the other's.
+// Its work is counted in units, COLS columns of one kv head by UNIT positions.
 template <bool BIG>
 struct Seq {
     static constexpr int COLS = BIG ? kBigCols : kCols;
     static constexpr int UNIT = BIG ? kBigUnit : kUnit;
-    int row0, rows, q_len, kv;  // first row, rows computed, rows there are, positions
+    int row0, rows, q_len, kv, group;  // first row, rows computed, rows there are, positions
 
-    __device__ __forceinline__ Seq(const Q8Args& a, int b) {
-        row0 = a.q_start[b];
-        const int n = a.q_start[b + 1] - row0;
-        q_len = n < 0 ? 0 : n;
+    __device__ __forceinline__ Seq(const Q8Args& a, int row, int row_end, int len) : row0(row), group(a.group) {
+        q_len = row_end > row ? row_end - row : 0;
         rows = q_len < a.max_q_len ? q_len : a.max_q_len;
-        if ((rows * a.group > kSmall) != BIG) rows = 0;
+        if ((rows * group > kSmall) != BIG) rows = 0;
         const int cap = a.max_blocks << a.page_shift;
-        const int len = a.kv_lens[b];
         kv = len < 0 ? 0 : len > cap ? cap : len;
     }
-    __device__ __forceinline__ int tiles(int group) const { return (rows * group + COLS - 1) / COLS; }
+    // of the same index in every lane
+    static __device__ __forceinline__ Seq uniform(const Q8Args& a, int b) {
+        return Seq(a, uniform_load(a.q_start, b), uniform_load(a.q_start, b + 1), uniform_load(a.kv_lens, b));
+    }
+    __device__ __forceinline__ int tiles() const { return (rows * group + COLS - 1) / COLS; }
     // positions that row i sees, i at most q_len - 1
     __device__ __forceinline__ int row_sees(int i) const {
         const int n = kv - q_len + i + 1;
         return n < 0 ? 0 : n;
     }
     // positions that the last column of a tile sees
-    __device__ __forceinline__ int sees(int tile, int group) const {
+    __device__ __forceinline__ int sees(int tile) const {
         const int i = (tile * COLS + COLS - 1) / group;
         return row_sees(i < q_len - 1 ? i : q_len - 1);
     }
     // units of one kv head's tile: one at least, which writes the zeros of rows that see nothing
-    __device__ __forceinline__ int units(int tile, int group) const {
-        const int n = (sees(tile, group) + UNIT - 1) / UNIT;
-        return n < 1 ? 1 : n;
+    __device__ __forceinline__ int units(int tile) const {
+        const int n = sees(tile);
+        return n > UNIT ? (n + UNIT - 1) / UNIT : 1;
     }
-    // f(tile, units) for every tile until it returns false
-    template <class F>
-    __device__ __forceinline__ void each_tile(int group, F f) const {
-        const int n = tiles(group), whole = COLS / group, part = COLS % group;
-        int i = (COLS - 1) / group, over = (COLS - 1) % group;  // sees() without its division
-        for (int t = 0; t < n; ++t) {
-            const int sees = row_sees(i < q_len - 1 ? i : q_len - 1);
-            if (!f(t, sees > UNIT ? (sees + UNIT - 1) / UNIT : 1)) return;
-            i += whole;
-            over += part;
-            if (over >= group) over -= group, ++i;
+    // What a tile of one kv head costs and what the tiles before it do, for the even split.  Few tiles: their
+    // units.  Many: about the positions that its columns see, a linear function of the tile, so that the sum
+    // needs no loop over the tiles.
+    __device__ __forceinline__ int64_t slope() const {
+        const int64_t n = static_cast<int64_t>(kv) - q_len + 1;
+        return (n < 1 ? 1 : n) * group - 1;
+    }
+    __device__ __forceinline__ int64_t cost(int tile) const {
+        if constexpr (!BIG) return units(tile);
+        else return slope() + static_cast<int64_t>(COLS) * (tile + 1);
+    }
+    __device__ __forceinline__ int64_t before(int tile) const {
+        if constexpr (!BIG) {
+            int64_t n = 0;
+            for (int t = 0; t < tile; ++t) n += units(t);
+            return n;
+        } else {
+            return slope() * tile + static_cast<int64_t>(COLS) * (static_cast<int64_t>(tile) * (tile + 1) / 2);
         }
     }
-    // of all kv heads and tiles
-    __device__ __forceinline__ int64_t all_units(const Q8Args& a) const {
-        int64_t n = 0;
-        each_tile(a.group, [&](int, int u) { return n += u, true; });
-        return n * a.n_kv_heads;
-    }
+    __device__ __forceinline__ int64_t all(const Q8Args& a) const { return before(tiles()) * a.n_kv_heads; }
 };
 
-// Prefix sums of the sequences' units over the workgroup: the total, and the
-// sequence that unit `find(total)` belongs to with the units before it.
-template <bool BIG, class F>
-__device__ __forceinline__ int64_t locate(const Q8Args& a, F find, int* seq, int64_t* before) {
+// 64-bit inclusive sum over a wave.
+__device__ __forceinline__ int64_t wave_scan(int64_t v) {
+    const int lane = threadIdx.x % kWave;
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+        const int64_t up = __shfl_up(v, d);
+        if (lane >= d) v += up;
+    }
+    return v;
+}
+
+// x / y rounded down for numbers below 2^53, where the quotient in 64-bit
+// floating point cannot be rounded up to a whole number it does not reach.
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
+    return static_cast<int64_t>(static_cast<double>(x) / static_cast<double>(y));
+}
+
+// Workgroups that share the work: none without any.
+__device__ __forceinline__ int sharers(int64_t total, int grid) {
+    return total < grid ? static_cast<int>(total) : grid;
+}
+
+// Where workgroup w begins, when `grid` of them share `total`.
+__device__ __forceinline__ int64_t cut(int w, int64_t total, int grid) { return quotient(w * total, grid); }
+
+// A place in the work, in the order of sequences, tiles, kv heads and units.
+// An item is a sequence's tile of one kv head.
+struct Place {
+    int seq, tile, head, unit, units;
+    int64_t item, cost;  // where the item begins, and what it costs
+};
+
+// The place of each of N points at(i, total, grid) < total, by sums over the
+// batch, and the total; grid becomes the number of sharers.  Returns false
+// if there is no work or at(0, ..) is negative.
+template <bool BIG, int N, class F>
+__device__ __forceinline__ bool find(const Q8Args& a, int* grid, int64_t* total, Place (&p)[N], F at) {
     __shared__ int64_t waves[kWaves];
-    __shared__ int64_t found_before;
-    __shared__ int found;
+    __shared__ int64_t found_before[N];
+    __shared__ int found[N];
     const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-    int64_t total = 0, mine = 0;
-    for (int pass = 0; pass < 2; ++pass) {
-        int64_t at = 0;
-        const int64_t target = pass ? find(total) : -1;
-        for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
-            if (!pass || a.batch > kThreads) mine = b0 + tid < a.batch ? Seq<BIG>(a, b0 + tid).all_units(a) : 0;
-            int64_t v = mine;
+    int64_t point[N], before[N];
+    const auto all_of = [&](int b) {
+        return b < a.batch ? Seq<BIG>(a, a.q_start[b], a.q_start[b + 1], a.kv_lens[b]).all(a) : 0;
+    };
+    const auto points = [&]() {
+        *grid = sharers(*total, *grid);
+        if (*grid == 0) return false;
 #pragma unroll
-            for (int d = 1; d < kWave; d *= 2) {
-                const int64_t up = __shfl_up(v, d);
-                if (lane >= d) v += up;
-            }
-            __syncthreads();
-            if (lane == kWave - 1) waves[wave] = v;
-            __syncthreads();
-            int64_t pre = at;
+        for (int i = 0; i < N; ++i) point[i] = at(i, *total, *grid);
+        return point[0] >= 0;
+    };
+    if (a.batch == 1) {
+        *total = Seq<BIG>::uniform(a, 0).all(a);
+        if (!points()) return false;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
-                if (w < wave) pre += waves[w];
-                at += waves[w];
+        for (int i = 0; i < N; ++i) p[i].seq = 0, before[i] = 0;
+    } else if (a.batch <= kWave) {  // every wave for itself
+        const int64_t mine = all_of(lane);
+        const int64_t upto = wave_scan(mine);
+        *total = __shfl(upto, kWave - 1);
+        if (!points()) return false;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int l = __builtin_ctzll(__ballot(upto > point[i]));
+            p[i].seq = l;
+            before[i] = __shfl(upto - mine, l);
+        }
+    } else {
+        int64_t sum = 0;
+        for (int pass = 0; pass < 2; ++pass) {
+            if (pass) {
+                *total = sum;
+                if (!points()) return false;
+                sum = 0;
             }
-            if (pass && pre + v > target && pre + v - mine <= target) {
-                found = b0 + tid;
-                found_before = pre + v - mine;
+            for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
+                const int64_t mine = all_of(b0 + tid);
+                const int64_t upto = wave_scan(mine);
+                __syncthreads();
+                if (lane == kWave - 1) waves[wave] = upto;
+                __syncthreads();
+                int64_t pre = sum;
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) {
+                    if (w < wave) pre += waves[w];
+                    sum += waves[w];
+                }
+                if (pass) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+                        if (pre + upto > point[i] && pre + upto - mine <= point[i])
+                            found[i] = b0 + tid, found_before[i] = pre + upto - mine;
+                }
             }
         }
-        total = at;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) p[i].seq = found[i], before[i] = found_before[i];
     }
-    __syncthreads();
-    *seq = __builtin_amdgcn_readfirstlane(found);
-    *before = found_before;
-    return total;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        p[i].seq = __builtin_amdgcn_readfirstlane(p[i].seq);
+        const Seq<BIG> s = Seq<BIG>::uniform(a, p[i].seq);
+        const int64_t rest = point[i] - before[i];
+        int lo = 0, hi = s.tiles() - 1;  // the last tile that begins at or before it
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (s.before(mid) * a.n_kv_heads <= rest) lo = mid;
+            else hi = mid - 1;
+        }
+        p[i].tile = __builtin_amdgcn_readfirstlane(lo);
+        p[i].units = s.units(lo);
+        p[i].cost = s.cost(lo);
+        const int64_t in_tile = rest - s.before(lo) * a.n_kv_heads;
+        p[i].head = __builtin_amdgcn_readfirstlane(static_cast<int>(quotient(in_tile, p[i].cost)));
+        const int64_t off = in_tile - p[i].head * p[i].cost;
+        p[i].item = point[i] - off;
+        const int unit = BIG ? static_cast<int>(quotient(off * p[i].units, p[i].cost)) : static_cast<int>(off);
+        p[i].unit = __builtin_amdgcn_readfirstlane(unit);
+    }
+    return true;
 }
 
-// Workgroups that get units: every one of them at least one, so that each
-// workgroup between an item's first and last has a part of it.
-__device__ __forceinline__ int sharers(int64_t total, int grid) {
-    return total < 1 ? 1 : total < grid ? static_cast<int>(total) : grid;
-}
-
-// A workgroup's place in the units, in the order of sequences, tiles, kv heads
-// and positions.
+// A workgroup's share: from one place to another.
 template <bool BIG>
-struct Place {
-    int64_t u, u_end;
-    int seq, tile, head, unit, units;
+struct Share {
+    Place p;
+    int end_seq, end_tile, end_head, end_unit;
 
-    // Of unit `at(total, grid)`; false if there is none for this workgroup.
-    template <class F>
-    __device__ __forceinline__ bool find(const Q8Args& a, int me, int* grid, int64_t* total, F at) {
-        int64_t before;
-        *total = locate<BIG>(a, [&](int64_t n) { return at(n, sharers(n, *grid)); }, &seq, &before);
-        *grid = sharers(*total, *grid);
-        if (me >= *grid || *total == 0) return false;
-        u = at(*total, *grid);
-        const Seq<BIG> s(a, seq);
-        int64_t rest = u - before;
-        s.each_tile(a.group, [&](int t, int n) {
-            tile = t;
-            units = n;
-            if (rest < static_cast<int64_t>(n) * a.n_kv_heads) return false;
-            rest -= static_cast<int64_t>(n) * a.n_kv_heads;
-            return true;
-        });
-        head = static_cast<int>(rest / units);
-        unit = static_cast<int>(rest % units);
-        seq = __builtin_amdgcn_readfirstlane(seq);
-        tile = __builtin_amdgcn_readfirstlane(tile);
-        head = __builtin_amdgcn_readfirstlane(head);
-        unit = __builtin_amdgcn_readfirstlane(unit);
-        units = __builtin_amdgcn_readfirstlane(units);
+    __device__ __forceinline__ bool find_mine(const Q8Args& a) {
+        const int me = blockIdx.x;
+        int grid = gridDim.x;
+        int64_t total;
+        Place ends[2];
+        // the last place is in front of the next workgroup's first; the last workgroup's is the end of all
+        bool to_end = false;
+        if (!find<BIG, 2>(a, &grid, &total, ends, [&](int i, int64_t n, int g) -> int64_t {
+                if (me >= g) return -1;
+                if (i == 0) return cut(me, n, g);
+                to_end = me + 1 == g;
+                return to_end ? n - 1 : cut(me + 1, n, g);
+            }))
+            return false;
+        p = ends[0];
+        end_seq = ends[1].seq;
+        end_tile = ends[1].tile;
+        end_head = ends[1].head;
+        end_unit = to_end ? ends[1].units : ends[1].unit;
         return true;
     }
-    // Past the item (a sequence's tile and kv head); u < u_end says that there is another one.
-    __device__ __forceinline__ void next(const Q8Args& a) {
-        unit = 0;
-        if (++head < a.n_kv_heads) return;
-        head = 0;
-        Seq<BIG> s(a, seq);
-        if (++tile == s.tiles(a.group)) {
-            tile = 0;
-            do s = Seq<BIG>(a, ++seq);
-            while (s.rows == 0);
+    // the end of this workgroup's units of the item p is in
+    __device__ __forceinline__ bool in_last() const {
+        return p.seq == end_seq && p.tile == end_tile && p.head == end_head;
+    }
+    __device__ __forceinline__ int last() const { return in_last() ? end_unit : p.units; }
+    // To the next item; false past the end of the share.
+    __device__ __forceinline__ bool next(const Q8Args& a) {
+        if (in_last()) return false;
+        p.unit = 0;
+        if (++p.head < a.n_kv_heads) return true;
+        p.head = 0;
+        Seq<BIG> s = Seq<BIG>::uniform(a, p.seq);
+        if (++p.tile == s.tiles()) {
+            p.tile = 0;
+            do s = Seq<BIG>::uniform(a, ++p.seq);
+            while (s.rows == 0);  // the end lies in a sequence behind
         }
-        units = s.units(tile, a.group);
+        p.units = s.units(p.tile);
+        return true;
     }
 };
 
@@ -215,6 +303,16 @@ struct Place {
 // the running maximum, the sum and the unnormalised output.
 __device__ __forceinline__ float* part_at(const Q8Args& a, int wg, bool begins, int hd) {
     return a.ws + static_cast<int64_t>(wg * 2 + (begins ? 1 : 0)) * a.part_cols * (hd + 2);
+}
+
+// y as the sum of two binary16 numbers, 22 bits of it.  The empty asm makes y
+// one fp32 value: otherwise the product that it came from may be rounded to
+// binary16 a second time, unrounded, and next to a tie that gives another
+// first number than the one the second number completes.
+__device__ __forceinline__ void split(float y, _Float16* hi, _Float16* lo) {
+    asm volatile("" : "+v"(y));
+    *hi = static_cast<_Float16>(y);
+    *lo = static_cast<_Float16>(y - static_cast<float>(*hi));
 }
 
 template <int QT>
@@ -250,19 +348,20 @@ __device__ __forceinline__ float across_rows(float v, Op op) {
     return op(v, __shfl_xor(v, 32));
 }
 
-// One workgroup's share of the units.  A wave multiplies 32 positions (two
-// groups of 16, each inside one page) by 16 columns at a time:
+// Single tokens and drafts.  A wave multiplies 32 positions (two groups of 16,
+// each inside one page) by 16 columns at a time:
 //   S' [16 positions x 16 columns] = K [16 x HD] Q' [HD x 16]
 //   O' [HD x 16 columns] += V' [HD x 32 positions] P [32 x 16]
 // The first product leaves lane (column r, row group g) with the positions
 // 4 g .. 4 g + 3 of each group of 16, and those eight are what the second
 // product takes from it as its k index, so P stays where it is.  A lane's
 // dimensions are r * HD / 16 + i for product i, so it reads V with one load a
-// position.
+// position.  The next positions' codes are loaded before these are used.
 template <int TYPE, int QT, int HD>
-__global__ __launch_bounds__(kThreads) void attention_q8_kernel(Q8Args a) {
+__global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void attention_q8_kernel(Q8Args a) {
     constexpr int PIECES = HD / 64;       // 64 dimensions of K: 16 a lane
     constexpr int DT = HD / 16;           // products over V; also dimensions a lane reads of a position
+    constexpr int VW = DT / 4;            // words of them
     constexpr bool F32 = QT == FENCE_F32;
     constexpr int PARTS = F32 ? 2 : 1;    // binary16 numbers that hold a q or a p
     extern __shared__ float lds[];
@@ -271,17 +370,13 @@ __global__ __launch_bounds__(kThreads) void attention_q8_kernel(Q8Args a) {
     const int r = lane % 16, g = lane / 16;
     const int hd = a.head_dim, page_mask = (1 << a.page_shift) - 1;
 
-    const int me = blockIdx.x;
-    int grid = gridDim.x;
-    int64_t total;
-    Place<false> at_;
-    if (!at_.find(a, me, &grid, &total, [&](int64_t n, int g) { return me * n / g; })) return;
-    at_.u_end = (me + 1) * total / grid;
-
-    while (at_.u < at_.u_end) {
-        const Seq<false> s(a, at_.seq);
-        const int tile = at_.tile, head = at_.head, first = at_.unit, units = at_.units;
-        const int last = at_.u_end - at_.u < units - first ? first + static_cast<int>(at_.u_end - at_.u) : units;
+    Share<false> share;
+    if (!share.find_mine(a)) return;
+    do {
+        const Seq<false> s = Seq<false>::uniform(a, share.p.seq);
+        const int tile = share.p.tile, head = share.p.head, first = share.p.unit, units = share.p.units;
+        const int last = share.last();
+        if (first >= last) continue;  // a share has at least one unit, but its end may be an item's beginning
         const int cols = s.rows * a.group - tile * kCols < kCols ? s.rows * a.group - tile * kCols : kCols;
         // this lane's column
         const int col = tile * kCols + r;
@@ -289,7 +384,52 @@ __global__ __launch_bounds__(kThreads) void attention_q8_kernel(Q8Args a) {
         const bool mine = r < cols;
         const int qhead = head * a.group + col % a.group;
         const int sees = mine ? s.row_sees(row) : 0;
-        const int end = s.sees(tile, a.group);
+        const int end = s.sees(tile);
+        const int least = s.row_sees(tile * kCols / a.group);  // what every column sees
+
+        // The codes of 32 positions; none of those that are not there.
+        struct Codes {
+            u4 k[2][PIECES];
+            uint32_t v[8][VW];
+            float ks[2], vs[2];
+            bool ok[2];  // the page is there
+        };
+        const int64_t table = static_cast<int64_t>(share.p.seq) * a.max_blocks;
+        const auto page_of = [&](int un, int t) {
+            const int pos = un * kUnit + wave * 32 + 16 * t;
+            return un < last && pos < end ? uniform_load(a.table, table + (pos >> a.page_shift)) : -1;
+        };
+        const auto load = [&](Codes& c, int un, const int (&ids)[2]) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int pos = un * kUnit + wave * 32 + 16 * t;
+                c.ok[t] = ids[t] >= 0 && ids[t] < a.n_pages;
+                const int64_t base = static_cast<int64_t>(c.ok[t] ? ids[t] : 0) * a.n_kv_heads + head;
+                c.ks[t] = c.ok[t] ? uniform_load(a.ks, base) : 0.0f;
+                c.vs[t] = c.ok[t] ? uniform_load(a.vs, base) : 0.0f;
+                const int64_t at = ((base << a.page_shift) + (pos & page_mask)) * hd;
+                const uint8_t* k = a.k + at + r * hd;
+                const uint8_t* v = a.v + at + g * 4 * hd + r * DT;
+#pragma unroll
+                for (int p = 0; p < PIECES; ++p) {
+                    const int d = p * 64 + g * 16;
+                    c.k[t][p] = u4{0, 0, 0, 0};
+                    if (c.ok[t] && d < hd) c.k[t][p] = *reinterpret_cast<const u4*>(k + d);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) c.v[4 * t + i][w] = 0;
+                    if (c.ok[t] && pos + g * 4 + i < end && r * DT < hd) {
+#pragma unroll
+                        for (int w = 0; w < VW; ++w) c.v[4 * t + i][w] = reinterpret_cast<const uint32_t*>(v + i * hd)[w];
+                    }
+                }
+            }
+        };
+        int ids[2] = {page_of(first, 0), page_of(first, 1)};
+        Codes now, then;
+        load(now, first, ids);
 
         h8 qf[PARTS][PIECES][2];
         float unscale = a.scale_log2;
@@ -322,10 +462,10 @@ __global__ __launch_bounds__(kThreads) void attention_q8_kernel(Q8Args a) {
                 for (int p = 0; p < PIECES; ++p)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float y = x[p][i] * up;
-                        const _Float16 hi = static_cast<_Float16>(y);
+                        _Float16 hi, lo;
+                        split(x[p][i] * up, &hi, &lo);
                         qf[0][p][i / 8][i % 8] = hi;
-                        qf[1][p][i / 8][i % 8] = static_cast<_Float16>(y - static_cast<float>(hi));
+                        qf[1][p][i / 8][i % 8] = lo;
                     }
             } else {
 #pragma unroll
@@ -351,39 +491,9 @@ __global__ __launch_bounds__(kThreads) void attention_q8_kernel(Q8Args a) {
         float m = -__builtin_inff(), l = 0.0f;
         float vref = 0.0f;  // the largest V scale so far: o is in units of it times 2^-14
 
-        const int32_t* row_of_table = a.table + static_cast<int64_t>(at_.seq) * a.max_blocks;
-        for (int un = first; un < last; ++un) {
-            const int pos0 = un * kUnit + wave * 32;
-            if (pos0 >= end) break;
+        const auto turn = [&](const Codes& c, int pos0, auto masked) {
             f4 st[2];
-            uint32_t vw[8][(DT + 3) / 4];
-            float vscale[2], kscale[2];
-            bool bad[2];
-            u4 kw[2][PIECES];
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                const int pos = pos0 + 16 * t;
-                const int id = pos < end ? row_of_table[pos >> a.page_shift] : -1;
-                bad[t] = id < 0 || id >= a.n_pages;
-                const int64_t base = static_cast<int64_t>(bad[t] ? 0 : id) * a.n_kv_heads + head;
-                kscale[t] = bad[t] ? 0.0f : a.ks[base];
-                vscale[t] = bad[t] ? 0.0f : a.vs[base];
-                const int64_t at = ((base << a.page_shift) + (pos & page_mask)) * hd;
-#pragma unroll
-                for (int p = 0; p < PIECES; ++p) {
-                    const int d = p * 64 + g * 16;
-                    kw[t][p] = u4{0, 0, 0, 0};
-                    if (!bad[t] && d < hd) kw[t][p] = *reinterpret_cast<const u4*>(a.k + at + r * hd + d);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bool there = !bad[t] && pos + g * 4 + i < end && r * DT < hd;
-                    const uint8_t* src = a.v + at + (g * 4 + i) * hd + r * DT;
-#pragma unroll
-                    for (int w = 0; w < DT / 4; ++w)
-                        vw[4 * t + i][w] = there ? reinterpret_cast<const uint32_t*>(src)[w] : 0;
-                }
-            }
+            float top = m;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -392,68 +502,88 @@ __global__ __launch_bounds__(kThreads) void attention_q8_kernel(Q8Args a) {
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         h2 c0, c1, c2, c3;
-                        codes_h<TYPE>(kw[t][p][2 * j], &c0, &c1);
-                        codes_h<TYPE>(kw[t][p][2 * j + 1], &c2, &c3);
+                        codes_h<TYPE>(c.k[t][p][2 * j], &c0, &c1);
+                        codes_h<TYPE>(c.k[t][p][2 * j + 1], &c2, &c3);
                         const h8 kf = join(c0, c1, c2, c3);
 #pragma unroll
                         for (int x = 0; x < PARTS; ++x)
                             acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[x][p][j], acc, 0, 0, 0);
                     }
-                const float f = kscale[t] * unscale;
+                const float f = c.ks[t] * unscale;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int pos = pos0 + 16 * t + g * 4 + i;
-                    st[t][i] = bad[t] || pos >= sees ? -__builtin_inff() : acc[i] * f;
+                    st[t][i] = acc[i] * f;
+                    if (!c.ok[t] || (masked && pos0 + 16 * t + g * 4 + i >= sees)) st[t][i] = -__builtin_inff();
+                    top = fmaxf(top, st[t][i]);
                 }
             }
-            float top = m;
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) top = fmaxf(top, st[t][i]);
             top = across_rows(top, OpMax{});
-            const float ref = top == -__builtin_inff() ? 0.0f : top;
             float vtop = vref;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
-                if (vscale[t] > vtop && vscale[t] < __builtin_inff()) vtop = vscale[t];
-            const float alpha = __builtin_amdgcn_exp2f(m - ref);  // m = -inf: 0
-            const float beta = vtop > 0.0f ? alpha * (vref / vtop) : 0.0f;
-            const float to_v = vtop > 0.0f ? 16384.0f / vtop : 0.0f;
-            m = top;
-            vref = vtop;
-            l *= alpha;
+                if (c.vs[t] > vtop && c.vs[t] < __builtin_inff()) vtop = c.vs[t];
+            if (__any(top > m) || vtop > vref) {
+                const float alpha = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+                const float beta = vtop > 0.0f ? alpha * (vref * __builtin_amdgcn_rcpf(vtop)) : 0.0f;
+                m = top;
+                vref = vtop;
+                l *= alpha;
+#pragma unroll
+                for (int i = 0; i < DT; ++i) o[i] *= beta;
+            }
+            const float ref = m == -__builtin_inff() ? 0.0f : m;
+            const float to_v = vref > 0.0f ? 16384.0f * __builtin_amdgcn_rcpf(vref) : 0.0f;
             h8 pf[PARTS];
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < 2; ++t) {
+                const float f = c.vs[t] * to_v;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float p = __builtin_amdgcn_exp2f(st[t][i] - ref);
                     l += p;
-                    const float y = st[t][i] == -__builtin_inff() ? 0.0f : p * (vscale[t] * to_v);
-                    const _Float16 hi = static_cast<_Float16>(y);
-                    pf[0][4 * t + i] = hi;
-                    if constexpr (F32) pf[1][4 * t + i] = static_cast<_Float16>(y - static_cast<float>(hi));
+                    float y = p * f;
+                    if (masked && p == 0.0f) y = 0.0f;  // behind a scale that is not finite
+                    if constexpr (F32) {
+                        _Float16 hi, lo;
+                        split(y, &hi, &lo);
+                        pf[0][4 * t + i] = hi;
+                        pf[1][4 * t + i] = lo;
+                    } else {
+                        pf[0][4 * t + i] = static_cast<_Float16>(y);
+                    }
                 }
+            }
 #pragma unroll
-            for (int i = 0; i < DT; ++i) o[i] *= beta;
-#pragma unroll
-            for (int w = 0; w < DT / 4; ++w) {
-                h2 c[4][4];  // [pair of positions][dimension of the word]
+            for (int w = 0; w < VW; ++w) {
+                h2 x[4][4];  // [pair of positions][dimension of the word]
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const uint32_t x = vw[2 * j][w], y = vw[2 * j + 1][w];
-                    codes_h<TYPE>(__builtin_amdgcn_perm(y, x, 0x05010400u), &c[j][0], &c[j][1]);
-                    codes_h<TYPE>(__builtin_amdgcn_perm(y, x, 0x07030602u), &c[j][2], &c[j][3]);
+                    const uint32_t y = c.v[2 * j][w], z = c.v[2 * j + 1][w];
+                    codes_h<TYPE>(__builtin_amdgcn_perm(z, y, 0x05010400u), &x[j][0], &x[j][1]);
+                    codes_h<TYPE>(__builtin_amdgcn_perm(z, y, 0x07030602u), &x[j][2], &x[j][3]);
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const h8 vf = join(c[0][i], c[1][i], c[2][i], c[3][i]);
+                    const h8 vf = join(x[0][i], x[1][i], x[2][i], x[3][i]);
 #pragma unroll
-                    for (int x = 0; x < PARTS; ++x)
-                        o[4 * w + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[x], o[4 * w + i], 0, 0, 0);
+                    for (int k = 0; k < PARTS; ++k)
+                        o[4 * w + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[k], o[4 * w + i], 0, 0, 0);
                 }
             }
+        };
+
+        ids[0] = page_of(first + 1, 0);
+        ids[1] = page_of(first + 1, 1);
+#pragma unroll 1
+        for (int un = first; un < last; ++un) {
+            const int pos0 = un * kUnit + wave * 32;
+            if (pos0 >= end) break;
+            load(then, un + 1, ids);
+            ids[0] = page_of(un + 2, 0);
+            ids[1] = page_of(un + 2, 1);
+            if (pos0 + 32 <= least) turn(now, pos0, std::false_type{});
+            else turn(now, pos0, std::true_type{});
+            now = then;
         }
 
         // The waves' parts together: lane (r, g) has dimensions (4 g + j) * DT + i of column r in o[i][j].
@@ -474,7 +604,7 @@ __global__ __launch_bounds__(kThreads) void attention_q8_kernel(Q8Args a) {
         }
         __syncthreads();
         const bool whole = first == 0 && last == units;
-        float* part = part_at(a, me, first == 0, HD);
+        float* part = part_at(a, blockIdx.x, first == 0, HD);
         for (int x = tid; x < cols * HD; x += kThreads) {
             const int c = x / HD, d = x % HD;
             float top = -__builtin_inff();
@@ -501,10 +631,7 @@ __global__ __launch_bounds__(kThreads) void attention_q8_kernel(Q8Args a) {
             }
         }
         __syncthreads();
-
-        at_.u += last - first;
-        if (at_.u < at_.u_end) at_.next(a);
-    }
+    } while (share.next(a));
 }
 
 // Prompts: a workgroup takes kBigCols columns, 32 a wave, and 64 positions at
@@ -545,32 +672,28 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
     const int n = lane % 32, g = lane / 32;
     const int hd = a.head_dim, page_mask = (1 << a.page_shift) - 1;
 
-    const int me = blockIdx.x;
-    int grid = gridDim.x;
-    int64_t total;
-    Place<true> at;
-    if (!at.find(a, me, &grid, &total, [&](int64_t units, int w) { return me * units / w; })) return;
-    at.u_end = (me + 1) * total / grid;
-
-    while (at.u < at.u_end) {
-        const Seq<true> s(a, at.seq);
-        const int tile = at.tile, head = at.head, first = at.unit, units = at.units;
-        const int last = at.u_end - at.u < units - first ? first + static_cast<int>(at.u_end - at.u) : units;
+    Share<true> share;
+    if (!share.find_mine(a)) return;
+    do {
+        const Seq<true> s = Seq<true>::uniform(a, share.p.seq);
+        const int tile = share.p.tile, head = share.p.head, first = share.p.unit, units = share.p.units;
+        const int last = share.last();
         const int cols = s.rows * a.group - tile * kBigCols;
         const int c = wave * 32 + n;  // this lane's column
         const bool mine = c < cols;
         const int row = (tile * kBigCols + c) / a.group;
         const int qhead = head * a.group + (tile * kBigCols + c) % a.group;
         const int sees = mine ? s.row_sees(row) : 0;
-        const int end = s.sees(tile, a.group);
-        // what every column of this wave sees, and what one of them sees at most
-        const int least = __builtin_amdgcn_readfirstlane(s.row_sees((tile * kBigCols + wave * 32) / a.group));
-        int most;
-        {
-            const int i = (tile * kBigCols + wave * 32 + 31) / a.group;
-            most = wave * 32 < cols ? s.row_sees(i < s.q_len - 1 ? i : s.q_len - 1) : 0;
-            most = __builtin_amdgcn_readfirstlane(most);
+        const int end = s.sees(tile);
+        if (first >= last) {
+            // Nothing of this item; if others take what is before and after, the join finds an empty part.
+            if (first > 0 && mine && g == 0) {
+                float* part = part_at(a, blockIdx.x, false, HD) + c * (HD + 2);
+                part[0] = -__builtin_inff(), part[1] = 0.0f;
+            }
+            continue;
         }
+        const int least = s.row_sees((tile * kBigCols + wave * 32) / a.group);  // what every column of this wave sees
 
         h8 qf[PARTS][KS];
         float unscale = a.scale_log2;
@@ -595,10 +718,10 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
                     const float* src = static_cast<const float*>(a.q) + from + k * 16 + g * 8;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const float y = mine && k * 16 < hd ? src[i] * up : 0.0f;
-                        const _Float16 hi = static_cast<_Float16>(y);
+                        _Float16 hi, lo;
+                        split(mine && k * 16 < hd ? src[i] * up : 0.0f, &hi, &lo);
                         qf[0][k][i] = hi;
-                        qf[1][k][i] = static_cast<_Float16>(y - static_cast<float>(hi));
+                        qf[1][k][i] = lo;
                     }
                 }
             } else {
@@ -621,7 +744,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
         float m = -__builtin_inff(), l = 0.0f, vref = 0.0f;
-        const int32_t* pages = a.table + static_cast<int64_t>(at.seq) * a.max_blocks;
+        const int32_t* pages = a.table + static_cast<int64_t>(share.p.seq) * a.max_blocks;
 
         // Lane i of a wave knows the page of position i of 64.
         const auto page_of = [&](int un) {
@@ -703,7 +826,8 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
         scales(id, &ks, &vs);
         convert(first & 1, vs);
         __syncthreads();
-        for (int un = first; un < last; ++un) {
+
+        const auto turn = [&](int un, auto masked) {
             const int half = un & 1, pos0 = un * kBigUnit;
             const uint64_t ok = __ballot(there(id));
             const int id_after = page_of(un + 2);
@@ -711,120 +835,124 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
                 load(un + 1, id_next);
                 scales(id_next, &ks_next, &vs_next);
             }
-            if (pos0 < most) {
-                f16v st[2];
+            f16v st[2];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) st[h][i] = 0.0f;
+                for (int i = 0; i < 16; ++i) st[h][i] = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < KS; ++k) {
-                        const h8 kf = kbuf[half][h][k][lane];
+                for (int k = 0; k < KS; ++k) {
+                    const h8 kf = kbuf[half][h][k][lane];
 #pragma unroll
-                        for (int x = 0; x < PARTS; ++x)
-                            st[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[x][k], st[h], 0, 0, 0);
-                    }
+                    for (int x = 0; x < PARTS; ++x)
+                        st[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[x][k], st[h], 0, 0, 0);
                 }
-                // scales of the four groups of 16 positions
-                float fk[4], fv[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    fk[q] = readlane(ks, 16 * q) * unscale;
-                    fv[q] = readlane(vs, 16 * q);
-                }
-                const bool open = pos0 + kBigUnit <= least && ok == ~0ull;
-                const auto seen = [&](int h, int i) {
-                    const int p = h * 32 + (i / 4) * 8 + g * 4 + i % 4;
-                    return pos0 + p < sees && (ok >> (h * 32 + (i / 8) * 16) & 1);
-                };
-                if (!open) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (!seen(h, i)) st[h][i] = -__builtin_inff();
-                }
-                float top = -__builtin_inff();
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    float t = st[q / 2][(q % 2) * 8];
-#pragma unroll
-                    for (int i = 1; i < 8; ++i) t = fmaxf(t, st[q / 2][(q % 2) * 8 + i]);
-                    if (t > -__builtin_inff()) top = fmaxf(top, t * fk[q]);
-                }
-                top = fmaxf(top, __shfl_xor(top, 32));
-                float vtop = vref;
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    if (fv[q] > vtop && fv[q] < __builtin_inff()) vtop = fv[q];
-                const bool grow_v = vtop > (F32 ? vref : 2.0f * vref);
-                if (__any(top > m + kSlack) || grow_v) {
-                    const float now = fmaxf(m, top);
-                    const float alpha = now == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - now);
-                    const float vnow = grow_v ? vtop : vref;
-                    const float beta = vnow > 0.0f ? alpha * (vref / vnow) : 0.0f;
-                    m = now;
-                    vref = vnow;
-                    l *= alpha;
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) o[t] *= beta;
-                }
-                const float ref = m == -__builtin_inff() ? 0.0f : m;
-                const float vone = vref > 0.0f ? 1.0f / vref : 0.0f;
-                h8 pf[PARTS][4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    if constexpr (F32) {
-                        const float to_v = fv[q] * vone * 16384.0f;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float x = st[q / 2][(q % 2) * 8 + i];
-                            float p = __builtin_amdgcn_exp2f(x * fk[q] - ref);
-                            if (!open && !seen(q / 2, (q % 2) * 8 + i)) p = 0.0f;
-                            l += p;
-                            const float y = p == 0.0f ? 0.0f : p * to_v;
-                            const _Float16 hi = static_cast<_Float16>(y);
-                            pf[0][q][i] = hi;
-                            pf[1][q][i] = static_cast<_Float16>(y - static_cast<float>(hi));
-                        }
-                    } else {
-                        const float ratio = fv[q] == 0.0f || vref == 0.0f ? 1.0f : fv[q] * vone;
-                        const float shift = __builtin_amdgcn_logf(ratio) + (kBase - ref);
-                        float sum = 0.0f;
-#pragma unroll
-                        for (int i = 0; i < 8; i += 2) {
-                            float x[2];
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[q / 2][(q % 2) * 8 + i + j], fk[q], shift));
-                                if (!open && !seen(q / 2, (q % 2) * 8 + i + j)) x[j] = 0.0f;
-                            }
-                            const h2 y = {static_cast<_Float16>(x[0]), static_cast<_Float16>(x[1])};
-                            pf[0][q][i] = y[0];
-                            pf[0][q][i + 1] = y[1];
-                            const h2 ones = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
-                            sum = __builtin_amdgcn_fdot2(y, ones, sum, false);
-                        }
-                        l += sum * (0x1p-10f / ratio);
-                    }
-                }
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const h8 vf = vbuf[half][t][q][lane];
-#pragma unroll
-                        for (int x = 0; x < PARTS; ++x)
-                            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[x][q], o[t], 0, 0, 0);
-                    }
             }
+            // scales of the four groups of 16 positions, and whether their page is there
+            float fk[4], fv[4];
+            bool in[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                fk[q] = readlane(ks, 16 * q) * unscale;
+                fv[q] = readlane(vs, 16 * q);
+                in[q] = (ok >> (16 * q) & 1) != 0;
+            }
+            const auto seen = [&](int h, int i) { return pos0 + h * 32 + (i / 4) * 8 + g * 4 + i % 4 < sees; };
+            if (masked) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (!seen(h, i)) st[h][i] = -__builtin_inff();
+            }
+            float top = -__builtin_inff();
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float t = st[q / 2][(q % 2) * 8];
+#pragma unroll
+                for (int i = 1; i < 8; ++i) t = fmaxf(t, st[q / 2][(q % 2) * 8 + i]);
+                // scales are not negative, so the largest product is the largest score
+                t = in[q] && t > -__builtin_inff() ? t * fk[q] : -__builtin_inff();
+                top = fmaxf(top, t);
+            }
+            top = fmaxf(top, __shfl_xor(top, 32));
+            float vtop = vref;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (fv[q] > vtop && fv[q] < __builtin_inff()) vtop = fv[q];
+            const bool grow_v = vtop > (F32 ? vref : 2.0f * vref);
+            if (__any(top > m + kSlack) || grow_v) {
+                const float now = fmaxf(m, top);
+                const float alpha = now == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - now);
+                const float vnow = grow_v ? vtop : vref;
+                const float beta = vnow > 0.0f ? alpha * (vref * __builtin_amdgcn_rcpf(vnow)) : 0.0f;
+                m = now;
+                vref = vnow;
+                l *= alpha;
+#pragma unroll
+                for (int t = 0; t < NT; ++t) o[t] *= beta;
+            }
+            const float ref = m == -__builtin_inff() ? 0.0f : m;
+            const float vone = vref > 0.0f ? __builtin_amdgcn_rcpf(vref) : 0.0f;
+            h8 pf[PARTS][4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float x[8];
+                if constexpr (F32) {
+                    const float to_v = fv[q] * vone * 16384.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        x[i] = __builtin_amdgcn_exp2f(st[q / 2][(q % 2) * 8 + i] * fk[q] - ref);
+                        if (!in[q] || (masked && !seen(q / 2, (q % 2) * 8 + i))) x[i] = 0.0f;
+                        l += x[i];
+                        const float y = masked && x[i] == 0.0f ? 0.0f : x[i] * to_v;
+                        _Float16 hi, lo;
+                        split(y, &hi, &lo);
+                        pf[0][q][i] = hi;
+                        pf[1][q][i] = lo;
+                    }
+                } else {
+                    const float ratio = fv[q] == 0.0f || vref == 0.0f ? 1.0f : fv[q] * vone;
+                    const float shift = in[q] ? __builtin_amdgcn_logf(ratio) + (kBase - ref) : -__builtin_inff();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[q / 2][(q % 2) * 8 + i], fk[q], shift));
+                        if (masked && !seen(q / 2, (q % 2) * 8 + i)) x[i] = 0.0f;
+                    }
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) {
+                        const h2 y = {static_cast<_Float16>(x[i]), static_cast<_Float16>(x[i + 1])};
+                        pf[0][q][i] = y[0];
+                        pf[0][q][i + 1] = y[1];
+                        const h2 ones = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
+                        sum = __builtin_amdgcn_fdot2(y, ones, sum, false);
+                    }
+                    l += sum * (0x1p-10f * __builtin_amdgcn_rcpf(ratio));
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const h8 vf = vbuf[half][t][q][lane];
+#pragma unroll
+                    for (int x = 0; x < PARTS; ++x)
+                        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[x][q], o[t], 0, 0, 0);
+                }
             if (un + 1 < last) convert((un + 1) & 1, vs_next);
             __syncthreads();
             id = id_next;
             id_next = id_after;
             ks = ks_next;
             vs = vs_next;
-        }
+        };
+        // The waves turn together; each masks from where its first column ends.
+        int un = first;
+#pragma unroll 1
+        for (; un < last && (un + 1) * kBigUnit <= least; ++un) turn(un, std::false_type{});
+#pragma unroll 1
+        for (; un < last; ++un) turn(un, std::true_type{});
 
         // o[t][i] is dimension (8 (i / 4) + 4 g + i % 4) * NT + t of this lane's column.
         l += __shfl_xor(l, 32);
@@ -841,7 +969,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
                         if (d < hd) put<QT>(a.out, to + d, l != 0.0f ? o[t][i] * f : 0.0f);
                     }
             } else {
-                float* part = part_at(a, me, first == 0, HD) + c * (HD + 2);
+                float* part = part_at(a, blockIdx.x, first == 0, HD) + c * (HD + 2);
                 if (g == 0) part[0] = m, part[1] = l;
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
@@ -850,43 +978,51 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
                         part[2 + (8 * (i / 4) + 4 * g + i % 4) * NT + t] = o[t][i] * unit_v;
             }
         }
-        at.u += last - first;
-        if (at.u < at.u_end) at.next(a);
-    }
+    } while (share.next(a));
 }
+
 // Joins the parts of the items that more than one workgroup took, in workgroup
-// order.  Workgroup w here looks at the border before workgroup w + 1 of the
-// other kernel: if it is the first one inside an item, the item's columns
-// [y * kJoinCols, (y + 1) * kJoinCols) are its to join.
+// order.  Workgroup x looks at the border between workgroups x and x + 1 of
+// the other kernel: if it is the first border inside an item, the item's
+// columns from y * kJoinCols on are its to join.
 constexpr int kJoinCols = 16;
 
 template <int QT, int HD, bool BIG>
 __global__ __launch_bounds__(kThreads) void join_q8_kernel(Q8Args a, int grid) {
-    const int w1 = blockIdx.x + 1;
+    const int w0 = blockIdx.x;
     int64_t total;
-    Place<BIG> p;
-    if (!p.find(a, w1, &grid, &total, [&](int64_t n, int g) { return (w1 < g ? w1 : 0) * n / g; })) return;
-    const int64_t u0 = p.u - p.unit;  // the item's first unit
-    if (p.unit == 0 || (w1 - 1) * total / grid > u0) return;
-    // the workgroup of the item's last unit
-    const int w_end = static_cast<int>(((u0 + p.units) * grid - 1) / total);
-    const Seq<BIG> s(a, p.seq);
-    const int col0 = p.tile * Seq<BIG>::COLS;
+    Place p[1];
+    if (!find<BIG, 1>(a, &grid, &total, p, [&](int, int64_t n, int g) -> int64_t {
+            return w0 + 1 < g ? cut(w0 + 1, n, g) : -1;
+        }))
+        return;
+    if (p[0].unit == 0) return;
+    const int64_t off0 = cut(w0, total, grid) - p[0].item;  // the border before
+    if (off0 > 0 && (BIG ? quotient(off0 * p[0].units, p[0].cost) : off0) > 0) return;
+    int w_end = w0 + 1;  // whose share holds the item's end
+    {
+        const int64_t end = p[0].item + p[0].cost;
+        w_end = static_cast<int>(quotient(end * grid - 1, total));
+        while (w_end + 1 < grid && cut(w_end + 1, total, grid) < end) ++w_end;
+        while (w_end > w0 + 1 && cut(w_end, total, grid) >= end) --w_end;
+    }
+    const Seq<BIG> s = Seq<BIG>::uniform(a, p[0].seq);
+    const int col0 = p[0].tile * Seq<BIG>::COLS;
     const int left = s.rows * a.group - col0;
     const int c0 = blockIdx.y * kJoinCols;
     int c1 = c0 + kJoinCols < left ? c0 + kJoinCols : left;
     if (c1 > Seq<BIG>::COLS) c1 = Seq<BIG>::COLS;
     const int hd = a.head_dim;
-    constexpr int AHEAD = 8;  // parts whose loads are in flight together
+    constexpr int AHEAD = 12;  // parts whose loads are in flight together
     for (int x = c0 * HD + threadIdx.x; x < c1 * HD; x += kThreads) {
         const int c = x / HD, d = x % HD;
         float top = -__builtin_inff(), sum = 0.0f, val = 0.0f;
-        for (int w = w1 - 1; w <= w_end; w += AHEAD) {
+        for (int w = w0; w <= w_end; w += AHEAD) {
             float m[AHEAD], l[AHEAD], v[AHEAD];
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) {
                 const int ww = w + i <= w_end ? w + i : w_end;
-                const float* part = part_at(a, ww, ww == w1 - 1, HD) + c * (HD + 2);
+                const float* part = part_at(a, ww, ww == w0, HD) + c * (HD + 2);
                 m[i] = part[0];
                 l[i] = part[1];
                 v[i] = part[2 + d];
@@ -900,10 +1036,12 @@ __global__ __launch_bounds__(kThreads) void join_q8_kernel(Q8Args a, int grid) {
             val *= f0;
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) {
-                if (w + i > w_end) break;
-                const float f = __builtin_amdgcn_exp2f(m[i] - ref);
-                sum += f * l[i];
-                val += f * v[i];
+                // a sum of 0: nothing seen, or a share without units, which leaves no output
+                if (w + i <= w_end && l[i] != 0.0f) {
+                    const float f = __builtin_amdgcn_exp2f(m[i] - ref);
+                    sum += f * l[i];
+                    val += f * v[i];
+                }
             }
             top = most;
         }
@@ -911,7 +1049,7 @@ __global__ __launch_bounds__(kThreads) void join_q8_kernel(Q8Args a, int grid) {
             const int cc = col0 + c;
             put<QT>(a.out,
                     static_cast<int64_t>(s.row0 + cc / a.group) * a.ldo +
-                        static_cast<int64_t>(p.head * a.group + cc % a.group) * hd + d,
+                        static_cast<int64_t>(p[0].head * a.group + cc % a.group) * hd + d,
                     sum != 0.0f ? val / sum : 0.0f);
         }
     }
