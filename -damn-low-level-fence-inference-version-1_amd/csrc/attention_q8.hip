@@ -28,6 +28,10 @@ constexpr int kCols = 16;              // attention_q8_kernel: each wave all of 
 constexpr int kUnit = 32 * kWaves;     // and the positions its workgroup takes at a time
 constexpr int kBigCols = 32 * kWaves;  // prompt_q8_kernel: each wave 32 of them, all positions
 constexpr int kBigUnit = 64;
+#ifndef FENCE_ATTN_Q8_ITEM
+#define FENCE_ATTN_Q8_ITEM 192
+#endif
+constexpr int kBigItem = FENCE_ATTN_Q8_ITEM;  // what an item costs besides its positions, in positions
 // Up to this many columns a sequence goes to attention_q8_kernel.
 #ifndef FENCE_ATTN_Q8_SMALL
 #define FENCE_ATTN_Q8_SMALL 32
@@ -58,6 +62,7 @@ struct Q8Args {
     int max_blocks, batch, max_q_len;
     int part_cols;  // columns of a part in the workspace
     float scale_log2;
+    int wide;  // out and its rows are 16-byte aligned
 };
 
 // Read-only data at addresses that are the same in every lane, through the
@@ -103,11 +108,11 @@ struct Seq {
         return n > UNIT ? (n + UNIT - 1) / UNIT : 1;
     }
     // What a tile of one kv head costs and what the tiles before it do, for the even split.  Few tiles: their
-    // units.  Many: about the positions that its columns see, a linear function of the tile, so that the sum
-    // needs no loop over the tiles.
+    // units.  Many: about the positions that its columns see and kBigItem more for beginning and ending an item,
+    // times the group; a linear function of the tile, so that the sum needs no loop over the tiles.
     __device__ __forceinline__ int64_t slope() const {
         const int64_t n = static_cast<int64_t>(kv) - q_len + 1;
-        return (n < 1 ? 1 : n) * group - 1;
+        return ((n < 1 ? 1 : n) + kBigItem) * group - 1;
     }
     __device__ __forceinline__ int64_t cost(int tile) const {
         if constexpr (!BIG) return units(tile);
@@ -134,6 +139,13 @@ __device__ __forceinline__ int64_t wave_scan(int64_t v) {
         if (lane >= d) v += up;
     }
     return v;
+}
+
+// A value that is the same in every lane, where the compiler cannot know it.
+__device__ __forceinline__ int64_t uniform64(int64_t v) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+    return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
 }
 
 // x / y rounded down for numbers below 2^53, where the quotient in 64-bit
@@ -171,10 +183,11 @@ __device__ __forceinline__ bool find(const Q8Args& a, int* grid, int64_t* total,
         return b < a.batch ? Seq<BIG>(a, a.q_start[b], a.q_start[b + 1], a.kv_lens[b]).all(a) : 0;
     };
     const auto points = [&]() {
+        *total = uniform64(*total);
         *grid = sharers(*total, *grid);
         if (*grid == 0) return false;
 #pragma unroll
-        for (int i = 0; i < N; ++i) point[i] = at(i, *total, *grid);
+        for (int i = 0; i < N; ++i) point[i] = uniform64(at(i, *total, *grid));
         return point[0] >= 0;
     };
     if (a.batch == 1) {
@@ -229,7 +242,7 @@ __device__ __forceinline__ bool find(const Q8Args& a, int* grid, int64_t* total,
     for (int i = 0; i < N; ++i) {
         p[i].seq = __builtin_amdgcn_readfirstlane(p[i].seq);
         const Seq<BIG> s = Seq<BIG>::uniform(a, p[i].seq);
-        const int64_t rest = point[i] - before[i];
+        const int64_t rest = point[i] - uniform64(before[i]);
         int lo = 0, hi = s.tiles() - 1;  // the last tile that begins at or before it
         while (lo < hi) {
             const int mid = (lo + hi + 1) / 2;
@@ -237,9 +250,9 @@ __device__ __forceinline__ bool find(const Q8Args& a, int* grid, int64_t* total,
             else hi = mid - 1;
         }
         p[i].tile = __builtin_amdgcn_readfirstlane(lo);
-        p[i].units = s.units(lo);
-        p[i].cost = s.cost(lo);
-        const int64_t in_tile = rest - s.before(lo) * a.n_kv_heads;
+        p[i].units = s.units(p[i].tile);
+        p[i].cost = s.cost(p[i].tile);
+        const int64_t in_tile = rest - s.before(p[i].tile) * a.n_kv_heads;
         p[i].head = __builtin_amdgcn_readfirstlane(static_cast<int>(quotient(in_tile, p[i].cost)));
         const int64_t off = in_tile - p[i].head * p[i].cost;
         p[i].item = point[i] - off;
@@ -300,10 +313,12 @@ struct Share {
 
 // Where a workgroup leaves its part of an item that it shares: the one that
 // it ends (or passes through) and the one that it begins.  A part: per column
-// the running maximum, the sum and the unnormalised output.
+// the unnormalised output, then per column the running maximum and the sum.
+__host__ __device__ __forceinline__ int64_t part_size(int cols, int hd) { return (static_cast<int64_t>(cols) * (hd + 2) + 3) / 4 * 4; }
 __device__ __forceinline__ float* part_at(const Q8Args& a, int wg, bool begins, int hd) {
-    return a.ws + static_cast<int64_t>(wg * 2 + (begins ? 1 : 0)) * a.part_cols * (hd + 2);
+    return a.ws + (wg * 2 + (begins ? 1 : 0)) * part_size(a.part_cols, hd);
 }
+__device__ __forceinline__ float* part_sums(const Q8Args& a, float* part, int hd) { return part + a.part_cols * hd; }
 
 // y as the sum of two binary16 numbers, 22 bits of it.  The empty asm makes y
 // one fp32 value: otherwise the product that it came from may be rounded to
@@ -319,6 +334,24 @@ template <int QT>
 __device__ __forceinline__ void put(void* out, int64_t at, float v) {
     if constexpr (QT == FENCE_F32) static_cast<float*>(out)[at] = v;
     else static_cast<uint16_t*>(out)[at] = f32_to_f16_bits(v);
+}
+
+// Eight in a row.  a.wide: 16-byte aligned.
+template <int QT>
+__device__ __forceinline__ void put8(const Q8Args& a, int64_t at, const float* y) {
+    if (!a.wide) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) put<QT>(a.out, at + i, y[i]);
+    } else if constexpr (QT == FENCE_F32) {
+        float* p = static_cast<float*>(a.out) + at;
+        *reinterpret_cast<f4*>(p) = f4{y[0], y[1], y[2], y[3]};
+        *reinterpret_cast<f4*>(p + 4) = f4{y[4], y[5], y[6], y[7]};
+    } else {
+        h8 h;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = static_cast<_Float16>(y[i]);
+        *reinterpret_cast<h8*>(static_cast<_Float16*>(a.out) + at) = h;
+    }
 }
 
 // Codes to binary16, four bytes to two pairs.  int8: with the sign bit
@@ -626,8 +659,11 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void attention_q8_kern
                     put<QT>(a.out, to, sum != 0.0f ? val / sum : 0.0f);
                 }
             } else {
-                part[c * (HD + 2) + 2 + d] = val;
-                if (d == 0) part[c * (HD + 2)] = top, part[c * (HD + 2) + 1] = sum;
+                part[c * HD + d] = val;
+                if (d == 0) {
+                    float* to = part_sums(a, part, HD) + 2 * c;
+                    to[0] = top, to[1] = sum;
+                }
             }
         }
         __syncthreads();
@@ -644,29 +680,33 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void attention_q8_kern
 // the second takes as its k index in that order, so P stays in registers; row
 // r of V' product t stands for dimension r * HD / 32 + t, so a thread that
 // converts 4 dimensions of 8 positions writes whole fragments, and a lane ends
-// with 16 consecutive dimensions of its column.
+// with runs of 4 * HD / 32 dimensions of its column.
 //
-// The next 64 positions' codes are loaded before the products of these and
-// converted behind them into the other half of LDS, with one barrier a turn.
+// Wave w converts positions 16 w .. 16 w + 15, which lie in one page, so its
+// addresses are a scalar and a 32-bit offset a lane.  The next positions'
+// codes are loaded before the products of these and converted behind them
+// into the other half of LDS, with one barrier a turn.  Left to itself the
+// compiler reads one fragment, waits and multiplies, 32 times a turn; the
+// scheduling groups put the reads a few products ahead.
 //
-// binary16 (QT = FENCE_F16): with the page's V scale as a power of two in the
-// exponent, one fused multiply-add and one exponential make the probability
-// that the product takes, and its sum comes from the rounded values by dot
-// products.  The running maximum and the largest V scale are only moved when
-// a value would grow past 2^15 (kSlack), so O is rarely rescaled.
+// binary16 (QT = FENCE_F16): with the page's V scale in the exponent, one
+// fused multiply-add and one exponential make the probability that the
+// product takes, and its sum comes from the rounded values by dot products.
+// The running maximum and the largest V scale are only moved when a value
+// would grow past 2^15 (kSlack), so O is rarely rescaled.
 template <int TYPE, int QT, int HD>
 __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(Q8Args a) {
     constexpr bool F32 = QT == FENCE_F32;
     constexpr int PARTS = F32 ? 2 : 1;
-    constexpr int KS = HD / 16;               // k steps of the first product
-    constexpr int NT = HD / 32;               // products over V
-    constexpr int KJ = HD * 4 / kThreads;     // 16-byte pieces of K a thread converts
-    constexpr int VITEMS = HD * 2;            // 8 positions x 4 dimensions of V
-    constexpr int VJ = (VITEMS + kThreads - 1) / kThreads;
+    constexpr int KS = HD / 16;   // k steps of the first product
+    constexpr int NT = HD / 32;   // products over V
+    constexpr int KJ = HD / 64;   // 16-byte pieces of K a lane converts
+    constexpr int VJ = HD <= 128 ? 1 : 2;  // 8 positions x 4 dimensions of V a lane converts
     constexpr float kBase = F32 ? 14.0f : 10.0f;  // log2 of what stands for 1 times the largest V scale
     constexpr float kSlack = F32 ? 0.0f : 4.0f;
     __shared__ h8 kbuf[2][2][KS][kWave];
-    __shared__ h8 vbuf[2][NT][4][kWave];
+    __shared__ h8 vbuf[2][4][NT][kWave];
+    __shared__ f4 sbuf[2][4];  // per 16 positions: K scale (-1 if the page is not there), V scale, its log2 and inverse
     const int tid = threadIdx.x, lane = tid % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int n = lane % 32, g = lane / 32;
@@ -674,6 +714,18 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
 
     Share<true> share;
     if (!share.find_mine(a)) return;
+    // what this lane converts: K position lane % 16, dimensions 16 (lane / 16 + 4 j) on; V positions 4 vg + (0 .. 3)
+    // and 8 more, dimensions vd on
+    const int kr = lane % 16, kc = lane / 16;
+    const int vd = HD == 256 ? lane * 4 : lane % (HD / 4) * 4;
+    const int vg = HD == 256 ? 0 : lane / (HD / 4) % 2;  // at HD = 64 the upper lanes load what the lower ones do
+    const bool vmine = (HD == 64 ? lane < 32 : true) && vd < hd;
+    if (hd < HD) {  // dimensions that are not there stay zero
+        const h8 zero = {};
+        for (int i = tid; i < 2 * 2 * KS * kWave; i += kThreads) (&kbuf[0][0][0][0])[i] = zero;
+        for (int i = tid; i < 2 * 4 * NT * kWave; i += kThreads) (&vbuf[0][0][0][0])[i] = zero;
+        __syncthreads();
+    }
     do {
         const Seq<true> s = Seq<true>::uniform(a, share.p.seq);
         const int tile = share.p.tile, head = share.p.head, first = share.p.unit, units = share.p.units;
@@ -688,12 +740,87 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
         if (first >= last) {
             // Nothing of this item; if others take what is before and after, the join finds an empty part.
             if (first > 0 && mine && g == 0) {
-                float* part = part_at(a, blockIdx.x, false, HD) + c * (HD + 2);
-                part[0] = -__builtin_inff(), part[1] = 0.0f;
+                float* ml = part_sums(a, part_at(a, blockIdx.x, false, HD), HD) + 2 * c;
+                ml[0] = -__builtin_inff(), ml[1] = 0.0f;
             }
             continue;
         }
         const int least = s.row_sees((tile * kBigCols + wave * 32) / a.group);  // what every column of this wave sees
+        const int64_t table = static_cast<int64_t>(share.p.seq) * a.max_blocks;
+
+        // The page of this wave's 16 positions of a unit.
+        const auto page_of = [&](int un) {
+            const int pos = un * kBigUnit + wave * 16;
+            return un < last && pos < end ? uniform_load(a.table, table + (pos >> a.page_shift)) : -1;
+        };
+        u4 kw[KJ];
+        uint32_t vw[VJ][8];
+        float ks, vs;
+        const auto load = [&](int un, int id) {
+            const bool there = id >= 0 && id < a.n_pages;
+            const int64_t base = static_cast<int64_t>(there ? id : 0) * a.n_kv_heads + head;
+            ks = there ? uniform_load(a.ks, base) : -1.0f;
+            vs = there ? uniform_load(a.vs, base) : 0.0f;
+            const int64_t at = ((base << a.page_shift) + ((un * kBigUnit + wave * 16) & page_mask)) * hd;
+            const uint8_t* k = a.k + at;
+            const uint8_t* v = a.v + at;
+#pragma unroll
+            for (int j = 0; j < KJ; ++j) {
+                const uint32_t d = (kc + 4 * j) * 16;
+                kw[j] = *reinterpret_cast<const u4*>(k + static_cast<uint32_t>(kr * hd) + (d < static_cast<uint32_t>(hd) ? d : 0));
+            }
+#pragma unroll
+            for (int j = 0; j < VJ; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    vw[j][i] = *reinterpret_cast<const uint32_t*>(
+                        v + ((i / 4) * 8 + i % 4) * hd +
+                        (static_cast<uint32_t>((vg + j) * 4 * hd) + static_cast<uint32_t>(vd < hd ? vd : 0)));
+        };
+        // Into half `half` of LDS.  Positions past the end, and pages whose V scale is 0, get V codes of 0.
+        const auto convert = [&](int un, int half) {
+            const int pos0 = un * kBigUnit + wave * 16;
+#pragma unroll
+            for (int j = 0; j < KJ; ++j) {
+                const int k = kc + 4 * j;
+                if (k * 16 < hd) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        h2 c0, c1, c2, c3;
+                        codes_h<TYPE>(kw[j][2 * i], &c0, &c1);
+                        codes_h<TYPE>(kw[j][2 * i + 1], &c2, &c3);
+                        kbuf[half][wave / 2][k][i * 32 + (wave % 2) * 16 + kr] = join(c0, c1, c2, c3);
+                    }
+                }
+            }
+            if (vs == 0.0f || pos0 + 16 > end) {
+#pragma unroll
+                for (int j = 0; j < VJ; ++j)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (vs == 0.0f || pos0 + (vg + j) * 4 + (i / 4) * 8 + i % 4 >= end) vw[j][i] = 0;
+            }
+#pragma unroll
+            for (int j = 0; j < VJ; ++j) {
+                h2 x[4][4];
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    const uint32_t y = vw[j][2 * p], z = vw[j][2 * p + 1];
+                    codes_h<TYPE>(__builtin_amdgcn_perm(z, y, 0x05010400u), &x[p][0], &x[p][1]);
+                    codes_h<TYPE>(__builtin_amdgcn_perm(z, y, 0x07030602u), &x[p][2], &x[p][3]);
+                }
+                if (vmine) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        vbuf[half][wave][(vd + i) % NT][(vg + j) * 32 + (vd + i) / NT] =
+                            join(x[0][i], x[1][i], x[2][i], x[3][i]);
+                }
+            }
+            if (lane == 0) sbuf[half][wave] = f4{ks, vs, __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs)};
+        };
+
+        load(first, page_of(first));
+        int id_next = page_of(first + 1);
 
         h8 qf[PARTS][KS];
         float unscale = a.scale_log2;
@@ -744,120 +871,51 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
         float m = -__builtin_inff(), l = 0.0f, vref = 0.0f;
-        const int32_t* pages = a.table + static_cast<int64_t>(share.p.seq) * a.max_blocks;
-
-        // Lane i of a wave knows the page of position i of 64.
-        const auto page_of = [&](int un) {
-            const int pos = un * kBigUnit + lane;
-            return un < last && pos < end ? pages[pos >> a.page_shift] : -1;
-        };
-        const auto there = [&](int id) { return id >= 0 && id < a.n_pages; };
-        u4 kw[KJ];
-        uint32_t vw[VJ][8];
-        // this thread's codes of a unit, 0 for positions that are not there
-        const auto load = [&](int un, int id) {
-            const bool ok = there(id);
-            const int64_t base = (static_cast<int64_t>(ok ? id : 0) * a.n_kv_heads + head) << a.page_shift;
-            const int64_t krow = (base + ((un * kBigUnit + lane) & page_mask)) * hd;
-#pragma unroll
-            for (int j = 0; j < KJ; ++j) {
-                const int d = (wave + kWaves * j) * 16;
-                kw[j] = u4{0, 0, 0, 0};
-                if (ok && d < hd) kw[j] = *reinterpret_cast<const u4*>(a.k + krow + d);
-            }
-#pragma unroll
-            for (int j = 0; j < VJ; ++j) {
-                const int item = tid + j * kThreads;
-                const int d = item % (HD / 4) * 4, sg = item / (HD / 4);
-                const int p0 = (sg / 2) * 16 + (sg % 2) * 4;
-                const int64_t vbase = __shfl(base, p0 & 63);
-                const bool vok = __shfl(static_cast<int>(ok), p0 & 63) && item < VITEMS && d < hd;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int p = un * kBigUnit + p0 + (i / 4) * 8 + i % 4;
-                    vw[j][i] = 0;
-                    if (vok && p < end)
-                        vw[j][i] = *reinterpret_cast<const uint32_t*>(a.v + (vbase + (p & page_mask)) * hd + d);
-                }
-            }
-        };
-        const auto scales = [&](int id, float* ks, float* vs) {
-            const int64_t i = static_cast<int64_t>(there(id) ? id : 0) * a.n_kv_heads + head;
-            *ks = there(id) ? a.ks[i] : 0.0f;
-            *vs = there(id) ? a.vs[i] : 0.0f;
-        };
-        const auto convert = [&](int half, float vs) {
-#pragma unroll
-            for (int j = 0; j < KJ; ++j) {
-                const int k = wave + kWaves * j;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    h2 c0, c1, c2, c3;
-                    codes_h<TYPE>(kw[j][2 * i], &c0, &c1);
-                    codes_h<TYPE>(kw[j][2 * i + 1], &c2, &c3);
-                    kbuf[half][lane / 32][k][i * 32 + lane % 32] = join(c0, c1, c2, c3);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < VJ; ++j) {
-                const int item = tid + j * kThreads;
-                const int d = item % (HD / 4) * 4, sg = item / (HD / 4);
-                // a page whose scale is 0 holds zeros, whatever its codes
-                const bool none = !F32 && __shfl(vs, ((sg / 2) * 16) & 63) == 0.0f;
-                h2 x[4][4];
-#pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                    const uint32_t y = none ? 0 : vw[j][2 * p], z = none ? 0 : vw[j][2 * p + 1];
-                    codes_h<TYPE>(__builtin_amdgcn_perm(z, y, 0x05010400u), &x[p][0], &x[p][1]);
-                    codes_h<TYPE>(__builtin_amdgcn_perm(z, y, 0x07030602u), &x[p][2], &x[p][3]);
-                }
-                if (item < VITEMS) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        vbuf[half][(d + i) % NT][sg / 2][(sg % 2) * 32 + (d + i) / NT] =
-                            join(x[0][i], x[1][i], x[2][i], x[3][i]);
-                }
-            }
-        };
-
-        int id = page_of(first), id_next = page_of(first + 1);
-        float ks, vs, ks_next = 0.0f, vs_next = 0.0f;
-        load(first, id);
-        scales(id, &ks, &vs);
-        convert(first & 1, vs);
+        convert(first, first & 1);
         __syncthreads();
 
         const auto turn = [&](int un, auto masked) {
             const int half = un & 1, pos0 = un * kBigUnit;
-            const uint64_t ok = __ballot(there(id));
-            const int id_after = page_of(un + 2);
-            if (un + 1 < last) {
-                load(un + 1, id_next);
-                scales(id_next, &ks_next, &vs_next);
-            }
+            if (un + 1 < last) load(un + 1, id_next);
+            id_next = page_of(un + 2);
             f16v st[2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) st[h][i] = 0.0f;
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int k = 0; k < KS; ++k) {
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
                     const h8 kf = kbuf[half][h][k][lane];
 #pragma unroll
                     for (int x = 0; x < PARTS; ++x)
                         st[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[x][k], st[h], 0, 0, 0);
                 }
+            f4 sc[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) sc[q] = sbuf[half][q];
+            // reads kAhead fragments ahead of the products
+            constexpr int kAhead = F32 ? 4 : 6;
+            __builtin_amdgcn_sched_group_barrier(0x100, kAhead + 4, 0);
+#pragma unroll
+            for (int i = 0; i < 2 * KS - kAhead; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, PARTS, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             }
-            // scales of the four groups of 16 positions, and whether their page is there
-            float fk[4], fv[4];
+            __builtin_amdgcn_sched_group_barrier(0x008, kAhead * PARTS, 0);
+            __builtin_amdgcn_sched_barrier(0);
+
+            float fk[4];
             bool in[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                fk[q] = readlane(ks, 16 * q) * unscale;
-                fv[q] = readlane(vs, 16 * q);
-                in[q] = (ok >> (16 * q) & 1) != 0;
+                in[q] = !(sc[q][0] < 0.0f);
+                fk[q] = sc[q][0] * unscale;
             }
-            const auto seen = [&](int h, int i) { return pos0 + h * 32 + (i / 4) * 8 + g * 4 + i % 4 < sees; };
+            const int limit = sees - pos0 - g * 4;  // of this lane's positions: see, those below it
+            const auto seen = [&](int h, int i) { return h * 32 + (i / 4) * 8 + i % 4 < limit; };
             if (masked) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
@@ -879,9 +937,9 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
             float vtop = vref;
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-                if (fv[q] > vtop && fv[q] < __builtin_inff()) vtop = fv[q];
+                if (sc[q][1] > vtop && sc[q][1] < __builtin_inff()) vtop = sc[q][1];
             const bool grow_v = vtop > (F32 ? vref : 2.0f * vref);
-            if (__any(top > m + kSlack) || grow_v) {
+            if (__any(top > m + kSlack || grow_v)) {
                 const float now = fmaxf(m, top);
                 const float alpha = now == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - now);
                 const float vnow = grow_v ? vtop : vref;
@@ -894,26 +952,27 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
             }
             const float ref = m == -__builtin_inff() ? 0.0f : m;
             const float vone = vref > 0.0f ? __builtin_amdgcn_rcpf(vref) : 0.0f;
-            h8 pf[PARTS][4];
+            const float vlog = vref > 0.0f ? __builtin_amdgcn_logf(vref) : 0.0f;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                float x[8];
+                h8 pf[PARTS];
                 if constexpr (F32) {
-                    const float to_v = fv[q] * vone * 16384.0f;
+                    const float to_v = sc[q][1] * vone * 16384.0f;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        x[i] = __builtin_amdgcn_exp2f(st[q / 2][(q % 2) * 8 + i] * fk[q] - ref);
-                        if (!in[q] || (masked && !seen(q / 2, (q % 2) * 8 + i))) x[i] = 0.0f;
-                        l += x[i];
-                        const float y = masked && x[i] == 0.0f ? 0.0f : x[i] * to_v;
+                        float x = __builtin_amdgcn_exp2f(st[q / 2][(q % 2) * 8 + i] * fk[q] - ref);
+                        if (!in[q] || (masked && !seen(q / 2, (q % 2) * 8 + i))) x = 0.0f;
+                        l += x;
+                        const float y = masked && x == 0.0f ? 0.0f : x * to_v;
                         _Float16 hi, lo;
                         split(y, &hi, &lo);
-                        pf[0][q][i] = hi;
-                        pf[1][q][i] = lo;
+                        pf[0][i] = hi;
+                        pf[PARTS - 1][i] = lo;
                     }
                 } else {
-                    const float ratio = fv[q] == 0.0f || vref == 0.0f ? 1.0f : fv[q] * vone;
-                    const float shift = in[q] ? __builtin_amdgcn_logf(ratio) + (kBase - ref) : -__builtin_inff();
+                    const bool none = sc[q][1] == 0.0f;  // its V codes are zero: any weight will do that can be taken back
+                    const float shift = in[q] ? (none ? 0.0f : sc[q][2] - vlog) + (kBase - ref) : -__builtin_inff();
+                    float x[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[q / 2][(q % 2) * 8 + i], fk[q], shift));
@@ -923,29 +982,23 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
 #pragma unroll
                     for (int i = 0; i < 8; i += 2) {
                         const h2 y = {static_cast<_Float16>(x[i]), static_cast<_Float16>(x[i + 1])};
-                        pf[0][q][i] = y[0];
-                        pf[0][q][i + 1] = y[1];
+                        pf[0][i] = y[0];
+                        pf[0][i + 1] = y[1];
                         const h2 ones = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
                         sum = __builtin_amdgcn_fdot2(y, ones, sum, false);
                     }
-                    l += sum * (0x1p-10f * __builtin_amdgcn_rcpf(ratio));
+                    l += sum * (none ? 0x1p-10f : 0x1p-10f * (vref * sc[q][3]));
                 }
-            }
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const h8 vf = vbuf[half][t][q][lane];
+                for (int t = 0; t < NT; ++t) {
+                    const h8 vf = vbuf[half][q][t][lane];
 #pragma unroll
                     for (int x = 0; x < PARTS; ++x)
-                        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[x][q], o[t], 0, 0, 0);
+                        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[x], o[t], 0, 0, 0);
                 }
-            if (un + 1 < last) convert((un + 1) & 1, vs_next);
+            }
+            if (un + 1 < last) convert(un + 1, half ^ 1);
             __syncthreads();
-            id = id_next;
-            id_next = id_after;
-            ks = ks_next;
-            vs = vs_next;
         };
         // The waves turn together; each masks from where its first column ends.
         int un = first;
@@ -954,29 +1007,37 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
 #pragma unroll 1
         for (; un < last; ++un) turn(un, std::true_type{});
 
-        // o[t][i] is dimension (8 (i / 4) + 4 g + i % 4) * NT + t of this lane's column.
+        // o[t][i] is dimension (8 (i / 4) + 4 g + i % 4) * NT + t of this lane's column: runs of 4 NT.
         l += __shfl_xor(l, 32);
         const float unit_v = vref * (F32 ? 0x1p-14f : 0x1p-10f);
         if (mine) {
-            if (first == 0 && last == units) {
-                const float f = l != 0.0f ? unit_v / l : 0.0f;
-                const int64_t to = static_cast<int64_t>(s.row0 + row) * a.ldo + static_cast<int64_t>(qhead) * hd;
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        const int d = (8 * (i / 4) + 4 * g + i % 4) * NT + t;
-                        if (d < hd) put<QT>(a.out, to + d, l != 0.0f ? o[t][i] * f : 0.0f);
-                    }
-            } else {
-                float* part = part_at(a, blockIdx.x, first == 0, HD) + c * (HD + 2);
-                if (g == 0) part[0] = m, part[1] = l;
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-#pragma unroll
-                    for (int t = 0; t < NT; ++t)
-                        part[2 + (8 * (i / 4) + 4 * g + i % 4) * NT + t] = o[t][i] * unit_v;
+            const bool whole = first == 0 && last == units;
+            const float f = whole ? (l != 0.0f ? unit_v / l : 0.0f) : unit_v;
+            float* part = part_at(a, blockIdx.x, first == 0, HD);
+            const int64_t to = static_cast<int64_t>(s.row0 + row) * a.ldo + static_cast<int64_t>(qhead) * hd;
+            if (!whole && g == 0) {
+                float* ml = part_sums(a, part, HD) + 2 * c;
+                ml[0] = m, ml[1] = l;
             }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int x = 0; x < 4 * NT; x += 8) {
+                    const int d = (8 * q + 4 * g) * NT + x;
+                    float y[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int j = (x + i) / NT, t = (x + i) % NT;
+                        y[i] = whole && l == 0.0f ? 0.0f : o[t][4 * q + j] * f;
+                    }
+                    if (whole) {
+                        if (d < hd) put8<QT>(a, to + d, y);
+                    } else {
+                        float* p = part + c * HD + d;
+                        *reinterpret_cast<f4*>(p) = f4{y[0], y[1], y[2], y[3]};
+                        *reinterpret_cast<f4*>(p + 4) = f4{y[4], y[5], y[6], y[7]};
+                    }
+                }
         }
     } while (share.next(a));
 }
@@ -984,9 +1045,8 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
 // Joins the parts of the items that more than one workgroup took, in workgroup
 // order.  Workgroup x looks at the border between workgroups x and x + 1 of
 // the other kernel: if it is the first border inside an item, the item's
-// columns from y * kJoinCols on are its to join.
-constexpr int kJoinCols = 16;
-
+// columns are its to join, together with the other workgroups of the same x,
+// a run of 4 dimensions a thread.
 template <int QT, int HD, bool BIG>
 __global__ __launch_bounds__(kThreads) void join_q8_kernel(Q8Args a, int grid) {
     const int w0 = blockIdx.x;
@@ -999,33 +1059,33 @@ __global__ __launch_bounds__(kThreads) void join_q8_kernel(Q8Args a, int grid) {
     if (p[0].unit == 0) return;
     const int64_t off0 = cut(w0, total, grid) - p[0].item;  // the border before
     if (off0 > 0 && (BIG ? quotient(off0 * p[0].units, p[0].cost) : off0) > 0) return;
-    int w_end = w0 + 1;  // whose share holds the item's end
-    {
-        const int64_t end = p[0].item + p[0].cost;
-        w_end = static_cast<int>(quotient(end * grid - 1, total));
-        while (w_end + 1 < grid && cut(w_end + 1, total, grid) < end) ++w_end;
-        while (w_end > w0 + 1 && cut(w_end, total, grid) >= end) --w_end;
-    }
+    // the workgroup whose share holds the item's end
+    const int64_t end = p[0].item + p[0].cost;
+    int w_end = static_cast<int>(quotient(end * grid - 1, total));
+    while (w_end + 1 < grid && cut(w_end + 1, total, grid) < end) ++w_end;
+    while (w_end > w0 + 1 && cut(w_end, total, grid) >= end) --w_end;
+    w_end = __builtin_amdgcn_readfirstlane(w_end);
     const Seq<BIG> s = Seq<BIG>::uniform(a, p[0].seq);
     const int col0 = p[0].tile * Seq<BIG>::COLS;
     const int left = s.rows * a.group - col0;
-    const int c0 = blockIdx.y * kJoinCols;
-    int c1 = c0 + kJoinCols < left ? c0 + kJoinCols : left;
-    if (c1 > Seq<BIG>::COLS) c1 = Seq<BIG>::COLS;
+    const int cols = left < Seq<BIG>::COLS ? left : Seq<BIG>::COLS;
     const int hd = a.head_dim;
-    constexpr int AHEAD = 12;  // parts whose loads are in flight together
-    for (int x = c0 * HD + threadIdx.x; x < c1 * HD; x += kThreads) {
-        const int c = x / HD, d = x % HD;
-        float top = -__builtin_inff(), sum = 0.0f, val = 0.0f;
+    constexpr int AHEAD = 8;  // parts whose loads are in flight together
+    for (int x = blockIdx.y * kThreads + threadIdx.x; x < cols * (HD / 4); x += gridDim.y * kThreads) {
+        const int c = x / (HD / 4), d = x % (HD / 4) * 4;
+        float top = -__builtin_inff(), sum = 0.0f;
+        f4 val = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int w = w0; w <= w_end; w += AHEAD) {
-            float m[AHEAD], l[AHEAD], v[AHEAD];
+            float m[AHEAD], l[AHEAD];
+            f4 v[AHEAD];
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) {
                 const int ww = w + i <= w_end ? w + i : w_end;
-                const float* part = part_at(a, ww, ww == w0, HD) + c * (HD + 2);
-                m[i] = part[0];
-                l[i] = part[1];
-                v[i] = part[2 + d];
+                float* part = part_at(a, ww, ww == w0, HD);
+                const float* ml = part_sums(a, part, HD) + 2 * c;
+                m[i] = ml[0];
+                l[i] = ml[1];
+                v[i] = *reinterpret_cast<const f4*>(part + c * HD + d);
             }
             float most = top;
 #pragma unroll
@@ -1040,17 +1100,17 @@ __global__ __launch_bounds__(kThreads) void join_q8_kernel(Q8Args a, int grid) {
                 if (w + i <= w_end && l[i] != 0.0f) {
                     const float f = __builtin_amdgcn_exp2f(m[i] - ref);
                     sum += f * l[i];
-                    val += f * v[i];
+                    val += v[i] * f;
                 }
             }
             top = most;
         }
         if (d < hd) {
             const int cc = col0 + c;
-            put<QT>(a.out,
-                    static_cast<int64_t>(s.row0 + cc / a.group) * a.ldo +
-                        static_cast<int64_t>(p[0].head * a.group + cc % a.group) * hd + d,
-                    sum != 0.0f ? val / sum : 0.0f);
+            const int64_t to = static_cast<int64_t>(s.row0 + cc / a.group) * a.ldo +
+                               static_cast<int64_t>(p[0].head * a.group + cc % a.group) * hd + d;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) put<QT>(a.out, to + i, sum != 0.0f ? val[i] / sum : 0.0f);
         }
     }
 }
@@ -1066,8 +1126,8 @@ int part_cols(int max_q_len, int group, bool is_big) {
 
 // Floats of the parts that the workgroups of one kernel may leave.
 int64_t part_floats(int max_q_len, int group, int head_dim, bool is_big) {
-    return static_cast<int64_t>(is_big ? kBigGrid : kGrid) * 2 * part_cols(max_q_len, group, is_big) *
-           (padded(head_dim) + 2);
+    return static_cast<int64_t>(is_big ? kBigGrid : kGrid) * 2 *
+           part_size(part_cols(max_q_len, group, is_big), padded(head_dim));
 }
 
 // Workgroups for at most `units` of work.
@@ -1088,8 +1148,8 @@ int attention_launch(Q8Args a, hipStream_t s) {
             grid_for((columns + kBigCols - 1) / kBigCols, a.n_kv_heads, positions, kBigUnit, a.batch, kBigGrid);
         if (const int st = launch(prompt_q8_kernel<TYPE, QT, HD>, dim3(grid), dim3(kThreads), 0, s, a)) return st;
         if (grid > 1)
-            if (const int st = launch(join_q8_kernel<QT, HD, true>, dim3(grid - 1, (a.part_cols + kJoinCols - 1) / kJoinCols),
-                                      dim3(kThreads), 0, s, a, static_cast<int>(grid)))
+            if (const int st = launch(join_q8_kernel<QT, HD, true>, dim3(grid - 1, 2), dim3(kThreads), 0, s, a,
+                                      static_cast<int>(grid)))
                 return st;
         a.ws += part_floats(a.max_q_len, a.group, a.head_dim, true);
     }
@@ -1158,7 +1218,7 @@ extern "C" int fence_gqa_attention_q8(void* out, const void* q, int type, int64_
                    cache->k_scale, cache->v_scale, block_table, kv_lens, q_start, static_cast<float*>(workspace),
                    cache->n_pages, __builtin_ctz(cache->page_size), cache->n_kv_heads, cache->head_dim, group,
                    max_blocks, batch, max_q_len, 0,
-                   static_cast<float>(scale * 1.4426950408889634)};
+                   static_cast<float>(scale * 1.4426950408889634), aligned(out, 16) && ldo * size % 16 == 0};
     if (cache->type == FENCE_KV_INT8)
         return type == FENCE_F32 ? attention_hd<FENCE_KV_INT8, FENCE_F32>(a, stream)
                                  : attention_hd<FENCE_KV_INT8, FENCE_F16>(a, stream);
