@@ -13,6 +13,16 @@
 
 #include <cmath>
 
+#ifndef FENCE_PRIO
+#define FENCE_PRIO 0
+#endif
+#ifndef FENCE_NC128
+#define FENCE_NC128 0
+#endif
+#ifndef FENCE_AHEAD
+#define FENCE_AHEAD 6
+#endif
+
 namespace fence {
 namespace {
 
@@ -23,11 +33,10 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
 // Columns of the products are the (row, head of the group) pairs of one kv
-// head; a sequence's are taken kCols or kBigCols at a time.
-constexpr int kCols = 16;              // attention_q8_kernel: each wave all of them, its own positions
-constexpr int kUnit = 32 * kWaves;     // and the positions its workgroup takes at a time
-constexpr int kBigCols = 32 * kWaves;  // prompt_q8_kernel: each wave 32 of them, all positions
-constexpr int kBigUnit = 64;
+// head; a sequence's are taken kCols or prompt_cols() at a time.
+constexpr int kCols = 16;           // attention_q8_kernel
+constexpr int kUnit = 32 * kWaves;  // positions its workgroup takes at a time
+constexpr int prompt_cols(int hd) { return FENCE_NC128 && hd <= 128 ? 256 : 128; }
 #ifndef FENCE_ATTN_Q8_ITEM
 #define FENCE_ATTN_Q8_ITEM 192
 #endif
@@ -72,12 +81,23 @@ __device__ __forceinline__ T uniform_load(const T* p, int64_t i) {
     return reinterpret_cast<const __attribute__((address_space(4))) T*>(reinterpret_cast<uintptr_t>(p))[i];
 }
 
-// A sequence as one of the two kernels sees it: rows = 0 if it is the other's.
-// Its work is counted in units, COLS columns of one kv head by UNIT positions.
-template <bool BIG>
+// The two kernels: work is counted in units, COLS columns of one kv head by
+// UNIT positions.
+struct Few {  // attention_q8_kernel: each wave all columns, its own positions
+    static constexpr bool MANY = false;
+    static constexpr int COLS = kCols, UNIT = kUnit;
+};
+template <int HD>
+struct Prompt {  // prompt_q8_kernel: each wave its own columns, all positions
+    static constexpr bool MANY = true;
+    static constexpr int COLS = prompt_cols(HD), UNIT = 64;
+};
+
+// A sequence as one of the kernels sees it: rows = 0 if it is the other's.
+template <class KIND>
 struct Seq {
-    static constexpr int COLS = BIG ? kBigCols : kCols;
-    static constexpr int UNIT = BIG ? kBigUnit : kUnit;
+    static constexpr bool BIG = KIND::MANY;
+    static constexpr int COLS = KIND::COLS, UNIT = KIND::UNIT;
     int row0, rows, q_len, kv, group;  // first row, rows computed, rows there are, positions
 
     __device__ __forceinline__ Seq(const Q8Args& a, int row, int row_end, int len) : row0(row), group(a.group) {
@@ -172,7 +192,7 @@ struct Place {
 // The place of each of N points at(i, total, grid) < total, by sums over the
 // batch, and the total; grid becomes the number of sharers.  Returns false
 // if there is no work or at(0, ..) is negative.
-template <bool BIG, int N, class F>
+template <class KIND, int N, class F>
 __device__ __forceinline__ bool find(const Q8Args& a, int* grid, int64_t* total, Place (&p)[N], F at) {
     __shared__ int64_t waves[kWaves];
     __shared__ int64_t found_before[N];
@@ -180,7 +200,7 @@ __device__ __forceinline__ bool find(const Q8Args& a, int* grid, int64_t* total,
     const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
     int64_t point[N], before[N];
     const auto all_of = [&](int b) {
-        return b < a.batch ? Seq<BIG>(a, a.q_start[b], a.q_start[b + 1], a.kv_lens[b]).all(a) : 0;
+        return b < a.batch ? Seq<KIND>(a, a.q_start[b], a.q_start[b + 1], a.kv_lens[b]).all(a) : 0;
     };
     const auto points = [&]() {
         *total = uniform64(*total);
@@ -191,7 +211,7 @@ __device__ __forceinline__ bool find(const Q8Args& a, int* grid, int64_t* total,
         return point[0] >= 0;
     };
     if (a.batch == 1) {
-        *total = Seq<BIG>::uniform(a, 0).all(a);
+        *total = Seq<KIND>::uniform(a, 0).all(a);
         if (!points()) return false;
 #pragma unroll
         for (int i = 0; i < N; ++i) p[i].seq = 0, before[i] = 0;
@@ -241,7 +261,7 @@ __device__ __forceinline__ bool find(const Q8Args& a, int* grid, int64_t* total,
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         p[i].seq = __builtin_amdgcn_readfirstlane(p[i].seq);
-        const Seq<BIG> s = Seq<BIG>::uniform(a, p[i].seq);
+        const Seq<KIND> s = Seq<KIND>::uniform(a, p[i].seq);
         const int64_t rest = point[i] - uniform64(before[i]);
         int lo = 0, hi = s.tiles() - 1;  // the last tile that begins at or before it
         while (lo < hi) {
@@ -256,14 +276,14 @@ __device__ __forceinline__ bool find(const Q8Args& a, int* grid, int64_t* total,
         p[i].head = __builtin_amdgcn_readfirstlane(static_cast<int>(quotient(in_tile, p[i].cost)));
         const int64_t off = in_tile - p[i].head * p[i].cost;
         p[i].item = point[i] - off;
-        const int unit = BIG ? static_cast<int>(quotient(off * p[i].units, p[i].cost)) : static_cast<int>(off);
+        const int unit = KIND::MANY ? static_cast<int>(quotient(off * p[i].units, p[i].cost)) : static_cast<int>(off);
         p[i].unit = __builtin_amdgcn_readfirstlane(unit);
     }
     return true;
 }
 
 // A workgroup's share: from one place to another.
-template <bool BIG>
+template <class KIND>
 struct Share {
     Place p;
     int end_seq, end_tile, end_head, end_unit;
@@ -275,7 +295,7 @@ struct Share {
         Place ends[2];
         // the last place is in front of the next workgroup's first; the last workgroup's is the end of all
         bool to_end = false;
-        if (!find<BIG, 2>(a, &grid, &total, ends, [&](int i, int64_t n, int g) -> int64_t {
+        if (!find<KIND, 2>(a, &grid, &total, ends, [&](int i, int64_t n, int g) -> int64_t {
                 if (me >= g) return -1;
                 if (i == 0) return cut(me, n, g);
                 to_end = me + 1 == g;
@@ -300,10 +320,10 @@ struct Share {
         p.unit = 0;
         if (++p.head < a.n_kv_heads) return true;
         p.head = 0;
-        Seq<BIG> s = Seq<BIG>::uniform(a, p.seq);
+        Seq<KIND> s = Seq<KIND>::uniform(a, p.seq);
         if (++p.tile == s.tiles()) {
             p.tile = 0;
-            do s = Seq<BIG>::uniform(a, ++p.seq);
+            do s = Seq<KIND>::uniform(a, ++p.seq);
             while (s.rows == 0);  // the end lies in a sequence behind
         }
         p.units = s.units(p.tile);
@@ -370,6 +390,18 @@ __device__ __forceinline__ void codes_h(uint32_t w, h2* lo, h2* hi) {
     }
 }
 
+// The larger of lanes l and l + 32, for both.  The two operands are exchanged
+// halfwise, so they have to be two registers; the empty asm keeps them apart.
+__device__ __forceinline__ float halves_max(float v) {
+    uint32_t x = __builtin_bit_cast(uint32_t, v), y = x;
+    asm volatile("" : "+v"(x), "+v"(y));
+    const auto r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+    x = r[0];
+    y = r[1];
+    asm volatile("" : "+v"(x), "+v"(y));
+    return fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
+}
+
 __device__ __forceinline__ h8 join(h2 a, h2 b, h2 c, h2 d) {
     return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
@@ -403,10 +435,10 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void attention_q8_kern
     const int r = lane % 16, g = lane / 16;
     const int hd = a.head_dim, page_mask = (1 << a.page_shift) - 1;
 
-    Share<false> share;
+    Share<Few> share;
     if (!share.find_mine(a)) return;
     do {
-        const Seq<false> s = Seq<false>::uniform(a, share.p.seq);
+        const Seq<Few> s = Seq<Few>::uniform(a, share.p.seq);
         const int tile = share.p.tile, head = share.p.head, first = share.p.unit, units = share.p.units;
         const int last = share.last();
         if (first >= last) continue;  // a share has at least one unit, but its end may be an item's beginning
@@ -670,9 +702,10 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void attention_q8_kern
     } while (share.next(a));
 }
 
-// Prompts: a workgroup takes kBigCols columns, 32 a wave, and 64 positions at
-// a time, whose codes it converts once into LDS for all of its columns:
-//   S' [32 positions x 32 columns] = K [32 x HD] Q' [HD x 32],  twice
+// Prompts: a workgroup takes 128 * NC columns, NC tiles of 32 a wave, and 64
+// positions at a time, whose codes it converts once into LDS for all of its
+// columns:
+//   S' [32 positions x 32 columns] = K [32 x HD] Q' [HD x 32],  twice a tile
 //   O' [HD x 32 columns] += V' [HD x 64 positions] P [64 x 32]
 // LDS holds the fragments as the products read them (16 bytes a lane, lanes in
 // a row, so reads and writes meet no bank twice).  The first product leaves
@@ -683,11 +716,15 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void attention_q8_kern
 // with runs of 4 * HD / 32 dimensions of its column.
 //
 // Wave w converts positions 16 w .. 16 w + 15, which lie in one page, so its
-// addresses are a scalar and a 32-bit offset a lane.  The next positions'
-// codes are loaded before the products of these and converted behind them
-// into the other half of LDS, with one barrier a turn.  Left to itself the
-// compiler reads one fragment, waits and multiplies, 32 times a turn; the
-// scheduling groups put the reads a few products ahead.
+// addresses are a scalar and a 32-bit offset a lane.  Codes are loaded two
+// turns ahead and converted one turn ahead, into the other half of LDS, with
+// one barrier a turn.  The vector pipe is the narrow one (an exponential is
+// 16 clocks, a conversion about 6 a code), and it can run behind a product
+// that takes 32 clocks, so the conversion stands beside the first products
+// and the exponentials of 16 positions beside the second products of the 16
+// before; the scheduling groups keep the compiler to that and its LDS reads
+// ahead.  Two column tiles a wave halve what a column pays for conversions,
+// loads and LDS reads.
 //
 // binary16 (QT = FENCE_F16): with the page's V scale in the exponent, one
 // fused multiply-add and one exponential make the probability that the
@@ -696,6 +733,8 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void attention_q8_kern
 // would grow past 2^15 (kSlack), so O is rarely rescaled.
 template <int TYPE, int QT, int HD>
 __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(Q8Args a) {
+    typedef Prompt<HD> Kind;
+    constexpr int NC = Kind::COLS / 128;
     constexpr bool F32 = QT == FENCE_F32;
     constexpr int PARTS = F32 ? 2 : 1;
     constexpr int KS = HD / 16;   // k steps of the first product
@@ -704,64 +743,78 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
     constexpr int VJ = HD <= 128 ? 1 : 2;  // 8 positions x 4 dimensions of V a lane converts
     constexpr float kBase = F32 ? 14.0f : 10.0f;  // log2 of what stands for 1 times the largest V scale
     constexpr float kSlack = F32 ? 0.0f : 4.0f;
-    __shared__ h8 kbuf[2][2][KS][kWave];
-    __shared__ h8 vbuf[2][4][NT][kWave];
-    __shared__ f4 sbuf[2][4];  // per 16 positions: K scale (-1 if the page is not there), V scale, its log2 and inverse
+    // A half of LDS in 16-byte pieces: K fragments [2][KS][64 lanes], V fragments [4][NT][64 lanes], per 16
+    // positions K scale (-1 if the page is not there), V scale, its log2 and inverse, and a place for each lane to
+    // write what nobody reads.
+    constexpr int V0 = 2 * KS * kWave, S0 = V0 + 4 * NT * kWave, X0 = S0 + 4, HALF = X0 + kWave;
+    __shared__ h8 buf[2 * HALF];
     const int tid = threadIdx.x, lane = tid % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int n = lane % 32, g = lane / 32;
     const int hd = a.head_dim, page_mask = (1 << a.page_shift) - 1;
 
-    Share<true> share;
+    Share<Kind> share;
     if (!share.find_mine(a)) return;
-    // what this lane converts: K position lane % 16, dimensions 16 (lane / 16 + 4 j) on; V positions 4 vg + (0 .. 3)
-    // and 8 more, dimensions vd on
+    // What this lane converts: K position lane % 16, dimensions 16 (lane / 16 + 4 j) on; V positions 4 vg + (0 .. 3)
+    // and 8 more, dimensions vd on.  At HD = 64 the upper lanes load the V that the lower ones do.
     const int kr = lane % 16, kc = lane / 16;
     const int vd = HD == 256 ? lane * 4 : lane % (HD / 4) * 4;
-    const int vg = HD == 256 ? 0 : lane / (HD / 4) % 2;  // at HD = 64 the upper lanes load what the lower ones do
+    const int vg = HD == 256 ? 0 : lane / (HD / 4) % 2;
     const bool vmine = (HD == 64 ? lane < 32 : true) && vd < hd;
+    int kto[KJ], vto[4], sto;  // where to
+#pragma unroll
+    for (int j = 0; j < KJ; ++j)
+        kto[j] = (kc + 4 * j) * 16 < hd ? (wave / 2 * KS + kc + 4 * j) * kWave + (wave % 2) * 16 + kr : X0 + kr;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        vto[i] = vmine ? V0 + (wave * NT + (vd + i) % NT) * kWave + vg * 32 + (vd + i) / NT : -1;
+    sto = lane == 0 ? S0 + wave : X0 + lane;
     if (hd < HD) {  // dimensions that are not there stay zero
         const h8 zero = {};
-        for (int i = tid; i < 2 * 2 * KS * kWave; i += kThreads) (&kbuf[0][0][0][0])[i] = zero;
-        for (int i = tid; i < 2 * 4 * NT * kWave; i += kThreads) (&vbuf[0][0][0][0])[i] = zero;
+        for (int i = tid; i < 2 * HALF; i += kThreads) buf[i] = zero;
         __syncthreads();
     }
     do {
-        const Seq<true> s = Seq<true>::uniform(a, share.p.seq);
+        const Seq<Kind> s = Seq<Kind>::uniform(a, share.p.seq);
         const int tile = share.p.tile, head = share.p.head, first = share.p.unit, units = share.p.units;
         const int last = share.last();
-        const int cols = s.rows * a.group - tile * kBigCols;
-        const int c = wave * 32 + n;  // this lane's column
-        const bool mine = c < cols;
-        const int row = (tile * kBigCols + c) / a.group;
-        const int qhead = head * a.group + (tile * kBigCols + c) % a.group;
-        const int sees = mine ? s.row_sees(row) : 0;
+        const int cols = s.rows * a.group - tile * Kind::COLS;
+        int c[NC], row[NC], qhead[NC], sees[NC];  // this lane's columns
+        bool mine[NC];
+#pragma unroll
+        for (int x = 0; x < NC; ++x) {
+            c[x] = (wave * NC + x) * 32 + n;
+            mine[x] = c[x] < cols;
+            row[x] = (tile * Kind::COLS + c[x]) / a.group;
+            qhead[x] = head * a.group + (tile * Kind::COLS + c[x]) % a.group;
+            sees[x] = mine[x] ? s.row_sees(row[x]) : 0;
+        }
         const int end = s.sees(tile);
         if (first >= last) {
             // Nothing of this item; if others take what is before and after, the join finds an empty part.
-            if (first > 0 && mine && g == 0) {
-                float* ml = part_sums(a, part_at(a, blockIdx.x, false, HD), HD) + 2 * c;
-                ml[0] = -__builtin_inff(), ml[1] = 0.0f;
-            }
+            float* ml = part_sums(a, part_at(a, blockIdx.x, false, HD), HD);
+#pragma unroll
+            for (int x = 0; x < NC; ++x)
+                if (first > 0 && mine[x] && g == 0) ml[2 * c[x]] = -__builtin_inff(), ml[2 * c[x] + 1] = 0.0f;
             continue;
         }
-        const int least = s.row_sees((tile * kBigCols + wave * 32) / a.group);  // what every column of this wave sees
+        // what every column of this wave sees
+        const int least = s.row_sees((tile * Kind::COLS + wave * NC * 32) / a.group);
         const int64_t table = static_cast<int64_t>(share.p.seq) * a.max_blocks;
 
         // The page of this wave's 16 positions of a unit.
         const auto page_of = [&](int un) {
-            const int pos = un * kBigUnit + wave * 16;
-            return un < last && pos < end ? uniform_load(a.table, table + (pos >> a.page_shift)) : -1;
+            const int pos = un * Kind::UNIT + wave * 16;
+            const int id = un < last && pos < end ? uniform_load(a.table, table + (pos >> a.page_shift)) : -1;
+            return id < a.n_pages ? id : -1;
         };
         u4 kw[KJ];
         uint32_t vw[VJ][8];
         float ks, vs;
+        // the codes of a unit, of page 0 if the page is not there
         const auto load = [&](int un, int id) {
-            const bool there = id >= 0 && id < a.n_pages;
-            const int64_t base = static_cast<int64_t>(there ? id : 0) * a.n_kv_heads + head;
-            ks = there ? uniform_load(a.ks, base) : -1.0f;
-            vs = there ? uniform_load(a.vs, base) : 0.0f;
-            const int64_t at = ((base << a.page_shift) + ((un * kBigUnit + wave * 16) & page_mask)) * hd;
+            const int64_t base = static_cast<int64_t>(id < 0 ? 0 : id) * a.n_kv_heads + head;
+            const int64_t at = ((base << a.page_shift) + ((un * Kind::UNIT + wave * 16) & page_mask)) * hd;
             const uint8_t* k = a.k + at;
             const uint8_t* v = a.v + at;
 #pragma unroll
@@ -777,60 +830,68 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
                         v + ((i / 4) * 8 + i % 4) * hd +
                         (static_cast<uint32_t>((vg + j) * 4 * hd) + static_cast<uint32_t>(vd < hd ? vd : 0)));
         };
-        // Into half `half` of LDS.  Positions past the end, and pages whose V scale is 0, get V codes of 0.
-        const auto convert = [&](int un, int half) {
-            const int pos0 = un * kBigUnit + wave * 16;
-#pragma unroll
-            for (int j = 0; j < KJ; ++j) {
-                const int k = kc + 4 * j;
-                if (k * 16 < hd) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        h2 c0, c1, c2, c3;
-                        codes_h<TYPE>(kw[j][2 * i], &c0, &c1);
-                        codes_h<TYPE>(kw[j][2 * i + 1], &c2, &c3);
-                        kbuf[half][wave / 2][k][i * 32 + (wave % 2) * 16 + kr] = join(c0, c1, c2, c3);
-                    }
-                }
-            }
-            if (vs == 0.0f || pos0 + 16 > end) {
+        const auto scales = [&](int id) {
+            const int64_t base = static_cast<int64_t>(id < 0 ? 0 : id) * a.n_kv_heads + head;
+            const float x = uniform_load(a.ks, base), y = uniform_load(a.vs, base);
+            ks = id < 0 ? -1.0f : x;
+            vs = id < 0 ? 0.0f : y;
+        };
+        // V codes of positions past the end: an e4m3 one may be NaN, which no weight of 0 removes.
+        const auto trim = [&](int un) {
+            const int pos0 = un * Kind::UNIT + wave * 16;
+            if (TYPE == FENCE_KV_E4M3 && pos0 + 16 > end) {
 #pragma unroll
                 for (int j = 0; j < VJ; ++j)
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        if (vs == 0.0f || pos0 + (vg + j) * 4 + (i / 4) * 8 + i % 4 >= end) vw[j][i] = 0;
+                        if (pos0 + (vg + j) * 4 + (i / 4) * 8 + i % 4 >= end) vw[j][i] = 0;
             }
+        };
+        // Into a half of LDS.  V codes of pages that are not there or whose scale is 0 become 0.
+        const auto convert = [&](h8* half) {
+#pragma unroll
+            for (int j = 0; j < KJ; ++j)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    h2 c0, c1, c2, c3;
+                    codes_h<TYPE>(kw[j][2 * i], &c0, &c1);
+                    codes_h<TYPE>(kw[j][2 * i + 1], &c2, &c3);
+                    half[kto[j] + i * 32] = join(c0, c1, c2, c3);
+                }
+            const uint32_t keep = vs == 0.0f ? 0u : ~0u;
 #pragma unroll
             for (int j = 0; j < VJ; ++j) {
                 h2 x[4][4];
 #pragma unroll
                 for (int p = 0; p < 4; ++p) {
-                    const uint32_t y = vw[j][2 * p], z = vw[j][2 * p + 1];
+                    const uint32_t y = vw[j][2 * p] & keep, z = vw[j][2 * p + 1] & keep;
                     codes_h<TYPE>(__builtin_amdgcn_perm(z, y, 0x05010400u), &x[p][0], &x[p][1]);
                     codes_h<TYPE>(__builtin_amdgcn_perm(z, y, 0x07030602u), &x[p][2], &x[p][3]);
                 }
-                if (vmine) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        vbuf[half][wave][(vd + i) % NT][(vg + j) * 32 + (vd + i) / NT] =
-                            join(x[0][i], x[1][i], x[2][i], x[3][i]);
-                }
+                for (int i = 0; i < 4; ++i)
+                    half[vto[i] < 0 ? X0 + lane : vto[i] + j * 32] = join(x[0][i], x[1][i], x[2][i], x[3][i]);
             }
-            if (lane == 0) sbuf[half][wave] = f4{ks, vs, __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs)};
+            *reinterpret_cast<f4*>(half + sto) = f4{ks, vs, __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs)};
         };
 
-        load(first, page_of(first));
-        int id_next = page_of(first + 1);
+        int id_next = page_of(first);
+        load(first, id_next);
+        scales(id_next);
+        id_next = page_of(first + 1);
 
-        h8 qf[PARTS][KS];
-        float unscale = a.scale_log2;
-        {
-            const int64_t from = mine ? static_cast<int64_t>(s.row0 + row) * a.ldq + static_cast<int64_t>(qhead) * hd : 0;
+        h8 qf[NC][PARTS][KS];
+        float unscale[NC];
+#pragma unroll
+        for (int x = 0; x < NC; ++x) {
+            unscale[x] = a.scale_log2;
+            const int64_t from =
+                mine[x] ? static_cast<int64_t>(s.row0 + row[x]) * a.ldq + static_cast<int64_t>(qhead[x]) * hd : 0;
             if constexpr (F32) {
                 float biggest = 0.0f;
 #pragma unroll
                 for (int k = 0; k < KS; ++k)
-                    if (mine && k * 16 < hd) {
+                    if (mine[x] && k * 16 < hd) {
                         const float* src = static_cast<const float*>(a.q) + from + k * 16 + g * 8;
 #pragma unroll
                         for (int i = 0; i < 8; ++i) biggest = fmaxf(biggest, fabsf(src[i]));
@@ -839,201 +900,234 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
                 uint32_t e = __builtin_bit_cast(uint32_t, biggest) >> 23;
                 e = e < 15 ? 15 : e > 254 ? 254 : e;
                 const float up = __builtin_bit_cast(float, (268 - e) << 23);
-                unscale *= __builtin_bit_cast(float, (e - 14) << 23);
+                unscale[x] *= __builtin_bit_cast(float, (e - 14) << 23);
 #pragma unroll
                 for (int k = 0; k < KS; ++k) {
                     const float* src = static_cast<const float*>(a.q) + from + k * 16 + g * 8;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         _Float16 hi, lo;
-                        split(mine && k * 16 < hd ? src[i] * up : 0.0f, &hi, &lo);
-                        qf[0][k][i] = hi;
-                        qf[1][k][i] = lo;
+                        split(mine[x] && k * 16 < hd ? src[i] * up : 0.0f, &hi, &lo);
+                        qf[x][0][k][i] = hi;
+                        qf[x][1][k][i] = lo;
                     }
                 }
             } else {
 #pragma unroll
                 for (int k = 0; k < KS; ++k) {
-                    h8 x = {};
-                    if (mine && k * 16 < hd) {
+                    h8 y = {};
+                    if (mine[x] && k * 16 < hd) {
                         const _Float16* src = static_cast<const _Float16*>(a.q) + from + k * 16 + g * 8;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) x[i] = src[i];
+                        for (int i = 0; i < 8; ++i) y[i] = src[i];
                     }
-                    qf[0][k] = x;
+                    qf[x][0][k] = y;
                 }
             }
         }
 
-        f16v o[NT];
+        f16v o[NC][NT];
+        float m[NC], l[NC], vref = 0.0f;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int x = 0; x < NC; ++x) {
+            m[x] = -__builtin_inff();
+            l[x] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
-        float m = -__builtin_inff(), l = 0.0f, vref = 0.0f;
-        convert(first, first & 1);
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[x][t][i] = 0.0f;
+        }
+        trim(first);
+        convert(buf + (first & 1) * HALF);
+        load(first + 1, id_next);
+        scales(id_next);
+        id_next = page_of(first + 2);
         __syncthreads();
 
         const auto turn = [&](int un, auto masked) {
-            const int half = un & 1, pos0 = un * kBigUnit;
-            if (un + 1 < last) load(un + 1, id_next);
-            id_next = page_of(un + 2);
-            f16v st[2];
+            const h8* half = buf + (un & 1) * HALF;
+            const int pos0 = un * Kind::UNIT;
+            trim(un + 1);
+            f16v st[NC][2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int x = 0; x < NC; ++x)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) st[h][i] = 0.0f;
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) st[x][h][i] = 0.0f;
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int k = 0; k < KS; ++k)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const h8 kf = kbuf[half][h][k][lane];
+                    const h8 kf = half[(h * KS + k) * kWave + lane];
 #pragma unroll
-                    for (int x = 0; x < PARTS; ++x)
-                        st[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[x][k], st[h], 0, 0, 0);
+                    for (int x = 0; x < NC; ++x)
+#pragma unroll
+                        for (int p = 0; p < PARTS; ++p)
+                            st[x][h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[x][p][k], st[x][h], 0, 0, 0);
                 }
             f4 sc[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) sc[q] = sbuf[half][q];
-            // reads kAhead fragments ahead of the products
-            constexpr int kAhead = F32 ? 4 : 6;
-            __builtin_amdgcn_sched_group_barrier(0x100, kAhead + 4, 0);
+            for (int q = 0; q < 4; ++q) sc[q] = *reinterpret_cast<const f4*>(half + S0 + q);
+            convert(buf + ((un + 1) & 1) * HALF);
+            // LDS reads kAhead fragments ahead of the products, and the conversion between them
+            constexpr int kAhead = 4, kEach = 128 * HD / 128 / (2 * KS) + 1;
+            __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
-            for (int i = 0; i < 2 * KS - kAhead; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, PARTS, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            for (int i = 0; i < 2 * KS; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, NC * PARTS, 0);
+                if (i < 2 * KS - kAhead + 4) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, kEach, 0);
+                __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
             }
-            __builtin_amdgcn_sched_group_barrier(0x008, kAhead * PARTS, 0);
             __builtin_amdgcn_sched_barrier(0);
+            load(un + 2, id_next);
+            // Scalar loads here, where no LDS read is waited for: with one in flight such a wait is for all.
+            scales(id_next);
+            id_next = page_of(un + 3);
 
-            float fk[4];
             bool in[4];
+            float vtop = vref;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 in[q] = !(sc[q][0] < 0.0f);
-                fk[q] = sc[q][0] * unscale;
-            }
-            const int limit = sees - pos0 - g * 4;  // of this lane's positions: see, those below it
-            const auto seen = [&](int h, int i) { return h * 32 + (i / 4) * 8 + i % 4 < limit; };
-            if (masked) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (!seen(h, i)) st[h][i] = -__builtin_inff();
-            }
-            float top = -__builtin_inff();
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                float t = st[q / 2][(q % 2) * 8];
-#pragma unroll
-                for (int i = 1; i < 8; ++i) t = fmaxf(t, st[q / 2][(q % 2) * 8 + i]);
-                // scales are not negative, so the largest product is the largest score
-                t = in[q] && t > -__builtin_inff() ? t * fk[q] : -__builtin_inff();
-                top = fmaxf(top, t);
-            }
-            top = fmaxf(top, __shfl_xor(top, 32));
-            float vtop = vref;
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
                 if (sc[q][1] > vtop && sc[q][1] < __builtin_inff()) vtop = sc[q][1];
-            const bool grow_v = vtop > (F32 ? vref : 2.0f * vref);
-            if (__any(top > m + kSlack || grow_v)) {
-                const float now = fmaxf(m, top);
-                const float alpha = now == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - now);
-                const float vnow = grow_v ? vtop : vref;
-                const float beta = vnow > 0.0f ? alpha * (vref * __builtin_amdgcn_rcpf(vnow)) : 0.0f;
-                m = now;
-                vref = vnow;
-                l *= alpha;
-#pragma unroll
-                for (int t = 0; t < NT; ++t) o[t] *= beta;
             }
-            const float ref = m == -__builtin_inff() ? 0.0f : m;
-            const float vone = vref > 0.0f ? __builtin_amdgcn_rcpf(vref) : 0.0f;
-            const float vlog = vref > 0.0f ? __builtin_amdgcn_logf(vref) : 0.0f;
+            const bool grow_v = vtop > (F32 ? vref : 2.0f * vref);
+            const float vnow = grow_v ? vtop : vref;
+            const float vone = vnow > 0.0f ? __builtin_amdgcn_rcpf(vnow) : 0.0f;
+            const float vlog = vnow > 0.0f ? __builtin_amdgcn_logf(vnow) : 0.0f;
+            float top[NC];
+            bool move = grow_v;
+            int limit[NC];  // of this lane's positions: those below it are seen
+            const auto seen = [&](int x, int h, int i) { return h * 32 + (i / 4) * 8 + i % 4 < limit[x]; };
+#pragma unroll
+            for (int x = 0; x < NC; ++x) {
+                limit[x] = sees[x] - pos0 - g * 4;
+                if (masked) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (!seen(x, h, i)) st[x][h][i] = -__builtin_inff();
+                }
+                top[x] = -__builtin_inff();
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    float t = st[x][q / 2][(q % 2) * 8];
+#pragma unroll
+                    for (int i = 1; i < 8; ++i) t = fmaxf(t, st[x][q / 2][(q % 2) * 8 + i]);
+                    // scales are not negative, so the largest product is the largest score
+                    t = in[q] && t > -__builtin_inff() ? t * (sc[q][0] * unscale[x]) : -__builtin_inff();
+                    top[x] = fmaxf(top[x], t);
+                }
+                top[x] = halves_max(top[x]);
+                move |= top[x] > m[x] + kSlack;
+            }
+            if (__any(move)) {
+#pragma unroll
+                for (int x = 0; x < NC; ++x) {
+                    const float now = fmaxf(m[x], top[x]);
+                    const float alpha = now == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m[x] - now);
+                    const float beta = alpha * (vref * vone);
+                    m[x] = now;
+                    l[x] *= alpha;
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) o[x][t] *= beta;
+                }
+                vref = vnow;
+            }
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                h8 pf[PARTS];
-                if constexpr (F32) {
-                    const float to_v = sc[q][1] * vone * 16384.0f;
+                h8 pf[NC][PARTS];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        float x = __builtin_amdgcn_exp2f(st[q / 2][(q % 2) * 8 + i] * fk[q] - ref);
-                        if (!in[q] || (masked && !seen(q / 2, (q % 2) * 8 + i))) x = 0.0f;
-                        l += x;
-                        const float y = masked && x == 0.0f ? 0.0f : x * to_v;
-                        _Float16 hi, lo;
-                        split(y, &hi, &lo);
-                        pf[0][i] = hi;
-                        pf[PARTS - 1][i] = lo;
-                    }
-                } else {
-                    const bool none = sc[q][1] == 0.0f;  // its V codes are zero: any weight will do that can be taken back
-                    const float shift = in[q] ? (none ? 0.0f : sc[q][2] - vlog) + (kBase - ref) : -__builtin_inff();
-                    float x[8];
+                for (int x = 0; x < NC; ++x) {
+                    const float ref = m[x] == -__builtin_inff() ? 0.0f : m[x];
+                    const float fk = sc[q][0] * unscale[x];
+                    if constexpr (F32) {
+                        const float to_v = sc[q][1] * vone * 16384.0f;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[q / 2][(q % 2) * 8 + i], fk[q], shift));
-                        if (masked && !seen(q / 2, (q % 2) * 8 + i)) x[i] = 0.0f;
-                    }
-                    float sum = 0.0f;
+                        for (int i = 0; i < 8; ++i) {
+                            float p = __builtin_amdgcn_exp2f(st[x][q / 2][(q % 2) * 8 + i] * fk - ref);
+                            if (!in[q] || (masked && !seen(x, q / 2, (q % 2) * 8 + i))) p = 0.0f;
+                            l[x] += p;
+                            const float y = masked && p == 0.0f ? 0.0f : p * to_v;
+                            _Float16 hi, lo;
+                            split(y, &hi, &lo);
+                            pf[x][0][i] = hi;
+                            pf[x][PARTS - 1][i] = lo;
+                        }
+                    } else {
+                        // V codes under a scale of 0 are zero: any weight will do that can be taken back
+                        const bool none = sc[q][1] == 0.0f;
+                        const float shift = in[q] ? (none ? 0.0f : sc[q][2] - vlog) + (kBase - ref) : -__builtin_inff();
+                        float p[8];
 #pragma unroll
-                    for (int i = 0; i < 8; i += 2) {
-                        const h2 y = {static_cast<_Float16>(x[i]), static_cast<_Float16>(x[i + 1])};
-                        pf[0][i] = y[0];
-                        pf[0][i + 1] = y[1];
-                        const h2 ones = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
-                        sum = __builtin_amdgcn_fdot2(y, ones, sum, false);
+                        for (int i = 0; i < 8; ++i) {
+                            p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x][q / 2][(q % 2) * 8 + i], fk, shift));
+                            if (masked && !seen(x, q / 2, (q % 2) * 8 + i)) p[i] = 0.0f;
+                        }
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 8; i += 2) {
+                            const h2 y = {static_cast<_Float16>(p[i]), static_cast<_Float16>(p[i + 1])};
+                            pf[x][0][i] = y[0];
+                            pf[x][0][i + 1] = y[1];
+                            const h2 ones = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
+                            sum = __builtin_amdgcn_fdot2(y, ones, sum, false);
+                        }
+                        l[x] += sum * (none ? 0x1p-10f : 0x1p-10f * (vnow * sc[q][3]));
                     }
-                    l += sum * (none ? 0x1p-10f : 0x1p-10f * (vref * sc[q][3]));
                 }
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    const h8 vf = vbuf[half][q][t][lane];
+                    const h8 vf = half[V0 + (q * NT + t) * kWave + lane];
 #pragma unroll
-                    for (int x = 0; x < PARTS; ++x)
-                        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[x], o[t], 0, 0, 0);
+                    for (int x = 0; x < NC; ++x)
+#pragma unroll
+                        for (int p = 0; p < PARTS; ++p)
+                            o[x][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[x][p], o[x][t], 0, 0, 0);
                 }
             }
-            if (un + 1 < last) convert(un + 1, half ^ 1);
             __syncthreads();
         };
         // The waves turn together; each masks from where its first column ends.
         int un = first;
 #pragma unroll 1
-        for (; un < last && (un + 1) * kBigUnit <= least; ++un) turn(un, std::false_type{});
+        for (; un < last && (un + 1) * Kind::UNIT <= least; ++un) turn(un, std::false_type{});
 #pragma unroll 1
         for (; un < last; ++un) turn(un, std::true_type{});
 
-        // o[t][i] is dimension (8 (i / 4) + 4 g + i % 4) * NT + t of this lane's column: runs of 4 NT.
-        l += __shfl_xor(l, 32);
+        // o[x][t][i] is dimension (8 (i / 4) + 4 g + i % 4) * NT + t of this lane's column: runs of 4 NT.
         const float unit_v = vref * (F32 ? 0x1p-14f : 0x1p-10f);
-        if (mine) {
-            const bool whole = first == 0 && last == units;
-            const float f = whole ? (l != 0.0f ? unit_v / l : 0.0f) : unit_v;
+        const bool whole = first == 0 && last == units;
+#pragma unroll
+        for (int x = 0; x < NC; ++x) {
+            const float sum = l[x] + __shfl_xor(l[x], 32);
+            if (!mine[x]) continue;
+            const float f = whole ? (sum != 0.0f ? unit_v / sum : 0.0f) : unit_v;
             float* part = part_at(a, blockIdx.x, first == 0, HD);
-            const int64_t to = static_cast<int64_t>(s.row0 + row) * a.ldo + static_cast<int64_t>(qhead) * hd;
+            const int64_t to = static_cast<int64_t>(s.row0 + row[x]) * a.ldo + static_cast<int64_t>(qhead[x]) * hd;
             if (!whole && g == 0) {
-                float* ml = part_sums(a, part, HD) + 2 * c;
-                ml[0] = m, ml[1] = l;
+                float* ml = part_sums(a, part, HD) + 2 * c[x];
+                ml[0] = m[x], ml[1] = sum;
             }
 #pragma unroll
             for (int q = 0; q < 4; ++q)
 #pragma unroll
-                for (int x = 0; x < 4 * NT; x += 8) {
-                    const int d = (8 * q + 4 * g) * NT + x;
+                for (int z = 0; z < 4 * NT; z += 8) {
+                    const int d = (8 * q + 4 * g) * NT + z;
                     float y[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const int j = (x + i) / NT, t = (x + i) % NT;
-                        y[i] = whole && l == 0.0f ? 0.0f : o[t][4 * q + j] * f;
+                        const int j = (z + i) / NT, t = (z + i) % NT;
+                        y[i] = whole && sum == 0.0f ? 0.0f : o[x][t][4 * q + j] * f;
                     }
                     if (whole) {
                         if (d < hd) put8<QT>(a, to + d, y);
                     } else {
-                        float* p = part + c * HD + d;
+                        float* p = part + c[x] * HD + d;
                         *reinterpret_cast<f4*>(p) = f4{y[0], y[1], y[2], y[3]};
                         *reinterpret_cast<f4*>(p + 4) = f4{y[4], y[5], y[6], y[7]};
                     }
@@ -1047,28 +1141,28 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
 // the other kernel: if it is the first border inside an item, the item's
 // columns are its to join, together with the other workgroups of the same x,
 // a run of 4 dimensions a thread.
-template <int QT, int HD, bool BIG>
+template <int QT, int HD, class KIND>
 __global__ __launch_bounds__(kThreads) void join_q8_kernel(Q8Args a, int grid) {
     const int w0 = blockIdx.x;
     int64_t total;
     Place p[1];
-    if (!find<BIG, 1>(a, &grid, &total, p, [&](int, int64_t n, int g) -> int64_t {
+    if (!find<KIND, 1>(a, &grid, &total, p, [&](int, int64_t n, int g) -> int64_t {
             return w0 + 1 < g ? cut(w0 + 1, n, g) : -1;
         }))
         return;
     if (p[0].unit == 0) return;
     const int64_t off0 = cut(w0, total, grid) - p[0].item;  // the border before
-    if (off0 > 0 && (BIG ? quotient(off0 * p[0].units, p[0].cost) : off0) > 0) return;
+    if (off0 > 0 && (KIND::MANY ? quotient(off0 * p[0].units, p[0].cost) : off0) > 0) return;
     // the workgroup whose share holds the item's end
     const int64_t end = p[0].item + p[0].cost;
     int w_end = static_cast<int>(quotient(end * grid - 1, total));
     while (w_end + 1 < grid && cut(w_end + 1, total, grid) < end) ++w_end;
     while (w_end > w0 + 1 && cut(w_end, total, grid) >= end) --w_end;
     w_end = __builtin_amdgcn_readfirstlane(w_end);
-    const Seq<BIG> s = Seq<BIG>::uniform(a, p[0].seq);
-    const int col0 = p[0].tile * Seq<BIG>::COLS;
+    const Seq<KIND> s = Seq<KIND>::uniform(a, p[0].seq);
+    const int col0 = p[0].tile * Seq<KIND>::COLS;
     const int left = s.rows * a.group - col0;
-    const int cols = left < Seq<BIG>::COLS ? left : Seq<BIG>::COLS;
+    const int cols = left < Seq<KIND>::COLS ? left : Seq<KIND>::COLS;
     const int hd = a.head_dim;
     constexpr int AHEAD = 8;  // parts whose loads are in flight together
     for (int x = blockIdx.y * kThreads + threadIdx.x; x < cols * (HD / 4); x += gridDim.y * kThreads) {
@@ -1119,15 +1213,15 @@ int padded(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 
 
 bool big(int max_q_len, int group) { return static_cast<int64_t>(max_q_len) * group > kSmall; }
 
-int part_cols(int max_q_len, int group, bool is_big) {
-    const int64_t most = is_big ? kBigCols : kCols, n = static_cast<int64_t>(max_q_len) * group;
+int part_cols(int max_q_len, int group, int head_dim, bool is_big) {
+    const int64_t most = is_big ? prompt_cols(head_dim) : kCols, n = static_cast<int64_t>(max_q_len) * group;
     return static_cast<int>(n < most ? n : most);
 }
 
 // Floats of the parts that the workgroups of one kernel may leave.
 int64_t part_floats(int max_q_len, int group, int head_dim, bool is_big) {
     return static_cast<int64_t>(is_big ? kBigGrid : kGrid) * 2 *
-           part_size(part_cols(max_q_len, group, is_big), padded(head_dim));
+           part_size(part_cols(max_q_len, group, head_dim, is_big), padded(head_dim));
 }
 
 // Workgroups for at most `units` of work.
@@ -1143,23 +1237,24 @@ int attention_launch(Q8Args a, hipStream_t s) {
     const int64_t columns = static_cast<int64_t>(a.max_q_len) * a.group;
     const int64_t positions = static_cast<int64_t>(a.max_blocks) << a.page_shift;
     if (both) {
-        a.part_cols = part_cols(a.max_q_len, a.group, true);
+        a.part_cols = part_cols(a.max_q_len, a.group, a.head_dim, true);
         const unsigned grid =
-            grid_for((columns + kBigCols - 1) / kBigCols, a.n_kv_heads, positions, kBigUnit, a.batch, kBigGrid);
+            grid_for((columns + Prompt<HD>::COLS - 1) / Prompt<HD>::COLS, a.n_kv_heads, positions, Prompt<HD>::UNIT,
+                     a.batch, kBigGrid);
         if (const int st = launch(prompt_q8_kernel<TYPE, QT, HD>, dim3(grid), dim3(kThreads), 0, s, a)) return st;
         if (grid > 1)
-            if (const int st = launch(join_q8_kernel<QT, HD, true>, dim3(grid - 1, 2), dim3(kThreads), 0, s, a,
+            if (const int st = launch(join_q8_kernel<QT, HD, Prompt<HD>>, dim3(grid - 1, 2), dim3(kThreads), 0, s, a,
                                       static_cast<int>(grid)))
                 return st;
         a.ws += part_floats(a.max_q_len, a.group, a.head_dim, true);
     }
     const int64_t small = columns < kSmall ? columns : kSmall;
-    a.part_cols = part_cols(a.max_q_len, a.group, false);
+    a.part_cols = part_cols(a.max_q_len, a.group, a.head_dim, false);
     const unsigned grid = grid_for((small + kCols - 1) / kCols, a.n_kv_heads, positions, kUnit, a.batch, kGrid);
     const size_t shmem = static_cast<size_t>(kWaves) * a.part_cols * (HD + 2) * sizeof(float);
     if (const int st = launch(attention_q8_kernel<TYPE, QT, HD>, dim3(grid), dim3(kThreads), shmem, s, a)) return st;
     if (grid == 1) return FENCE_SUCCESS;
-    return launch(join_q8_kernel<QT, HD, false>, dim3(grid - 1), dim3(kThreads), 0, s, a, static_cast<int>(grid));
+    return launch(join_q8_kernel<QT, HD, Few>, dim3(grid - 1), dim3(kThreads), 0, s, a, static_cast<int>(grid));
 }
 
 template <int TYPE, int QT>
