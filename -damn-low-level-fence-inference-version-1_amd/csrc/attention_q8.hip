@@ -13,15 +13,6 @@
 
 #include <cmath>
 
-#ifndef FENCE_PRIO
-#define FENCE_PRIO 0
-#endif
-#ifndef FENCE_NC128
-#define FENCE_NC128 0
-#endif
-#ifndef FENCE_AHEAD
-#define FENCE_AHEAD 6
-#endif
 
 namespace fence {
 namespace {
@@ -33,12 +24,12 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
 // Columns of the products are the (row, head of the group) pairs of one kv
-// head; a sequence's are taken kCols or prompt_cols() at a time.
+// head; a sequence's are taken kCols or kPromptCols at a time.
 constexpr int kCols = 16;           // attention_q8_kernel
 constexpr int kUnit = 32 * kWaves;  // positions its workgroup takes at a time
-constexpr int prompt_cols(int hd) { return FENCE_NC128 && hd <= 128 ? 256 : 128; }
+constexpr int kPromptCols = 32 * kWaves;  // prompt_q8_kernel
 #ifndef FENCE_ATTN_Q8_ITEM
-#define FENCE_ATTN_Q8_ITEM 192
+#define FENCE_ATTN_Q8_ITEM 384
 #endif
 constexpr int kBigItem = FENCE_ATTN_Q8_ITEM;  // what an item costs besides its positions, in positions
 // Up to this many columns a sequence goes to attention_q8_kernel.
@@ -87,10 +78,9 @@ struct Few {  // attention_q8_kernel: each wave all columns, its own positions
     static constexpr bool MANY = false;
     static constexpr int COLS = kCols, UNIT = kUnit;
 };
-template <int HD>
 struct Prompt {  // prompt_q8_kernel: each wave its own columns, all positions
     static constexpr bool MANY = true;
-    static constexpr int COLS = prompt_cols(HD), UNIT = 64;
+    static constexpr int COLS = kPromptCols, UNIT = 64;
 };
 
 // A sequence as one of the kernels sees it: rows = 0 if it is the other's.
@@ -702,10 +692,9 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void attention_q8_kern
     } while (share.next(a));
 }
 
-// Prompts: a workgroup takes 128 * NC columns, NC tiles of 32 a wave, and 64
-// positions at a time, whose codes it converts once into LDS for all of its
-// columns:
-//   S' [32 positions x 32 columns] = K [32 x HD] Q' [HD x 32],  twice a tile
+// Prompts: a workgroup takes kPromptCols columns, 32 a wave, and 64 positions
+// at a time, whose codes it converts once into LDS for all of its columns:
+//   S' [32 positions x 32 columns] = K [32 x HD] Q' [HD x 32],  twice
 //   O' [HD x 32 columns] += V' [HD x 64 positions] P [64 x 32]
 // LDS holds the fragments as the products read them (16 bytes a lane, lanes in
 // a row, so reads and writes meet no bank twice).  The first product leaves
@@ -723,8 +712,9 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void attention_q8_kern
 // that takes 32 clocks, so the conversion stands beside the first products
 // and the exponentials of 16 positions beside the second products of the 16
 // before; the scheduling groups keep the compiler to that and its LDS reads
-// ahead.  Two column tiles a wave halve what a column pays for conversions,
-// loads and LDS reads.
+// ahead.  (Two column tiles a wave would halve what a column pays for
+// conversions and LDS reads, but take all registers of a SIMD for one wave:
+// 8,192 rows in 1,130 us against 868.)
 //
 // binary16 (QT = FENCE_F16): with the page's V scale in the exponent, one
 // fused multiply-add and one exponential make the probability that the
@@ -733,8 +723,6 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void attention_q8_kern
 // would grow past 2^15 (kSlack), so O is rarely rescaled.
 template <int TYPE, int QT, int HD>
 __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(Q8Args a) {
-    typedef Prompt<HD> Kind;
-    constexpr int NC = Kind::COLS / 128;
     constexpr bool F32 = QT == FENCE_F32;
     constexpr int PARTS = F32 ? 2 : 1;
     constexpr int KS = HD / 16;   // k steps of the first product
@@ -753,7 +741,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
     const int n = lane % 32, g = lane / 32;
     const int hd = a.head_dim, page_mask = (1 << a.page_shift) - 1;
 
-    Share<Kind> share;
+    Share<Prompt> share;
     if (!share.find_mine(a)) return;
     // What this lane converts: K position lane % 16, dimensions 16 (lane / 16 + 4 j) on; V positions 4 vg + (0 .. 3)
     // and 8 more, dimensions vd on.  At HD = 64 the upper lanes load the V that the lower ones do.
@@ -775,36 +763,31 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
         __syncthreads();
     }
     do {
-        const Seq<Kind> s = Seq<Kind>::uniform(a, share.p.seq);
+        const Seq<Prompt> s = Seq<Prompt>::uniform(a, share.p.seq);
         const int tile = share.p.tile, head = share.p.head, first = share.p.unit, units = share.p.units;
         const int last = share.last();
-        const int cols = s.rows * a.group - tile * Kind::COLS;
-        int c[NC], row[NC], qhead[NC], sees[NC];  // this lane's columns
-        bool mine[NC];
-#pragma unroll
-        for (int x = 0; x < NC; ++x) {
-            c[x] = (wave * NC + x) * 32 + n;
-            mine[x] = c[x] < cols;
-            row[x] = (tile * Kind::COLS + c[x]) / a.group;
-            qhead[x] = head * a.group + (tile * Kind::COLS + c[x]) % a.group;
-            sees[x] = mine[x] ? s.row_sees(row[x]) : 0;
-        }
+        const int cols = s.rows * a.group - tile * Prompt::COLS;
+        const int c = wave * 32 + n;  // this lane's column
+        const bool mine = c < cols;
+        const int row = (tile * Prompt::COLS + c) / a.group;
+        const int qhead = head * a.group + (tile * Prompt::COLS + c) % a.group;
+        const int sees = mine ? s.row_sees(row) : 0;
         const int end = s.sees(tile);
         if (first >= last) {
             // Nothing of this item; if others take what is before and after, the join finds an empty part.
-            float* ml = part_sums(a, part_at(a, blockIdx.x, false, HD), HD);
-#pragma unroll
-            for (int x = 0; x < NC; ++x)
-                if (first > 0 && mine[x] && g == 0) ml[2 * c[x]] = -__builtin_inff(), ml[2 * c[x] + 1] = 0.0f;
+            if (first > 0 && mine && g == 0) {
+                float* ml = part_sums(a, part_at(a, blockIdx.x, false, HD), HD) + 2 * c;
+                ml[0] = -__builtin_inff(), ml[1] = 0.0f;
+            }
             continue;
         }
         // what every column of this wave sees
-        const int least = s.row_sees((tile * Kind::COLS + wave * NC * 32) / a.group);
+        const int least = s.row_sees((tile * Prompt::COLS + wave * 32) / a.group);
         const int64_t table = static_cast<int64_t>(share.p.seq) * a.max_blocks;
 
         // The page of this wave's 16 positions of a unit.
         const auto page_of = [&](int un) {
-            const int pos = un * Kind::UNIT + wave * 16;
+            const int pos = un * Prompt::UNIT + wave * 16;
             const int id = un < last && pos < end ? uniform_load(a.table, table + (pos >> a.page_shift)) : -1;
             return id < a.n_pages ? id : -1;
         };
@@ -814,7 +797,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
         // the codes of a unit, of page 0 if the page is not there
         const auto load = [&](int un, int id) {
             const int64_t base = static_cast<int64_t>(id < 0 ? 0 : id) * a.n_kv_heads + head;
-            const int64_t at = ((base << a.page_shift) + ((un * Kind::UNIT + wave * 16) & page_mask)) * hd;
+            const int64_t at = ((base << a.page_shift) + ((un * Prompt::UNIT + wave * 16) & page_mask)) * hd;
             const uint8_t* k = a.k + at;
             const uint8_t* v = a.v + at;
 #pragma unroll
@@ -838,7 +821,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
         };
         // V codes of positions past the end: an e4m3 one may be NaN, which no weight of 0 removes.
         const auto trim = [&](int un) {
-            const int pos0 = un * Kind::UNIT + wave * 16;
+            const int pos0 = un * Prompt::UNIT + wave * 16;
             if (TYPE == FENCE_KV_E4M3 && pos0 + 16 > end) {
 #pragma unroll
                 for (int j = 0; j < VJ; ++j)
@@ -880,18 +863,15 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
         scales(id_next);
         id_next = page_of(first + 1);
 
-        h8 qf[NC][PARTS][KS];
-        float unscale[NC];
-#pragma unroll
-        for (int x = 0; x < NC; ++x) {
-            unscale[x] = a.scale_log2;
-            const int64_t from =
-                mine[x] ? static_cast<int64_t>(s.row0 + row[x]) * a.ldq + static_cast<int64_t>(qhead[x]) * hd : 0;
+        h8 qf[PARTS][KS];
+        float unscale = a.scale_log2;
+        {
+            const int64_t from = mine ? static_cast<int64_t>(s.row0 + row) * a.ldq + static_cast<int64_t>(qhead) * hd : 0;
             if constexpr (F32) {
                 float biggest = 0.0f;
 #pragma unroll
                 for (int k = 0; k < KS; ++k)
-                    if (mine[x] && k * 16 < hd) {
+                    if (mine && k * 16 < hd) {
                         const float* src = static_cast<const float*>(a.q) + from + k * 16 + g * 8;
 #pragma unroll
                         for (int i = 0; i < 8; ++i) biggest = fmaxf(biggest, fabsf(src[i]));
@@ -900,43 +880,38 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
                 uint32_t e = __builtin_bit_cast(uint32_t, biggest) >> 23;
                 e = e < 15 ? 15 : e > 254 ? 254 : e;
                 const float up = __builtin_bit_cast(float, (268 - e) << 23);
-                unscale[x] *= __builtin_bit_cast(float, (e - 14) << 23);
+                unscale *= __builtin_bit_cast(float, (e - 14) << 23);
 #pragma unroll
                 for (int k = 0; k < KS; ++k) {
                     const float* src = static_cast<const float*>(a.q) + from + k * 16 + g * 8;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         _Float16 hi, lo;
-                        split(mine[x] && k * 16 < hd ? src[i] * up : 0.0f, &hi, &lo);
-                        qf[x][0][k][i] = hi;
-                        qf[x][1][k][i] = lo;
+                        split(mine && k * 16 < hd ? src[i] * up : 0.0f, &hi, &lo);
+                        qf[0][k][i] = hi;
+                        qf[1][k][i] = lo;
                     }
                 }
             } else {
 #pragma unroll
                 for (int k = 0; k < KS; ++k) {
                     h8 y = {};
-                    if (mine[x] && k * 16 < hd) {
+                    if (mine && k * 16 < hd) {
                         const _Float16* src = static_cast<const _Float16*>(a.q) + from + k * 16 + g * 8;
 #pragma unroll
                         for (int i = 0; i < 8; ++i) y[i] = src[i];
                     }
-                    qf[x][0][k] = y;
+                    qf[0][k] = y;
                 }
             }
         }
 
-        f16v o[NC][NT];
-        float m[NC], l[NC], vref = 0.0f;
+        f16v o[NT];
 #pragma unroll
-        for (int x = 0; x < NC; ++x) {
-            m[x] = -__builtin_inff();
-            l[x] = 0.0f;
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[x][t][i] = 0.0f;
-        }
+            for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
+        float m = -__builtin_inff(), l = 0.0f, vref = 0.0f;
         trim(first);
         convert(buf + (first & 1) * HALF);
         load(first + 1, id_next);
@@ -946,15 +921,13 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
 
         const auto turn = [&](int un, auto masked) {
             const h8* half = buf + (un & 1) * HALF;
-            const int pos0 = un * Kind::UNIT;
+            const int pos0 = un * Prompt::UNIT;
             trim(un + 1);
-            f16v st[NC][2];
+            f16v st[2];
 #pragma unroll
-            for (int x = 0; x < NC; ++x)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) st[x][h][i] = 0.0f;
+                for (int i = 0; i < 16; ++i) st[h][i] = 0.0f;
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int k = 0; k < KS; ++k)
@@ -962,10 +935,8 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
                 for (int h = 0; h < 2; ++h) {
                     const h8 kf = half[(h * KS + k) * kWave + lane];
 #pragma unroll
-                    for (int x = 0; x < NC; ++x)
-#pragma unroll
-                        for (int p = 0; p < PARTS; ++p)
-                            st[x][h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[x][p][k], st[x][h], 0, 0, 0);
+                    for (int p = 0; p < PARTS; ++p)
+                        st[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[p][k], st[h], 0, 0, 0);
                 }
             f4 sc[4];
 #pragma unroll
@@ -976,7 +947,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
             __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
             for (int i = 0; i < 2 * KS; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, NC * PARTS, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, PARTS, 0);
                 if (i < 2 * KS - kAhead + 4) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x002, kEach, 0);
                 __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
@@ -998,96 +969,81 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
             const float vnow = grow_v ? vtop : vref;
             const float vone = vnow > 0.0f ? __builtin_amdgcn_rcpf(vnow) : 0.0f;
             const float vlog = vnow > 0.0f ? __builtin_amdgcn_logf(vnow) : 0.0f;
-            float top[NC];
-            bool move = grow_v;
-            int limit[NC];  // of this lane's positions: those below it are seen
-            const auto seen = [&](int x, int h, int i) { return h * 32 + (i / 4) * 8 + i % 4 < limit[x]; };
+            const int limit = sees - pos0 - g * 4;  // of this lane's positions: those below it are seen
+            const auto seen = [&](int h, int i) { return h * 32 + (i / 4) * 8 + i % 4 < limit; };
+            if (masked) {
 #pragma unroll
-            for (int x = 0; x < NC; ++x) {
-                limit[x] = sees[x] - pos0 - g * 4;
-                if (masked) {
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (!seen(x, h, i)) st[x][h][i] = -__builtin_inff();
-                }
-                top[x] = -__builtin_inff();
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    float t = st[x][q / 2][(q % 2) * 8];
-#pragma unroll
-                    for (int i = 1; i < 8; ++i) t = fmaxf(t, st[x][q / 2][(q % 2) * 8 + i]);
-                    // scales are not negative, so the largest product is the largest score
-                    t = in[q] && t > -__builtin_inff() ? t * (sc[q][0] * unscale[x]) : -__builtin_inff();
-                    top[x] = fmaxf(top[x], t);
-                }
-                top[x] = halves_max(top[x]);
-                move |= top[x] > m[x] + kSlack;
+                    for (int i = 0; i < 16; ++i)
+                        if (!seen(h, i)) st[h][i] = -__builtin_inff();
             }
-            if (__any(move)) {
-#pragma unroll
-                for (int x = 0; x < NC; ++x) {
-                    const float now = fmaxf(m[x], top[x]);
-                    const float alpha = now == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m[x] - now);
-                    const float beta = alpha * (vref * vone);
-                    m[x] = now;
-                    l[x] *= alpha;
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) o[x][t] *= beta;
-                }
-                vref = vnow;
-            }
+            float top = -__builtin_inff();
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                h8 pf[NC][PARTS];
+                float t = st[q / 2][(q % 2) * 8];
 #pragma unroll
-                for (int x = 0; x < NC; ++x) {
-                    const float ref = m[x] == -__builtin_inff() ? 0.0f : m[x];
-                    const float fk = sc[q][0] * unscale[x];
-                    if constexpr (F32) {
-                        const float to_v = sc[q][1] * vone * 16384.0f;
+                for (int i = 1; i < 8; ++i) t = fmaxf(t, st[q / 2][(q % 2) * 8 + i]);
+                // scales are not negative, so the largest product is the largest score
+                t = in[q] && t > -__builtin_inff() ? t * (sc[q][0] * unscale) : -__builtin_inff();
+                top = fmaxf(top, t);
+            }
+            top = halves_max(top);
+            if (__any(top > m + kSlack || grow_v)) {
+                const float now = fmaxf(m, top);
+                const float alpha = now == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - now);
+                const float beta = alpha * (vref * vone);
+                m = now;
+                vref = vnow;
+                l *= alpha;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            float p = __builtin_amdgcn_exp2f(st[x][q / 2][(q % 2) * 8 + i] * fk - ref);
-                            if (!in[q] || (masked && !seen(x, q / 2, (q % 2) * 8 + i))) p = 0.0f;
-                            l[x] += p;
-                            const float y = masked && p == 0.0f ? 0.0f : p * to_v;
-                            _Float16 hi, lo;
-                            split(y, &hi, &lo);
-                            pf[x][0][i] = hi;
-                            pf[x][PARTS - 1][i] = lo;
-                        }
-                    } else {
-                        // V codes under a scale of 0 are zero: any weight will do that can be taken back
-                        const bool none = sc[q][1] == 0.0f;
-                        const float shift = in[q] ? (none ? 0.0f : sc[q][2] - vlog) + (kBase - ref) : -__builtin_inff();
-                        float p[8];
+                for (int t = 0; t < NT; ++t) o[t] *= beta;
+            }
+            const float ref = m == -__builtin_inff() ? 0.0f : m;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[x][q / 2][(q % 2) * 8 + i], fk, shift));
-                            if (masked && !seen(x, q / 2, (q % 2) * 8 + i)) p[i] = 0.0f;
-                        }
-                        float sum = 0.0f;
+            for (int q = 0; q < 4; ++q) {
+                h8 pf[PARTS];
+                const float fk = sc[q][0] * unscale;
+                if constexpr (F32) {
+                    const float to_v = sc[q][1] * vone * 16384.0f;
 #pragma unroll
-                        for (int i = 0; i < 8; i += 2) {
-                            const h2 y = {static_cast<_Float16>(p[i]), static_cast<_Float16>(p[i + 1])};
-                            pf[x][0][i] = y[0];
-                            pf[x][0][i + 1] = y[1];
-                            const h2 ones = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
-                            sum = __builtin_amdgcn_fdot2(y, ones, sum, false);
-                        }
-                        l[x] += sum * (none ? 0x1p-10f : 0x1p-10f * (vnow * sc[q][3]));
+                    for (int i = 0; i < 8; ++i) {
+                        float p = __builtin_amdgcn_exp2f(st[q / 2][(q % 2) * 8 + i] * fk - ref);
+                        if (!in[q] || (masked && !seen(q / 2, (q % 2) * 8 + i))) p = 0.0f;
+                        l += p;
+                        const float y = masked && p == 0.0f ? 0.0f : p * to_v;
+                        _Float16 hi, lo;
+                        split(y, &hi, &lo);
+                        pf[0][i] = hi;
+                        pf[PARTS - 1][i] = lo;
                     }
+                } else {
+                    // V codes under a scale of 0 are zero: any weight will do that can be taken back
+                    const bool none = sc[q][1] == 0.0f;
+                    const float shift = in[q] ? (none ? 0.0f : sc[q][2] - vlog) + (kBase - ref) : -__builtin_inff();
+                    float p[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[q / 2][(q % 2) * 8 + i], fk, shift));
+                        if (masked && !seen(q / 2, (q % 2) * 8 + i)) p[i] = 0.0f;
+                    }
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) {
+                        const h2 y = {static_cast<_Float16>(p[i]), static_cast<_Float16>(p[i + 1])};
+                        pf[0][i] = y[0];
+                        pf[0][i + 1] = y[1];
+                        const h2 ones = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
+                        sum = __builtin_amdgcn_fdot2(y, ones, sum, false);
+                    }
+                    l += sum * (none ? 0x1p-10f : 0x1p-10f * (vnow * sc[q][3]));
                 }
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     const h8 vf = half[V0 + (q * NT + t) * kWave + lane];
 #pragma unroll
-                    for (int x = 0; x < NC; ++x)
-#pragma unroll
-                        for (int p = 0; p < PARTS; ++p)
-                            o[x][t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[x][p], o[x][t], 0, 0, 0);
+                    for (int p = 0; p < PARTS; ++p)
+                        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pf[p], o[t], 0, 0, 0);
                 }
             }
             __syncthreads();
@@ -1095,23 +1051,21 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
         // The waves turn together; each masks from where its first column ends.
         int un = first;
 #pragma unroll 1
-        for (; un < last && (un + 1) * Kind::UNIT <= least; ++un) turn(un, std::false_type{});
+        for (; un < last && (un + 1) * Prompt::UNIT <= least; ++un) turn(un, std::false_type{});
 #pragma unroll 1
         for (; un < last; ++un) turn(un, std::true_type{});
 
-        // o[x][t][i] is dimension (8 (i / 4) + 4 g + i % 4) * NT + t of this lane's column: runs of 4 NT.
+        // o[t][i] is dimension (8 (i / 4) + 4 g + i % 4) * NT + t of this lane's column: runs of 4 NT.
+        const float sum = l + __shfl_xor(l, 32);
         const float unit_v = vref * (F32 ? 0x1p-14f : 0x1p-10f);
-        const bool whole = first == 0 && last == units;
-#pragma unroll
-        for (int x = 0; x < NC; ++x) {
-            const float sum = l[x] + __shfl_xor(l[x], 32);
-            if (!mine[x]) continue;
+        if (mine) {
+            const bool whole = first == 0 && last == units;
             const float f = whole ? (sum != 0.0f ? unit_v / sum : 0.0f) : unit_v;
             float* part = part_at(a, blockIdx.x, first == 0, HD);
-            const int64_t to = static_cast<int64_t>(s.row0 + row[x]) * a.ldo + static_cast<int64_t>(qhead[x]) * hd;
+            const int64_t to = static_cast<int64_t>(s.row0 + row) * a.ldo + static_cast<int64_t>(qhead) * hd;
             if (!whole && g == 0) {
-                float* ml = part_sums(a, part, HD) + 2 * c[x];
-                ml[0] = m[x], ml[1] = sum;
+                float* ml = part_sums(a, part, HD) + 2 * c;
+                ml[0] = m, ml[1] = sum;
             }
 #pragma unroll
             for (int q = 0; q < 4; ++q)
@@ -1122,12 +1076,12 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const int j = (z + i) / NT, t = (z + i) % NT;
-                        y[i] = whole && sum == 0.0f ? 0.0f : o[x][t][4 * q + j] * f;
+                        y[i] = whole && sum == 0.0f ? 0.0f : o[t][4 * q + j] * f;
                     }
                     if (whole) {
                         if (d < hd) put8<QT>(a, to + d, y);
                     } else {
-                        float* p = part + c[x] * HD + d;
+                        float* p = part + c * HD + d;
                         *reinterpret_cast<f4*>(p) = f4{y[0], y[1], y[2], y[3]};
                         *reinterpret_cast<f4*>(p + 4) = f4{y[4], y[5], y[6], y[7]};
                     }
@@ -1142,8 +1096,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
 // columns are its to join, together with the other workgroups of the same x,
 // a run of 4 dimensions a thread.
 template <int QT, int HD, class KIND>
-__global__ __launch_bounds__(kThreads) void join_q8_kernel(Q8Args a, int grid) {
-    const int w0 = blockIdx.x;
+__device__ __forceinline__ void join_at(const Q8Args& a, int w0, int grid) {
     int64_t total;
     Place p[1];
     if (!find<KIND, 1>(a, &grid, &total, p, [&](int, int64_t n, int g) -> int64_t {
@@ -1209,19 +1162,27 @@ __global__ __launch_bounds__(kThreads) void join_q8_kernel(Q8Args a, int grid) {
     }
 }
 
+// The borders of both kernels in one launch: first those of the prompts.
+template <int QT, int HD>
+__global__ __launch_bounds__(kThreads) void join_q8_kernel(Q8Args many, int many_grid, Q8Args few, int few_grid) {
+    const int border = blockIdx.x;
+    if (border < many_grid - 1) join_at<QT, HD, Prompt>(many, border, many_grid);
+    else join_at<QT, HD, Few>(few, border - (many_grid > 1 ? many_grid - 1 : 0), few_grid);
+}
+
 int padded(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 
 bool big(int max_q_len, int group) { return static_cast<int64_t>(max_q_len) * group > kSmall; }
 
-int part_cols(int max_q_len, int group, int head_dim, bool is_big) {
-    const int64_t most = is_big ? prompt_cols(head_dim) : kCols, n = static_cast<int64_t>(max_q_len) * group;
+int part_cols(int max_q_len, int group, bool is_big) {
+    const int64_t most = is_big ? kPromptCols : kCols, n = static_cast<int64_t>(max_q_len) * group;
     return static_cast<int>(n < most ? n : most);
 }
 
 // Floats of the parts that the workgroups of one kernel may leave.
 int64_t part_floats(int max_q_len, int group, int head_dim, bool is_big) {
     return static_cast<int64_t>(is_big ? kBigGrid : kGrid) * 2 *
-           part_size(part_cols(max_q_len, group, head_dim, is_big), padded(head_dim));
+           part_size(part_cols(max_q_len, group, is_big), padded(head_dim));
 }
 
 // Workgroups for at most `units` of work.
@@ -1232,29 +1193,27 @@ unsigned grid_for(int64_t tiles, int64_t heads, int64_t positions, int unit, int
 }
 
 template <int TYPE, int QT, int HD>
-int attention_launch(Q8Args a, hipStream_t s) {
-    const bool both = big(a.max_q_len, a.group);
+int attention_launch(const Q8Args& a, hipStream_t s) {
     const int64_t columns = static_cast<int64_t>(a.max_q_len) * a.group;
     const int64_t positions = static_cast<int64_t>(a.max_blocks) << a.page_shift;
-    if (both) {
-        a.part_cols = part_cols(a.max_q_len, a.group, a.head_dim, true);
-        const unsigned grid =
-            grid_for((columns + Prompt<HD>::COLS - 1) / Prompt<HD>::COLS, a.n_kv_heads, positions, Prompt<HD>::UNIT,
-                     a.batch, kBigGrid);
-        if (const int st = launch(prompt_q8_kernel<TYPE, QT, HD>, dim3(grid), dim3(kThreads), 0, s, a)) return st;
-        if (grid > 1)
-            if (const int st = launch(join_q8_kernel<QT, HD, Prompt<HD>>, dim3(grid - 1, 2), dim3(kThreads), 0, s, a,
-                                      static_cast<int>(grid)))
-                return st;
-        a.ws += part_floats(a.max_q_len, a.group, a.head_dim, true);
+    Q8Args many = a, few = a;
+    unsigned many_grid = 0;
+    if (big(a.max_q_len, a.group)) {
+        many.part_cols = part_cols(a.max_q_len, a.group, true);
+        many_grid = grid_for((columns + Prompt::COLS - 1) / Prompt::COLS, a.n_kv_heads, positions, Prompt::UNIT, a.batch,
+                             kBigGrid);
+        if (const int st = launch(prompt_q8_kernel<TYPE, QT, HD>, dim3(many_grid), dim3(kThreads), 0, s, many)) return st;
+        few.ws += part_floats(a.max_q_len, a.group, a.head_dim, true);
     }
     const int64_t small = columns < kSmall ? columns : kSmall;
-    a.part_cols = part_cols(a.max_q_len, a.group, a.head_dim, false);
-    const unsigned grid = grid_for((small + kCols - 1) / kCols, a.n_kv_heads, positions, kUnit, a.batch, kGrid);
-    const size_t shmem = static_cast<size_t>(kWaves) * a.part_cols * (HD + 2) * sizeof(float);
-    if (const int st = launch(attention_q8_kernel<TYPE, QT, HD>, dim3(grid), dim3(kThreads), shmem, s, a)) return st;
-    if (grid == 1) return FENCE_SUCCESS;
-    return launch(join_q8_kernel<QT, HD, Few>, dim3(grid - 1), dim3(kThreads), 0, s, a, static_cast<int>(grid));
+    few.part_cols = part_cols(a.max_q_len, a.group, false);
+    const unsigned few_grid = grid_for((small + kCols - 1) / kCols, a.n_kv_heads, positions, kUnit, a.batch, kGrid);
+    const size_t shmem = static_cast<size_t>(kWaves) * few.part_cols * (HD + 2) * sizeof(float);
+    if (const int st = launch(attention_q8_kernel<TYPE, QT, HD>, dim3(few_grid), dim3(kThreads), shmem, s, few)) return st;
+    const unsigned borders = (many_grid > 1 ? many_grid - 1 : 0) + few_grid - 1;
+    if (borders == 0) return FENCE_SUCCESS;
+    return launch(join_q8_kernel<QT, HD>, dim3(borders, many_grid > 1 ? 2 : 1), dim3(kThreads), 0, s, many,
+                  static_cast<int>(many_grid), few, static_cast<int>(few_grid));
 }
 
 template <int TYPE, int QT>
