@@ -25,18 +25,13 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
 // Columns of the products are the (row, head of the group) pairs of one kv
 // head; a sequence's are taken kCols or kPromptCols at a time.
-constexpr int kCols = 16;           // attention_q8_kernel
+constexpr int kCols = 16;           // few_columns; a sequence with no more of them goes there
 constexpr int kUnit = 32 * kWaves;  // positions its workgroup takes at a time
-constexpr int kPromptCols = 32 * kWaves;  // prompt_q8_kernel
+constexpr int kPromptCols = 32 * kWaves;  // many_columns
 #ifndef FENCE_ATTN_Q8_ITEM
 #define FENCE_ATTN_Q8_ITEM 384
 #endif
 constexpr int kBigItem = FENCE_ATTN_Q8_ITEM;  // what an item costs besides its positions, in positions
-// Up to this many columns a sequence goes to attention_q8_kernel.
-#ifndef FENCE_ATTN_Q8_SMALL
-#define FENCE_ATTN_Q8_SMALL 32
-#endif
-constexpr int kSmall = FENCE_ATTN_Q8_SMALL;
 #ifndef FENCE_ATTN_Q8_GRID
 #define FENCE_ATTN_Q8_GRID 1024
 #endif
@@ -74,11 +69,11 @@ __device__ __forceinline__ T uniform_load(const T* p, int64_t i) {
 
 // The two kernels: work is counted in units, COLS columns of one kv head by
 // UNIT positions.
-struct Few {  // attention_q8_kernel: each wave all columns, its own positions
+struct Few {  // few_columns: each wave all columns, its own positions
     static constexpr bool MANY = false;
     static constexpr int COLS = kCols, UNIT = kUnit;
 };
-struct Prompt {  // prompt_q8_kernel: each wave its own columns, all positions
+struct Prompt {  // many_columns: each wave its own columns, all positions
     static constexpr bool MANY = true;
     static constexpr int COLS = kPromptCols, UNIT = 64;
 };
@@ -93,7 +88,7 @@ struct Seq {
     __device__ __forceinline__ Seq(const Q8Args& a, int row, int row_end, int len) : row0(row), group(a.group) {
         q_len = row_end > row ? row_end - row : 0;
         rows = q_len < a.max_q_len ? q_len : a.max_q_len;
-        if ((rows * group > kSmall) != BIG) rows = 0;
+        if ((rows * group > kCols) != BIG) rows = 0;
         const int cap = a.max_blocks << a.page_shift;
         kv = len < 0 ? 0 : len > cap ? cap : len;
     }
@@ -117,8 +112,8 @@ struct Seq {
         const int n = sees(tile);
         return n > UNIT ? (n + UNIT - 1) / UNIT : 1;
     }
-    // What a tile of one kv head costs and what the tiles before it do, for the even split.  Few tiles: their
-    // units.  Many: about the positions that its columns see and kBigItem more for beginning and ending an item,
+    // What a tile of one kv head costs and what the tiles before it do, for the even split.  Few columns, so one
+    // tile: its units.  Many: about the positions that its columns see and kBigItem more for beginning and ending an item,
     // times the group; a linear function of the tile, so that the sum needs no loop over the tiles.
     __device__ __forceinline__ int64_t slope() const {
         const int64_t n = static_cast<int64_t>(kv) - q_len + 1;
@@ -130,9 +125,7 @@ struct Seq {
     }
     __device__ __forceinline__ int64_t before(int tile) const {
         if constexpr (!BIG) {
-            int64_t n = 0;
-            for (int t = 0; t < tile; ++t) n += units(t);
-            return n;
+            return tile ? units(0) : 0;
         } else {
             return slope() * tile + static_cast<int64_t>(COLS) * (static_cast<int64_t>(tile) * (tile + 1) / 2);
         }
@@ -278,9 +271,8 @@ struct Share {
     Place p;
     int end_seq, end_tile, end_head, end_unit;
 
-    __device__ __forceinline__ bool find_mine(const Q8Args& a) {
-        const int me = blockIdx.x;
-        int grid = gridDim.x;
+    // workgroup `me` of `grid`
+    __device__ __forceinline__ bool find_mine(const Q8Args& a, int me, int grid) {
         int64_t total;
         Place ends[2];
         // the last place is in front of the next workgroup's first; the last workgroup's is the end of all
@@ -413,20 +405,19 @@ __device__ __forceinline__ float across_rows(float v, Op op) {
 // dimensions are r * HD / 16 + i for product i, so it reads V with one load a
 // position.  The next positions' codes are loaded before these are used.
 template <int TYPE, int QT, int HD>
-__global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void attention_q8_kernel(Q8Args a) {
+__device__ __forceinline__ void few_columns(const Q8Args& a, float* lds, int me, int grid) {
     constexpr int PIECES = HD / 64;       // 64 dimensions of K: 16 a lane
     constexpr int DT = HD / 16;           // products over V; also dimensions a lane reads of a position
     constexpr int VW = DT / 4;            // words of them
     constexpr bool F32 = QT == FENCE_F32;
     constexpr int PARTS = F32 ? 2 : 1;    // binary16 numbers that hold a q or a p
-    extern __shared__ float lds[];
     const int tid = threadIdx.x, lane = tid % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int r = lane % 16, g = lane / 16;
     const int hd = a.head_dim, page_mask = (1 << a.page_shift) - 1;
 
     Share<Few> share;
-    if (!share.find_mine(a)) return;
+    if (!share.find_mine(a, me, grid)) return;
     do {
         const Seq<Few> s = Seq<Few>::uniform(a, share.p.seq);
         const int tile = share.p.tile, head = share.p.head, first = share.p.unit, units = share.p.units;
@@ -659,7 +650,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void attention_q8_kern
         }
         __syncthreads();
         const bool whole = first == 0 && last == units;
-        float* part = part_at(a, blockIdx.x, first == 0, HD);
+        float* part = part_at(a, me, first == 0, HD);
         for (int x = tid; x < cols * HD; x += kThreads) {
             const int c = x / HD, d = x % HD;
             float top = -__builtin_inff();
@@ -721,8 +712,16 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void attention_q8_kern
 // product takes, and its sum comes from the rounded values by dot products.
 // The running maximum and the largest V scale are only moved when a value
 // would grow past 2^15 (kSlack), so O is rarely rescaled.
+template <int HD>
+struct PromptLds {
+    // A half in 16-byte pieces: K fragments [2][HD / 16][64 lanes], V fragments [4][HD / 32][64 lanes], per 16
+    // positions K scale (-1 if the page is not there), V scale, its log2 and inverse, and a place for each lane to
+    // write what nobody reads.
+    static constexpr int V0 = HD / 8 * kWave, S0 = V0 + HD / 8 * kWave, X0 = S0 + 4, HALF = X0 + kWave;
+};
+
 template <int TYPE, int QT, int HD>
-__global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(Q8Args a) {
+__device__ __forceinline__ void many_columns(const Q8Args& a, h8* buf, int me, int grid) {
     constexpr bool F32 = QT == FENCE_F32;
     constexpr int PARTS = F32 ? 2 : 1;
     constexpr int KS = HD / 16;   // k steps of the first product
@@ -731,18 +730,14 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
     constexpr int VJ = HD <= 128 ? 1 : 2;  // 8 positions x 4 dimensions of V a lane converts
     constexpr float kBase = F32 ? 14.0f : 10.0f;  // log2 of what stands for 1 times the largest V scale
     constexpr float kSlack = F32 ? 0.0f : 4.0f;
-    // A half of LDS in 16-byte pieces: K fragments [2][KS][64 lanes], V fragments [4][NT][64 lanes], per 16
-    // positions K scale (-1 if the page is not there), V scale, its log2 and inverse, and a place for each lane to
-    // write what nobody reads.
-    constexpr int V0 = 2 * KS * kWave, S0 = V0 + 4 * NT * kWave, X0 = S0 + 4, HALF = X0 + kWave;
-    __shared__ h8 buf[2 * HALF];
+    constexpr int V0 = PromptLds<HD>::V0, S0 = PromptLds<HD>::S0, X0 = PromptLds<HD>::X0, HALF = PromptLds<HD>::HALF;
     const int tid = threadIdx.x, lane = tid % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const int n = lane % 32, g = lane / 32;
     const int hd = a.head_dim, page_mask = (1 << a.page_shift) - 1;
 
     Share<Prompt> share;
-    if (!share.find_mine(a)) return;
+    if (!share.find_mine(a, me, grid)) return;
     // What this lane converts: K position lane % 16, dimensions 16 (lane / 16 + 4 j) on; V positions 4 vg + (0 .. 3)
     // and 8 more, dimensions vd on.  At HD = 64 the upper lanes load the V that the lower ones do.
     const int kr = lane % 16, kc = lane / 16;
@@ -776,7 +771,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
         if (first >= last) {
             // Nothing of this item; if others take what is before and after, the join finds an empty part.
             if (first > 0 && mine && g == 0) {
-                float* ml = part_sums(a, part_at(a, blockIdx.x, false, HD), HD) + 2 * c;
+                float* ml = part_sums(a, part_at(a, me, false, HD), HD) + 2 * c;
                 ml[0] = -__builtin_inff(), ml[1] = 0.0f;
             }
             continue;
@@ -1061,7 +1056,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
         if (mine) {
             const bool whole = first == 0 && last == units;
             const float f = whole ? (sum != 0.0f ? unit_v / sum : 0.0f) : unit_v;
-            float* part = part_at(a, blockIdx.x, first == 0, HD);
+            float* part = part_at(a, me, first == 0, HD);
             const int64_t to = static_cast<int64_t>(s.row0 + row) * a.ldo + static_cast<int64_t>(qhead) * hd;
             if (!whole && g == 0) {
                 float* ml = part_sums(a, part, HD) + 2 * c;
@@ -1088,6 +1083,23 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void prompt_q8_kernel(
                 }
         }
     } while (share.next(a));
+}
+
+template <int TYPE, int QT, int HD>
+__global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void attention_q8_kernel(Q8Args a) {
+    extern __shared__ float lds[];
+    few_columns<TYPE, QT, HD>(a, lds, blockIdx.x, gridDim.x);
+}
+
+// Both in one launch, for batches that may hold prompts: the workgroups that
+// take few columns come behind those of the prompts and fill what these leave.
+template <int TYPE, int QT, int HD>
+__global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void mixed_q8_kernel(Q8Args many, int many_grid, Q8Args few) {
+    __shared__ h8 buf[2 * PromptLds<HD>::HALF];
+    static_assert(sizeof(buf) >= kWaves * kCols * (HD + 2) * sizeof(float), "the other kernel's LDS");
+    const int wg = blockIdx.x;
+    if (wg < many_grid) many_columns<TYPE, QT, HD>(many, buf, wg, many_grid);
+    else few_columns<TYPE, QT, HD>(few, reinterpret_cast<float*>(buf), wg - many_grid, gridDim.x - many_grid);
 }
 
 // Joins the parts of the items that more than one workgroup took, in workgroup
@@ -1172,7 +1184,7 @@ __global__ __launch_bounds__(kThreads) void join_q8_kernel(Q8Args many, int many
 
 int padded(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 
-bool big(int max_q_len, int group) { return static_cast<int64_t>(max_q_len) * group > kSmall; }
+bool big(int max_q_len, int group) { return static_cast<int64_t>(max_q_len) * group > kCols; }
 
 int part_cols(int max_q_len, int group, bool is_big) {
     const int64_t most = is_big ? kPromptCols : kCols, n = static_cast<int64_t>(max_q_len) * group;
@@ -1197,19 +1209,22 @@ int attention_launch(const Q8Args& a, hipStream_t s) {
     const int64_t columns = static_cast<int64_t>(a.max_q_len) * a.group;
     const int64_t positions = static_cast<int64_t>(a.max_blocks) << a.page_shift;
     Q8Args many = a, few = a;
+    few.part_cols = part_cols(a.max_q_len, a.group, false);
+    const unsigned few_grid = grid_for(1, a.n_kv_heads, positions, kUnit, a.batch, kGrid);
     unsigned many_grid = 0;
-    if (big(a.max_q_len, a.group)) {
+    if (columns > kCols) {
         many.part_cols = part_cols(a.max_q_len, a.group, true);
+        few.ws += part_floats(a.max_q_len, a.group, a.head_dim, true);
         many_grid = grid_for((columns + Prompt::COLS - 1) / Prompt::COLS, a.n_kv_heads, positions, Prompt::UNIT, a.batch,
                              kBigGrid);
-        if (const int st = launch(prompt_q8_kernel<TYPE, QT, HD>, dim3(many_grid), dim3(kThreads), 0, s, many)) return st;
-        few.ws += part_floats(a.max_q_len, a.group, a.head_dim, true);
+        if (const int st = launch(mixed_q8_kernel<TYPE, QT, HD>, dim3(many_grid + few_grid), dim3(kThreads), 0, s, many,
+                                  static_cast<int>(many_grid), few))
+            return st;
+    } else {
+        const size_t shmem = static_cast<size_t>(kWaves) * few.part_cols * (HD + 2) * sizeof(float);
+        if (const int st = launch(attention_q8_kernel<TYPE, QT, HD>, dim3(few_grid), dim3(kThreads), shmem, s, few))
+            return st;
     }
-    const int64_t small = columns < kSmall ? columns : kSmall;
-    few.part_cols = part_cols(a.max_q_len, a.group, false);
-    const unsigned few_grid = grid_for((small + kCols - 1) / kCols, a.n_kv_heads, positions, kUnit, a.batch, kGrid);
-    const size_t shmem = static_cast<size_t>(kWaves) * few.part_cols * (HD + 2) * sizeof(float);
-    if (const int st = launch(attention_q8_kernel<TYPE, QT, HD>, dim3(few_grid), dim3(kThreads), shmem, s, few)) return st;
     const unsigned borders = (many_grid > 1 ? many_grid - 1 : 0) + few_grid - 1;
     if (borders == 0) return FENCE_SUCCESS;
     return launch(join_q8_kernel<QT, HD>, dim3(borders, many_grid > 1 ? 2 : 1), dim3(kThreads), 0, s, many,
