@@ -10,42 +10,60 @@
 // time, and a sum over a whole vocabulary stays exact enough that tokens next
 // to a border fall on the right side.
 //
-// One workgroup takes a row.
-//   1. One pass finds the maximum and each thread's maximum.  For a top-k up
-//      to kListK, the k-th largest of those is a lower bound of the k-th
-//      largest logit with few more logits above it than k.
-//   2. A second pass collects the logits above that bound in LDS.  Without a
-//      small top-k it makes a histogram by distance from the maximum instead,
-//      which says how far down the filters and the draw can reach, and a third
-//      pass collects what lies above that.
-//   3. The list is sorted and summed, and the filters and the draw are read
-//      off the sums.
-// A list that would not fit (flat rows) is never made: the histogram leads to
-// one bin for each question, whose elements are listed, or, if they are too
-// many as well, divided by the digits of their keys.
+// A call is four launches over workgroups that find out on the device what is
+// left to do:
+//   1. sample_scan: a thread takes a few dozen logits of a row and leaves their
+//      maximum and, where a filter or the draw is about the whole row, the
+//      sum of their weights relative to that maximum.
+//   2. sample_list, a workgroup a row: the row's maximum; a bound that as many
+//      of the threads' maxima reach as top-k asks for (or kTopThreads); the
+//      logits above it, out of those threads' alone, sorted and summed; the
+//      filters and the draw from the sums.  Peaked rows and any top-k up to
+//      kListK end here, having read the row once.
+//   3. sample_histogram, for the rows that are left (flat ones): weights and
+//      counts by distance from the maximum.
+//   4. sample_flat, a workgroup a row: from there to one bin for each question;
+//      its elements are listed, or, if they are too many for that as well,
+//      divided by the digits of their keys.
 #include "common.hpp"
 
 namespace fence {
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 1024;  // of a workgroup that has a row
 constexpr int kWaves = kThreads / kWave;
-constexpr int kListK = 512;    // largest top-k that the bound from the threads' maxima serves
-constexpr int kList = 4096;    // elements a list holds
-constexpr int kBins = 2048;    // of the histogram; the last one takes everything further away
-constexpr float kReach = 10.0f;  // how far below the maximum the histogram reaches, in units of T
+constexpr int kScanThreads = 256;
+constexpr int kListK = 1024;       // largest top-k that the bound from the threads' maxima serves
+constexpr int kTopThreads = 640;   // threads whose maxima bound the list without a top-k
+constexpr int kList = 4096;        // elements a list holds
+constexpr int kBins = 2048;        // of the histogram; the last one takes everything further away
+constexpr int kMaxVocab = 1 << 26; // so that a row's threads can be counted in 21 bits
+constexpr float kReach = 10.0f;    // how far below the maximum the histogram reaches, in units of T
 typedef unsigned long long u64;
+
+struct RowState {  // from sample_list to the launches behind it
+    uint32_t top;  // the maximum's key
+    uint32_t flat; // whether anything is left to do
+    u64 mass;      // the whole row's weight
+};
 
 struct SampleArgs {
     int32_t* out;
     const float* x;
     int64_t ld;
     int vocab, shift;
+    int slots;  // threads of sample_scan a row has
     const float* temperature;
     const int32_t* top_k;
     const float* top_p;
     const float* min_p;
     const float* u;
+    // workspace, per row
+    double* slot_mass;    // [slots]
+    u64* bin_mass;        // [kBins]
+    RowState* state;
+    uint32_t* slot_top;   // [slots]
+    uint32_t* bin_count;  // [kBins]
 };
 
 // Unsigned keys that order like the logits; NaN as -inf, -0 as 0.
@@ -80,50 +98,172 @@ __device__ __forceinline__ double exp2_64(double y) {
     return ldexp(p, static_cast<int>(n));
 }
 
+// The same to about 3e-10, for the many: 2^y = 2^n 2^(j/64) e^r with |r| <=
+// ln 2 / 128, the middle factor from a table in LDS and e^r - 1 in 32 bits,
+// where its rounding is 2^-24 of 0.0054.  A third of the other's time.
+constexpr int kTable = 64;
+__device__ __forceinline__ void fill_table(double* table) {
+    if (threadIdx.x < kTable) table[threadIdx.x] = 2.0 * exp2_64(threadIdx.x * (1.0 / kTable) - 1.0);
+}
+__device__ __forceinline__ double exp2_table(double y, const double* table) {
+    y = y > -1000.0 ? y : -1000.0;
+    constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number
+    const double z = fma(y, static_cast<double>(kTable), kRound);
+    const int n = static_cast<int>(__builtin_bit_cast(u64, z));
+    const float r = static_cast<float>(fma(z - kRound, -1.0 / kTable, y)) * 0.693147182464599609375f;
+    const float e = r + r * r * (0.5f + r * (0.16666667f + r * 0.041666668f));
+    const double t = table[n & (kTable - 1)];
+    return ldexp(fma(t, static_cast<double>(e), t), n >> 6);
+}
+
+struct Params {
+    int k;        // 0: no top-k
+    float top_p;  // at least 1: none
+    float least;  // 0: no min-p
+    float u;
+    float t;
+    bool greedy;
+    __device__ __forceinline__ Params(const SampleArgs& a, int64_t r) {
+        t = a.temperature ? a.temperature[r] : 1.0f;
+        greedy = !(t > 0.0f);
+        k = a.top_k ? a.top_k[r] : 0;
+        if (k <= 0 || k >= a.vocab) k = 0;
+        top_p = a.top_p ? a.top_p[r] : 1.0f;
+        if (!(top_p < 1.0f)) top_p = 1.0f;
+        const float m = a.min_p ? a.min_p[r] : 0.0f;
+        least = m > 0.0f ? (m < 1.0f ? m : 1.0f) : 0.0f;
+        u = a.u[r];
+    }
+    __device__ __forceinline__ bool use_p() const { return top_p < 1.0f; }
+    // a list of the largest k logits answers everything
+    __device__ __forceinline__ bool by_k(const SampleArgs& a) const { return k && k <= kListK && 2 * k <= a.slots; }
+};
+
+// ------------------------------------------------------------------ 1. scan
+
+// E float4s a thread: which logits slot `slot` of a row has.
+__device__ __forceinline__ int64_t slot_first(int slot, int e, int j) {
+    return 4 * ((static_cast<int64_t>(slot / kScanThreads) * e + j) * kScanThreads + slot % kScanThreads);
+}
+
+// Four logits from index i on; -inf behind the last.
+__device__ __forceinline__ f4 load4(const float* x, int64_t i, int n, bool wide) {
+    if (wide && i + 4 <= n) return *reinterpret_cast<const f4*>(x + i);
+    f4 v;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) v[c] = i + c < n ? x[i + c] : -__builtin_inff();
+    return v;
+}
+
+template <int E>
+__global__ __launch_bounds__(kScanThreads) void sample_scan(SampleArgs a) {
+    __shared__ double table[kTable];
+    const int64_t r = blockIdx.y;
+    const int slot = blockIdx.x * kScanThreads + threadIdx.x;
+    const float* x = a.x + r * a.ld;
+    const bool wide = reinterpret_cast<uintptr_t>(x) % 16 == 0;
+    f4 v[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) v[j] = load4(x, slot_first(slot, E, j), a.vocab, wide);
+    const Params par(a, r);
+    const bool weigh = !par.greedy && !par.by_k(a);
+    if (weigh) {
+        fill_table(table);
+        __syncthreads();
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const uint32_t key = key_of(v[j][c]);
+            top = key > top ? key : top;
+        }
+    a.slot_top[r * a.slots + slot] = top;
+    if (!weigh) return;
+    const double rate = 1.4426950408889634074 / static_cast<double>(par.t);
+    const double ref = static_cast<double>(of_key(top));
+    double sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            // behind the last logit and NaN: weight 0, unless all is -inf, which weighs nothing in the row
+            const float y = v[j][c];
+            if (key_of(y) == top) sum += 1.0;
+            else if (y > -__builtin_inff()) sum += exp2_table((static_cast<double>(y) - ref) * rate, table);
+        }
+    a.slot_mass[r * a.slots + slot] = sum;
+}
+
+// ------------------------------------------------------------------ what the others share
+
 struct Shared {
     u64 mass[kBins];
     uint32_t count[kBins];
     u64 list[kList];  // key << 32 | ~index: larger comes first
+    double table[kTable];
     u64 wave[kWaves];
     u64 found[4];
     uint32_t n;
 };
 
-// What a row's passes have in common.
+// A row and its weights.
 struct Row {
     const float* x;
     int n;
-    bool vec;
+    bool wide;
     uint32_t top;    // the maximum's key
     float top_value;
     double rate;     // log2(e) / T
     double one;      // 2^shift
     float bins_per;  // histogram bins per unit of logit
 
+    __device__ __forceinline__ Row(const SampleArgs& a, int64_t r, float t, uint32_t top_key) {
+        x = a.x + r * a.ld;
+        n = a.vocab;
+        wide = reinterpret_cast<uintptr_t>(x) % 16 == 0;
+        top = top_key;
+        top_value = of_key(top);
+        rate = 1.4426950408889634074 / static_cast<double>(t);
+        one = ldexp(1.0, a.shift);
+        const float per = static_cast<float>(kBins) / kReach / t;
+        bins_per = per < 3e38f ? per : 3e38f;
+    }
+    // f(logit, index) for every one, THREADS of a workgroup from float4 `from` to `to`
+    template <int THREADS, class F>
+    __device__ __forceinline__ void each(int64_t from, int64_t to, F f) const {
+#pragma unroll 4
+        for (int64_t i = from + threadIdx.x; i < to; i += THREADS) {
+            const f4 v = load4(x, 4 * i, n, wide);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (4 * i + j < n) f(v[j], static_cast<int>(4 * i + j));
+        }
+    }
     template <class F>
     __device__ __forceinline__ void each(F f) const {
-        int done = 0;
-        if (vec) {
-            const int n4 = n / 4;
-#pragma unroll 4
-            for (int i = threadIdx.x; i < n4; i += kThreads) {
-                const f4 v = *reinterpret_cast<const f4*>(x + 4 * static_cast<int64_t>(i));
-#pragma unroll
-                for (int j = 0; j < 4; ++j) f(v[j], 4 * i + j);
-            }
-            done = n4 * 4;
-        }
-        for (int64_t i = done + threadIdx.x; i < n; i += kThreads) f(x[i], static_cast<int>(i));
+        each<kThreads>(0, (static_cast<int64_t>(n) + 3) / 4, f);
     }
     __device__ __forceinline__ double weight(uint32_t key) const {
         if (key == top) return 1.0;
         return exp2_64((static_cast<double>(of_key(key)) - static_cast<double>(top_value)) * rate);
     }
     __device__ __forceinline__ u64 units(uint32_t key) const { return static_cast<u64>(rint(weight(key) * one)); }
-    // non-increasing in the key: the order of bins is the order of elements
+    __device__ __forceinline__ u64 units(uint32_t key, const double* table) const {
+        if (key == top) return static_cast<u64>(one);
+        return static_cast<u64>(
+            rint(exp2_table((static_cast<double>(of_key(key)) - static_cast<double>(top_value)) * rate, table) * one));
+    }
+    // never falls as the key does: the order of bins is the order of elements
     __device__ __forceinline__ int bin(uint32_t key) const {
         if (key == top) return 0;
         const float d = (top_value - of_key(key)) * bins_per;
+        return d < static_cast<float>(kBins - 1) ? static_cast<int>(d) : kBins - 1;
+    }
+    // a bin that no element weighing w is more than one away from
+    __device__ __forceinline__ int bin_of_weight(float w, float t) const {
+        const float d = -logf(w) * t * bins_per;
         return d < static_cast<float>(kBins - 1) ? static_cast<int>(d) : kBins - 1;
     }
 };
@@ -164,22 +304,9 @@ __device__ __forceinline__ u64 block_max(Shared& s, u64 v) {
     return v;
 }
 
-// The list's elements that pass `in`, in any order; how many there were,
-// which may be more than a list holds.
-template <class P>
-__device__ __forceinline__ uint32_t collect(Shared& s, const Row& row, P in) {
-    __syncthreads();
-    if (threadIdx.x == 0) s.n = 0;
-    __syncthreads();
-    row.each([&](float x, int i) {
-        const uint32_t key = key_of(x);
-        if (in(key)) {
-            const uint32_t at = atomicAdd(&s.n, 1u);
-            if (at < kList) s.list[at] = static_cast<u64>(key) << 32 | static_cast<uint32_t>(~i);
-        }
-    });
-    __syncthreads();
-    return s.n;
+__device__ __forceinline__ void append(Shared& s, uint32_t key, int index) {
+    const uint32_t at = atomicAdd(&s.n, 1u);
+    if (at < kList) s.list[at] = static_cast<u64>(key) << 32 | static_cast<uint32_t>(~index);
 }
 
 // The first n entries of the list in falling order (bitonic, over the next
@@ -200,84 +327,245 @@ __device__ __forceinline__ void sort_list(Shared& s, int n) {
     __syncthreads();
 }
 
-// Running sums over the sorted list, kPer consecutive entries a thread.
+// Running sums over the sorted list, `per` consecutive entries a thread.
 constexpr int kPer = kList / kThreads;
 struct Sums {
     u64 upto[kPer];  // inclusive
-};
-__device__ __forceinline__ Sums list_sums(Shared& s, const Row& row, int n, int per) {
-    Sums r;
-    u64 mine = 0;
+    int per, n;
+    __device__ __forceinline__ Sums(Shared& s, const Row& row, int count) : n(count) {
+        per = (n + kThreads - 1) / kThreads;
+        u64 mine = 0;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-        const int i = threadIdx.x * per + j;
-        if (j < per && i < n) mine += row.units(static_cast<uint32_t>(s.list[i] >> 32));
-        r.upto[j] = mine;
+        for (int j = 0; j < kPer; ++j) {
+            const int i = threadIdx.x * per + j;
+            if (j < per && i < n) mine += row.units(static_cast<uint32_t>(s.list[i] >> 32));
+            upto[j] = mine;
+        }
+        u64 total;
+        const u64 before = block_scan(s, mine, &total) - mine;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) upto[j] += before;
     }
-    u64 total;
-    const u64 before = block_scan(s, mine, &total) - mine;
+    // the sum at place i < n
+    __device__ __forceinline__ u64 at(Shared& s, int i) const {
+        __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) r.upto[j] += before;
-    return r;
-}
-
-// The first place of the list whose sum passes(), or n - 1, and its sum.
-template <class P>
-__device__ __forceinline__ int first_place(Shared& s, const Sums& sums, int n, int per, P passes, u64* sum) {
-    __syncthreads();
-    if (threadIdx.x == 0) s.found[0] = n - 1;
-    __syncthreads();
-    for (int j = kPer - 1; j >= 0; --j) {
-        const int i = threadIdx.x * per + j;
-        if (j < per && i < n && passes(sums.upto[j])) atomicMin(&s.found[0], static_cast<u64>(i));
+        for (int j = 0; j < kPer; ++j)
+            if (j < per && static_cast<int>(threadIdx.x) * per + j == i) s.found[1] = upto[j];
+        __syncthreads();
+        return s.found[1];
     }
-    __syncthreads();
-    const int at = static_cast<int>(s.found[0]);
+    // the first place whose sum reaches goal, or n - 1
+    __device__ __forceinline__ int reaches(Shared& s, u64 goal) const {
+        __syncthreads();
+        if (threadIdx.x == 0) s.found[0] = n - 1;
+        __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kPer; ++j)
-        if (j < per && static_cast<int>(threadIdx.x) * per + j == at) s.found[1] = sums.upto[j];
-    __syncthreads();
-    *sum = s.found[1];
-    return at;
-}
-
-// A question about the whole order: at which element does the running sum of
-// weights (or the running count) reach `goal`?
-struct Place {
-    int index;
-    u64 mass;  // the running sum of weights there, inclusive
+        for (int j = kPer - 1; j >= 0; --j) {
+            const int i = threadIdx.x * per + j;
+            if (j < per && i < n && upto[j] >= goal) atomicMin(&s.found[0], static_cast<u64>(i));
+        }
+        __syncthreads();
+        return static_cast<int>(s.found[0]);
+    }
 };
 
-// Divides the elements that pass `in` by `digit` (0 .. kBins - 1, falling along
-// the order is 0 first), adding up weights and counts.
-template <class P, class D>
-__device__ __forceinline__ void histogram(Shared& s, const Row& row, P in, D digit) {
+// u times a sum, rounded down: the running sum has to be above it.
+__device__ __forceinline__ u64 draw_goal(float u, u64 mass) {
+    u = u > 0.0f ? u : 0.0f;
+    const u64 goal = static_cast<u64>(static_cast<double>(u) * static_cast<double>(mass)) + 1;
+    return goal < mass ? goal : mass > 0 ? mass : 1;  // u = 1 and above: the last one
+}
+
+__device__ __forceinline__ u64 top_p_goal(float p, u64 mass) {
+    p = p > 0.0f ? p : 0.0f;
+    const u64 goal = static_cast<u64>(ceil(static_cast<double>(p) * static_cast<double>(mass)));
+    return goal < 1 ? 1 : goal < mass ? goal : mass;
+}
+
+// ------------------------------------------------------------------ 2. lists
+
+template <int E>
+__global__ __launch_bounds__(kThreads) void sample_list(SampleArgs a) {
+    __shared__ Shared s;
+    const int64_t r = blockIdx.x;
+    const int tid = threadIdx.x;
+    const Params par(a, r);
+    const uint32_t* tops = a.slot_top + r * a.slots;
+    uint32_t best = 0;
+    for (int i = tid; i < a.slots; i += kThreads) best = tops[i] > best ? tops[i] : best;
+    const uint32_t top = static_cast<uint32_t>(block_max(s, best));
+    if (tid == 0) a.state[r] = RowState{top, 0, 0};
+    if (top <= kKeyLowest) {
+        if (tid == 0) a.out[r] = 0;
+        return;
+    }
+    const Row row(a, r, par.greedy ? 1.0f : par.t, top);
+
+    u64 mass = 0;
+    if (!par.greedy && !par.by_k(a)) {  // the whole row's weight
+        const double* slot_mass = a.slot_mass + r * a.slots;
+        u64 v = 0;
+        for (int i = tid; i < a.slots; i += kThreads) v += static_cast<u64>(rint(slot_mass[i] * row.weight(tops[i]) * row.one));
+        block_scan(s, v, &mass);
+    }
+    // A bound that `want` of the threads' maxima reach, to 16 bits of the key; two bits a turn.
+    uint32_t bound = 0;
+    const bool all = a.vocab <= kList && !par.greedy;
+    const int want = par.by_k(a) ? par.k : kTopThreads < a.slots / 2 ? kTopThreads : a.slots / 2;
+    if (par.greedy) {
+        bound = top;
+    } else if (!all) {
+        for (int bit = 30; bit >= 16; bit -= 2) {
+            uint32_t c[3] = {0, 0, 0};
+            for (int i = tid; i < a.slots; i += kThreads) {
+                const uint32_t t = tops[i];
+#pragma unroll
+                for (int j = 0; j < 3; ++j) c[j] += t >= (bound | static_cast<uint32_t>(j + 1) << bit);
+            }
+            u64 packed = c[0] | static_cast<u64>(c[1]) << 21 | static_cast<u64>(c[2]) << 42, sum;
+            block_scan(s, packed, &sum);
+            for (int j = 2; j >= 0; --j)
+                if (static_cast<int>(sum >> (21 * j) & 0x1FFFFF) >= want) {
+                    bound |= static_cast<uint32_t>(j + 1) << bit;
+                    break;
+                }
+        }
+    }
+    // The logits above it, out of the threads' that have one; s.mass holds those threads' numbers meanwhile.
+    uint32_t* slots = reinterpret_cast<uint32_t*>(s.mass);
+    constexpr int kSlots = kBins * 2;
     __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += kThreads) s.mass[i] = 0, s.count[i] = 0;
+    if (tid == 0) s.n = 0, s.found[2] = 0, s.found[3] = ~0ull;
+    __syncthreads();
+    for (int i = tid; i < a.slots; i += kThreads)
+        if (tops[i] >= bound) {
+            const uint32_t at = static_cast<uint32_t>(atomicAdd(&s.found[2], 1ull));
+            if (at < kSlots) slots[at] = i;
+        }
+    __syncthreads();
+    const uint32_t named = static_cast<uint32_t>(s.found[2]);
+    bool listed = named <= kSlots;
+    if (listed || par.greedy) {
+        const int64_t work = static_cast<int64_t>(listed ? named : a.slots) * E;
+        u64 lowest = ~0ull;
+        for (int64_t w = tid; w < work; w += kThreads) {
+            const int slot = listed ? slots[w / E] : static_cast<int>(w / E);
+            const int64_t i = slot_first(slot, E, static_cast<int>(w % E));
+            const f4 v = load4(row.x, i, row.n, row.wide);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const uint32_t key = key_of(v[c]);
+                if (key < bound || i + c >= row.n) continue;
+                if (par.greedy) lowest = lowest < static_cast<u64>(i + c) ? lowest : static_cast<u64>(i + c);
+                else append(s, key, static_cast<int>(i + c));
+            }
+        }
+        if (par.greedy) {
+            const u64 first = ~block_max(s, ~lowest);
+            if (tid == 0) a.out[r] = static_cast<int>(first);
+            return;
+        }
+        __syncthreads();
+        listed = s.n <= kList;
+    }
+    if (listed) {
+        const int n = static_cast<int>(s.n);
+        sort_list(s, n);
+        const Sums sums(s, row, n);
+        const u64 held = sums.at(s, n - 1);
+        const bool complete = n == row.n;
+        // The filters, as long as the list holds what they keep.
+        bool known = true;
+        int keep = n;
+        u64 kept = complete ? held : mass;
+        if (par.k) {
+            known = par.k <= n;
+            if (known) keep = par.k, kept = sums.at(s, keep - 1);
+        }
+        if (known && par.use_p()) {
+            const u64 goal = top_p_goal(par.top_p, kept);
+            known = goal <= held || complete;
+            const int at = sums.reaches(s, goal);
+            if (known && at + 1 <= keep) keep = at + 1, kept = sums.at(s, at);
+        }
+        if (par.least > 0.0f && (known || !par.k || !par.use_p())) {
+            // An element past the end of the list weighs no more than its last one.  (With both top-k and top-p
+            // the weight that top-p is about has to be known first.)
+            int passing = 0;
+            for (int i = tid; i < keep; i += kThreads)
+                passing += row.weight(static_cast<uint32_t>(s.list[i] >> 32)) >= static_cast<double>(par.least);
+            u64 total;
+            block_scan(s, static_cast<u64>(passing), &total);
+            if (static_cast<int>(total) < n || complete) {
+                known = true;
+                keep = total < 1 ? 1 : static_cast<int>(total);
+                kept = sums.at(s, keep - 1);
+            } else {
+                known = known && (par.k || par.use_p());
+            }
+        }
+        if (known) {
+            const u64 goal = draw_goal(par.u, kept);
+            if (goal <= held || complete) {
+                const int at = sums.reaches(s, goal);
+                if (tid == 0) a.out[r] = static_cast<int>(~static_cast<uint32_t>(s.list[at]));
+                return;
+            }
+        }
+    }
+    // Not here: a histogram, from zero.
+    if (tid == 0) a.state[r] = RowState{top, 1, mass};
+    for (int i = tid; i < kBins; i += kThreads) a.bin_mass[r * kBins + i] = 0, a.bin_count[r * kBins + i] = 0;
+}
+
+// ------------------------------------------------------------------ 3. histograms
+
+// A thread's share of the last bin, which takes most of a peaked row, stays in
+// registers: not through one address.
+__global__ __launch_bounds__(kThreads) void sample_histogram(SampleArgs a, int64_t chunk) {
+    __shared__ u64 mass[kBins];
+    __shared__ uint32_t count[kBins];
+    __shared__ double table[kTable];
+    const int64_t r = blockIdx.y;
+    const RowState state = a.state[r];
+    if (!state.flat) return;
+    const Params par(a, r);
+    const Row row(a, r, par.t, state.top);
+    fill_table(table);
+    for (int i = threadIdx.x; i < kBins; i += kThreads) mass[i] = 0, count[i] = 0;
     __syncthreads();
     u64 last_mass = 0;
     uint32_t last_count = 0;
-    row.each([&](float x, int) {
+    const int64_t n4 = (static_cast<int64_t>(row.n) + 3) / 4;
+    const int64_t from = blockIdx.x * chunk, to = from + chunk < n4 ? from + chunk : n4;
+    row.each<kThreads>(from, to, [&](float x, int) {
         const uint32_t key = key_of(x);
-        if (!in(key)) return;
-        const int d = digit(key);
-        const u64 w = row.units(key);
-        if (d == kBins - 1) {  // most of a peaked row: not through one address
+        const int b = row.bin(key);
+        const u64 w = row.units(key, table);
+        if (b == kBins - 1) {
             last_mass += w;
             ++last_count;
         } else {
-            atomicAdd(&s.mass[d], w);
-            atomicAdd(&s.count[d], 1u);
+            atomicAdd(&mass[b], w);
+            atomicAdd(&count[b], 1u);
         }
     });
     if (last_count) {
-        atomicAdd(&s.mass[kBins - 1], last_mass);
-        atomicAdd(&s.count[kBins - 1], last_count);
+        atomicAdd(&mass[kBins - 1], last_mass);
+        atomicAdd(&count[kBins - 1], last_count);
     }
     __syncthreads();
+    for (int i = threadIdx.x; i < kBins; i += kThreads)
+        if (count[i]) {
+            atomicAdd(&a.bin_mass[r * kBins + i], mass[i]);
+            atomicAdd(&a.bin_count[r * kBins + i], count[i]);
+        }
 }
 
-// The bin in which the running sum (count) reaches goal; what came before it.
+// ------------------------------------------------------------------ 4. flat rows
+
+// The bin of s in which the running sum (count) reaches goal; what came before it.
 __device__ __forceinline__ int find_bin(Shared& s, bool by_count, u64 goal, u64* mass_before, u64* count_before) {
     constexpr int kEach = kBins / kThreads;
     u64 m[kEach], c[kEach], mm = 0, cc = 0, total;
@@ -286,83 +574,103 @@ __device__ __forceinline__ int find_bin(Shared& s, bool by_count, u64 goal, u64*
         mm += m[j] = s.mass[threadIdx.x * kEach + j];
         cc += c[j] = s.count[threadIdx.x * kEach + j];
     }
-    u64 m0 = block_scan(s, mm, &total) - mm;
-    u64 c0 = block_scan(s, cc, &total) - cc;
+    u64 ms = block_scan(s, mm, &total) - mm;
+    u64 cs = block_scan(s, cc, &total) - cc;
     __syncthreads();
     if (threadIdx.x == 0) s.found[0] = ~0ull;
     __syncthreads();
-    u64 ms = m0, cs = c0;
     int at = -1;
     u64 mb = 0, cb = 0;
+    int last = -1;  // this thread's last bin that holds anything, should the sums end below the goal
+    u64 lm = 0, lc = 0;
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
-        if (at < 0 && c[j] && (by_count ? cs + c[j] : ms + m[j]) >= goal) at = threadIdx.x * kEach + j, mb = ms, cb = cs;
+        const int i = threadIdx.x * kEach + j;
+        if (at < 0 && c[j] && (by_count ? cs + c[j] : ms + m[j]) >= goal) at = i, mb = ms, cb = cs;
+        if (c[j]) last = i, lm = ms, lc = cs;
         ms += m[j];
         cs += c[j];
     }
     if (at >= 0) atomicMin(&s.found[0], static_cast<u64>(at));
     __syncthreads();
-    const u64 first = s.found[0];
+    u64 first = s.found[0];
+    if (first == ~0ull) {
+        first = block_max(s, static_cast<u64>(last + 1)) - 1;
+        if (last >= 0 && static_cast<u64>(last) == first) at = last, mb = lm, cb = lc;
+    }
     if (at >= 0 && static_cast<u64>(at) == first) s.found[1] = mb, s.found[2] = cb;
     __syncthreads();
     *mass_before = s.found[1];
     *count_before = s.found[2];
-    return first == ~0ull ? -1 : static_cast<int>(first);
+    return static_cast<int>(first);
 }
 
-// Where the running sum (or count) over the whole row reaches goal >= 1, from
-// the row's histogram by distance, which is in s on entry if `fresh`.
-__device__ __forceinline__ Place locate(Shared& s, const Row& row, bool by_count, u64 goal, bool fresh) {
-    const auto all = [](uint32_t) { return true; };
-    if (!fresh) histogram(s, row, all, [&](uint32_t k) { return row.bin(k); });
+// At which element does the row's running sum of weights (or count) reach a
+// number?
+struct Place {
+    int index;
+    u64 mass;  // the running sum of weights there, inclusive
+};
+
+// For goal >= 1, from the histogram by distance.
+__device__ __forceinline__ Place locate(Shared& s, const SampleArgs& a, int64_t r, const Row& row, bool by_count, u64 goal) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < kBins; i += kThreads) {
+        s.mass[i] = a.bin_mass[r * kBins + i];
+        s.count[i] = a.bin_count[r * kBins + i];
+    }
+    __syncthreads();
     u64 mass, count;
     const int b = find_bin(s, by_count, goal, &mass, &count);
     uint32_t lo = 0, hi = ~0u;  // keys that are left, both inclusive
     int left = static_cast<int>(s.count[b]);
     const auto in = [&](uint32_t k) { return k >= lo && k <= hi && row.bin(k) == b; };
-    // too many for a list: their keys by 11 bits at a time
+    // too many for a list: their keys by 11 bits at a time, the larger digit first
     for (int bits = 32; left > kList && bits > 0;) {
         const int take = bits < 11 ? bits : 11;
         bits -= take;
         const uint32_t mask = (1u << take) - 1;
-        histogram(s, row, in, [&](uint32_t k) { return static_cast<int>(mask - ((k >> bits) & mask)); });
+        __syncthreads();
+        for (int i = threadIdx.x; i < kBins; i += kThreads) s.mass[i] = 0, s.count[i] = 0;
+        __syncthreads();
+        row.each([&](float x, int) {
+            const uint32_t key = key_of(x);
+            if (!in(key)) return;
+            const uint32_t d = mask - ((key >> bits) & mask);
+            atomicAdd(&s.mass[d], row.units(key, s.table));
+            atomicAdd(&s.count[d], 1u);
+        });
+        __syncthreads();
         u64 m, c;
-        const int d = find_bin(s, by_count, by_count ? goal - count : goal - mass, &m, &c);
+        const u64 before = by_count ? count : mass;
+        const int d = find_bin(s, by_count, goal > before ? goal - before : 1, &m, &c);
         mass += m;
         count += c;
         left = static_cast<int>(s.count[d]);
-        const uint32_t digit = mask - static_cast<uint32_t>(d);
-        lo |= digit << bits;
+        lo |= (mask - static_cast<uint32_t>(d)) << bits;
         hi = lo | ((1u << bits) - 1);
     }
     Place p;
+    const u64 before = by_count ? count : mass;
+    const u64 rest = goal > before ? goal - before : 1;
     if (left <= kList) {
-        collect(s, row, in);
+        __syncthreads();
+        if (threadIdx.x == 0) s.n = 0;
+        __syncthreads();
+        row.each([&](float x, int i) {
+            const uint32_t key = key_of(x);
+            if (in(key)) append(s, key, i);
+        });
+        __syncthreads();
         sort_list(s, left);
-        const int per = (left + kThreads - 1) / kThreads;
-        const Sums sums = list_sums(s, row, left, per);
-        u64 sum;
-        int at;
-        if (by_count) {
-            at = static_cast<int>(goal - count) - 1;
-            const int want = at;
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < kPer; ++j)
-                if (j < per && static_cast<int>(threadIdx.x) * per + j == want) s.found[1] = sums.upto[j];
-            __syncthreads();
-            sum = s.found[1];
-        } else {
-            const u64 rest = goal - mass;
-            at = first_place(s, sums, left, per, [&](u64 v) { return v >= rest; }, &sum);
-        }
+        const Sums sums(s, row, left);
+        const int at = by_count ? static_cast<int>(rest < static_cast<u64>(left) ? rest : left) - 1 : sums.reaches(s, rest);
+        p.mass = mass + sums.at(s, at);
         p.index = static_cast<int>(~static_cast<uint32_t>(s.list[at]));
-        p.mass = mass + sum;
     } else {
         // equal logits, more than a list holds: the n-th of them by index
         const u64 w = row.units(lo);
-        u64 nth = by_count ? goal - count : w ? (goal - mass + w - 1) / w : 1;
-        if (nth < 1) nth = 1;
+        u64 nth = by_count ? rest : w ? (rest + w - 1) / w : 1;
         if (nth > static_cast<u64>(left)) nth = left;
         const int64_t each = (static_cast<int64_t>(row.n) + kThreads - 1) / kThreads;
         const int64_t i0 = threadIdx.x * each, i1 = i0 + each < row.n ? i0 + each : row.n;
@@ -384,161 +692,41 @@ __device__ __forceinline__ Place locate(Shared& s, const Row& row, bool by_count
     return p;
 }
 
-// u times a sum, rounded down: the running sum has to be above it.
-__device__ __forceinline__ u64 draw_goal(float u, u64 mass) {
-    u = u > 0.0f ? u : 0.0f;
-    double t = static_cast<double>(u) * static_cast<double>(mass);
-    const u64 goal = static_cast<u64>(t) + 1;
-    return goal < mass ? goal : mass > 0 ? mass : 1;  // u = 1 and above: the last one
-}
-
-__device__ __forceinline__ u64 top_p_goal(float p, u64 mass) {
-    p = p > 0.0f ? p : 0.0f;
-    const u64 goal = static_cast<u64>(ceil(static_cast<double>(p) * static_cast<double>(mass)));
-    return goal < 1 ? 1 : goal < mass ? goal : mass;
-}
-
-__global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
+__global__ __launch_bounds__(kThreads) void sample_flat(SampleArgs a) {
     __shared__ Shared s;
     const int64_t r = blockIdx.x;
-    const float t = a.temperature ? a.temperature[r] : 1.0f;
-    Row row;
-    row.x = a.x + r * a.ld;
-    row.n = a.vocab;
-    row.vec = reinterpret_cast<uintptr_t>(row.x) % 16 == 0;
-    // 1. the maximum, its first index, and this thread's maximum
-    u64 best = 0;
-    row.each([&](float x, int i) {
-        const u64 e = static_cast<u64>(key_of(x)) << 32 | static_cast<uint32_t>(~i);
-        best = e > best ? e : best;
-    });
-    const u64 first = block_max(s, best);
-    row.top = static_cast<uint32_t>(first >> 32);
-    row.top_value = of_key(row.top);
-    if (!(t > 0.0f) || row.top <= kKeyLowest) {
-        if (threadIdx.x == 0)
-            a.out[r] = row.top <= kKeyLowest ? 0 : static_cast<int>(~static_cast<uint32_t>(first));
-        return;
-    }
-    row.rate = 1.4426950408889634074 / static_cast<double>(t);
-    row.one = ldexp(1.0, a.shift);
-    const float per = static_cast<float>(kBins) / kReach / t;
-    row.bins_per = per < 3e38f ? per : 3e38f;
-    int k = a.top_k ? a.top_k[r] : 0;
-    if (k <= 0 || k >= row.n) k = 0;
-    const float top_p = a.top_p ? a.top_p[r] : 1.0f;
-    const bool use_p = top_p < 1.0f;
-    const float min_p = a.min_p ? a.min_p[r] : 0.0f;
-    const float least = min_p > 0.0f ? (min_p < 1.0f ? min_p : 1.0f) : 0.0f;
-    const float u = a.u ? a.u[r] : 0.0f;
-
-    // 2. a list that holds all that the filters keep, if one can
-    int n = 0;
-    u64 mass = 0;  // of the elements that top-p is about, if the list does not say it
-    bool listed = false, fresh = false;
-    if (k && k <= kListK) {
-        // the largest bound (of 16 bits) that k threads' maxima reach
-        uint32_t bound = 0;
-        const uint32_t mine = static_cast<uint32_t>(best >> 32);
-        for (int bit = 31; bit >= 16; --bit) {
-            const uint32_t trial = bound | 1u << bit;
-            if (__syncthreads_count(mine >= trial) >= k) bound = trial;
-        }
-        const uint32_t found = collect(s, row, [&](uint32_t key) { return key >= bound; });
-        listed = found <= kList;
-        n = static_cast<int>(found);
-    }
-    if (!listed) {
-        histogram(s, row, [](uint32_t) { return true; }, [&](uint32_t key) { return row.bin(key); });
-        fresh = true;
-        u64 total = 0, part, before, count;
-        {
-            u64 v = 0;
-            for (int i = threadIdx.x; i < kBins; i += kThreads) v += s.mass[i];
-            block_scan(s, v, &total);
-        }
-        mass = total;
-        // the last bin that matters
-        int reach = kBins - 1;
-        if (k) {
-            reach = find_bin(s, true, k, &before, &count);
-        } else {
-            if (use_p) reach = find_bin(s, false, top_p_goal(top_p, total), &before, &count);
-            else if (!(least > 0.0f)) reach = find_bin(s, false, draw_goal(u, total), &before, &count);
-        }
-        if (least > 0.0f && !(k && use_p)) {  // (top-p after top-k needs the weight of all k.)  One bin more than the distance says, for its rounding
-            const float d = -logf(least) * t * row.bins_per + 1.0f;
-            const int last = d < static_cast<float>(kBins - 1) ? static_cast<int>(d) + 1 : kBins - 1;
-            reach = last < reach ? last : reach;
-        }
+    const RowState state = a.state[r];
+    if (!state.flat) return;
+    const Params par(a, r);
+    const Row row(a, r, par.t, state.top);
+    fill_table(s.table);
+    __syncthreads();
+    u64 kept = state.mass;
+    if (par.by_k(a)) {  // sample_scan summed nothing: its list was too long for ties
         u64 v = 0;
-        for (int i = threadIdx.x; i <= reach; i += kThreads) v += s.count[i];
-        block_scan(s, v, &part);
-        if (part <= kList) {
-            collect(s, row, [&](uint32_t key) { return row.bin(key) <= reach; });
-            n = static_cast<int>(part);
-            listed = true;
-        }
+        for (int i = threadIdx.x; i < kBins; i += kThreads) v += a.bin_mass[r * kBins + i];
+        block_scan(s, v, &kept);
     }
-
-    if (listed) {
-        // 3. the filters and the draw on the sorted list
-        sort_list(s, n);
-        const int per_thread = (n + kThreads - 1) / kThreads;
-        const Sums sums = list_sums(s, row, n, per_thread);
-        int keep = n;
-        u64 kept = mass, sum;
-        if (k && k <= n) {
-            keep = k;
-            // the sum at place k - 1
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < kPer; ++j)
-                if (j < per_thread && static_cast<int>(threadIdx.x) * per_thread + j == k - 1) s.found[1] = sums.upto[j];
-            __syncthreads();
-            kept = s.found[1];
-        }
-        if (use_p) {
-            const u64 goal = top_p_goal(top_p, kept);
-            const int at = first_place(s, sums, n, per_thread, [&](u64 v) { return v >= goal; }, &sum);
-            if (at + 1 <= keep) keep = at + 1, kept = sum;
-        }
-        if (least > 0.0f) {
-            int passing = 0;
-            for (int i = threadIdx.x; i < keep; i += kThreads)
-                passing += row.weight(static_cast<uint32_t>(s.list[i] >> 32)) >= static_cast<double>(least);
-            u64 total;
-            block_scan(s, static_cast<u64>(passing), &total);
-            keep = total < 1 ? 1 : static_cast<int>(total);
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < kPer; ++j)
-                if (j < per_thread && static_cast<int>(threadIdx.x) * per_thread + j == keep - 1) s.found[1] = sums.upto[j];
-            __syncthreads();
-            kept = s.found[1];
-        }
-        const u64 goal = draw_goal(u, kept);
-        const int at = first_place(s, sums, n, per_thread, [&](u64 v) { return v >= goal; }, &sum);
-        if (threadIdx.x == 0) a.out[r] = static_cast<int>(~static_cast<uint32_t>(s.list[at]));
-        return;
-    }
-
-    // A flat row: one question at a time on the whole of it.
-    u64 kept = mass;
-    if (k) kept = locate(s, row, true, k, fresh).mass, fresh = false;
-    if (use_p) kept = locate(s, row, false, top_p_goal(top_p, kept), fresh).mass, fresh = false;
-    if (least > 0.0f) {
+    if (par.k) kept = locate(s, a, r, row, true, par.k).mass;
+    if (par.use_p()) kept = locate(s, a, r, row, false, top_p_goal(par.top_p, kept)).mass;
+    if (par.least > 0.0f) {
+        // whole bins above the border's, and what weighs enough in the three about it
+        const int border = row.bin_of_weight(par.least, par.t);
         u64 v = 0, total;
+        for (int i = threadIdx.x; i < border - 1; i += kThreads) v += a.bin_mass[r * kBins + i];
         row.each([&](float x, int) {
             const uint32_t key = key_of(x);
-            if (row.weight(key) >= static_cast<double>(least)) v += row.units(key);
+            const int b = row.bin(key);
+            if (b >= border - 1 && b <= border + 1 && row.weight(key) >= static_cast<double>(par.least)) v += row.units(key);
         });
         block_scan(s, v, &total);
         kept = total < kept ? total : kept;
     }
-    const Place p = locate(s, row, false, draw_goal(u, kept), fresh);
+    const Place p = locate(s, a, r, row, false, draw_goal(par.u, kept));
     if (threadIdx.x == 0) a.out[r] = p.index;
 }
+
+// ------------------------------------------------------------------ host
 
 int shift_for(int vocab) {
     int bits = 1;
@@ -546,19 +734,37 @@ int shift_for(int vocab) {
     return 62 - bits;  // the sum of vocab weights of at most 2^shift stays below 2^63
 }
 
+// float4s a thread of sample_scan takes: fewer while the grid would not fill the GPU.
+int scan_width(int64_t rows, int vocab) {
+    const int64_t wide = (static_cast<int64_t>(vocab) + 40 * kScanThreads - 1) / (40 * kScanThreads);
+    return rows * wide < 512 ? 3 : 10;
+}
+int slots_of(int64_t rows, int vocab) {
+    const int64_t per = 4ll * scan_width(rows, vocab) * kScanThreads;
+    return static_cast<int>((vocab + per - 1) / per) * kScanThreads;
+}
+
+int64_t row_bytes(int slots) {
+    return slots * static_cast<int64_t>(sizeof(double) + sizeof(uint32_t)) +
+           kBins * static_cast<int64_t>(sizeof(u64) + sizeof(uint32_t)) + static_cast<int64_t>(sizeof(RowState));
+}
+
 }  // namespace
 }  // namespace fence
 
 extern "C" int64_t fence_sample_workspace(int64_t rows, int vocab) {
-    if (rows < 0 || vocab < 1) return 0;
-    return 16;
+    using namespace fence;
+    if (rows < 0 || rows > INT32_MAX || vocab < 1 || vocab > kMaxVocab) return 0;
+    const int64_t n = rows * row_bytes(slots_of(rows, vocab));
+    return n < 16 ? 16 : n;
 }
 
 extern "C" int fence_sample(int32_t* out, const float* logits, int64_t rows, int vocab, int64_t ld,
                             const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
                             const float* u, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
     using namespace fence;
-    if (!out || !logits || !u || !workspace || rows < 0 || vocab < 1 || ld < vocab) return FENCE_ERROR_INVALID_VALUE;
+    if (!out || !logits || !u || !workspace || rows < 0 || vocab < 1 || vocab > kMaxVocab || ld < vocab)
+        return FENCE_ERROR_INVALID_VALUE;
     if (rows > INT32_MAX || ld > INT64_MAX / 8 / (rows + 1)) return FENCE_ERROR_INVALID_VALUE;
     if (!aligned(out, 4) || !aligned(logits, 4) || !aligned(u, 4) || !aligned(workspace, 16) ||
         (temperature && !aligned(temperature, 4)) || (top_k && !aligned(top_k, 4)) || (top_p && !aligned(top_p, 4)) ||
@@ -566,14 +772,45 @@ extern "C" int fence_sample(int32_t* out, const float* logits, int64_t rows, int
         return FENCE_ERROR_INVALID_VALUE;
     if (workspace_bytes < fence_sample_workspace(rows, vocab)) return FENCE_ERROR_INVALID_VALUE;
     if (rows == 0) return FENCE_SUCCESS;
-    const int64_t most = kMaxLaunchLanes / kThreads;  // rows of a launch
-    for (int64_t r0 = 0; r0 < rows; r0 += most) {
-        const int64_t m = rows - r0 < most ? rows - r0 : most;
-        const SampleArgs part{out + r0, logits + r0 * ld, ld, vocab, shift_for(vocab), temperature ? temperature + r0 : nullptr,
-                              top_k ? top_k + r0 : nullptr, top_p ? top_p + r0 : nullptr,
-                              min_p ? min_p + r0 : nullptr, u + r0};
-        if (const int st = launch(sample_kernel, dim3(static_cast<unsigned>(m)), dim3(kThreads), 0, stream, part))
+    const int slots = slots_of(rows, vocab), width = scan_width(rows, vocab);
+    SampleArgs a{out, logits, ld, vocab, shift_for(vocab), slots, temperature, top_k, top_p, min_p, u,
+                 nullptr, nullptr, nullptr, nullptr, nullptr};
+    a.slot_mass = static_cast<double*>(workspace);
+    a.bin_mass = reinterpret_cast<u64*>(a.slot_mass + rows * slots);
+    a.state = reinterpret_cast<RowState*>(a.bin_mass + rows * kBins);
+    a.slot_top = reinterpret_cast<uint32_t*>(a.state + rows);
+    a.bin_count = a.slot_top + rows * slots;
+    const int64_t n4 = (static_cast<int64_t>(vocab) + 3) / 4;
+    // workgroups a row's histogram takes: enough to fill the GPU, none with fewer than 2048 logits
+    int64_t parts = (1024 + rows - 1) / rows, chunk;
+    if (parts > (n4 + 511) / 512) parts = (n4 + 511) / 512;
+    chunk = (n4 + parts - 1) / parts;
+    constexpr int64_t kRows = 32768;  // of a launch: grid.y and the lanes of a grid are bounded
+    for (int64_t r0 = 0; r0 < rows; r0 += kRows) {
+        const unsigned m = static_cast<unsigned>(rows - r0 < kRows ? rows - r0 : kRows);
+        SampleArgs p = a;
+        p.out += r0;
+        p.x += r0 * ld;
+        if (p.temperature) p.temperature += r0;
+        if (p.top_k) p.top_k += r0;
+        if (p.top_p) p.top_p += r0;
+        if (p.min_p) p.min_p += r0;
+        p.u += r0;
+        p.slot_mass += r0 * slots;
+        p.bin_mass += r0 * kBins;
+        p.state += r0;
+        p.slot_top += r0 * slots;
+        p.bin_count += r0 * kBins;
+        const dim3 scan(slots / kScanThreads, m);
+        int st = width == 3 ? launch(sample_scan<3>, scan, dim3(kScanThreads), 0, stream, p)
+                            : launch(sample_scan<10>, scan, dim3(kScanThreads), 0, stream, p);
+        if (st) return st;
+        st = width == 3 ? launch(sample_list<3>, dim3(m), dim3(kThreads), 0, stream, p)
+                        : launch(sample_list<10>, dim3(m), dim3(kThreads), 0, stream, p);
+        if (st) return st;
+        if ((st = launch(sample_histogram, dim3(static_cast<unsigned>(parts), m), dim3(kThreads), 0, stream, p, chunk)))
             return st;
+        if ((st = launch(sample_flat, dim3(m), dim3(kThreads), 0, stream, p))) return st;
     }
     return FENCE_SUCCESS;
 }

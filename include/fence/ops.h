@@ -444,7 +444,7 @@ int64_t fence_gqa_attention_q8_workspace(int batch, int max_q_len, int n_q_heads
  * out-of-range filters (top_k outside 1..vocab-1, top_p not below 1, min_p
  * not above 0): off.  temperature <= 0: the largest logit, the lowest index
  * first.  NaN logits count as -inf; +inf ones share all the weight; a row
- * with nothing above -inf gives 0.
+ * with nothing above -inf gives 0.  vocab <= 2^26.
  * workspace: fence_sample_workspace(rows, vocab) bytes, 16-byte aligned;
  * calls that overlap must not share it. */
 int fence_sample(int32_t* out, const float* logits, int64_t rows, int vocab, int64_t ld,

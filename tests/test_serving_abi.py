@@ -91,7 +91,8 @@ def sample(out=P[0], x=P[1], rows=0, vocab=100, ld=100, t=None, k=None, p=None, 
 @pytest.mark.parametrize("change", [
     dict(out=None), dict(x=None), dict(u=None), dict(ws=None), dict(rows=-1), dict(vocab=0), dict(ld=99), dict(size=0),
     dict(out=P[0] + 2), dict(x=P[1] + 1), dict(t=P[4] + 2), dict(k=P[4] + 2), dict(p=P[4] + 1), dict(m=P[4] + 3),
-    dict(u=P[2] + 2), dict(ws=P[3] + 8), dict(rows=2 ** 31), dict(ld=2 ** 62, rows=4)])
+    dict(u=P[2] + 2), dict(ws=P[3] + 8), dict(rows=2 ** 31), dict(ld=2 ** 62, rows=4),
+    dict(vocab=2 ** 26 + 1, ld=2 ** 27)])
 def test_sample_refuses(change):
     assert sample() == OK
     assert sample(**change) == E
@@ -99,7 +100,7 @@ def test_sample_refuses(change):
 
 def test_sample_workspace():
     assert F.sample_workspace(1, 1) > 0
-    assert F.sample_workspace(-1, 5) == 0 and F.sample_workspace(1, 0) == 0
+    assert F.sample_workspace(-1, 5) == 0 and F.sample_workspace(1, 0) == 0 and F.sample_workspace(1, 2 ** 26 + 1) == 0
 
 
 def test_reference_codes():
