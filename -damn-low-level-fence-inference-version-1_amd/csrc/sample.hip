@@ -38,7 +38,7 @@ constexpr int kTopThreads = 640;   // threads whose maxima bound the list withou
 constexpr int kList = 4096;        // elements a list holds
 constexpr int kBins = 2048;        // of the histogram; the last one takes everything further away
 constexpr int kMaxVocab = 1 << 26; // so that a row's threads can be counted in 21 bits
-constexpr float kReach = 10.0f;    // how far below the maximum the histogram reaches, in units of T
+constexpr float kReach = 24.0f;    // how far below the maximum the histogram reaches, in units of T
 typedef unsigned long long u64;
 
 struct RowState {  // from sample_list to the launches behind it
@@ -309,16 +309,41 @@ __device__ __forceinline__ void append(Shared& s, uint32_t key, int index) {
     if (at < kList) s.list[at] = static_cast<u64>(key) << 32 | static_cast<uint32_t>(~index);
 }
 
-// The first n entries of the list in falling order (bitonic, over the next
-// power of two, filled up with zeros, which come last).
+// The first n entries of the list in falling order: a bitonic network over the
+// next power of two, filled up with zeros, which come last.  Up to one entry a
+// thread the entries stay in registers and only exchanges across waves go
+// through LDS and a barrier (10 of 55 steps for 1024 entries).
 __device__ __forceinline__ void sort_list(Shared& s, int n) {
     int size = kWave;
     while (size < n) size *= 2;
-    for (int i = n + threadIdx.x; i < size; i += kThreads) s.list[i] = 0;
+    const int tid = threadIdx.x;
+    if (size <= kThreads) {
+        u64 v = tid < n ? s.list[tid] : 0;
+        for (int k = 2; k <= size; k *= 2)
+            for (int j = k / 2; j > 0; j /= 2) {
+                u64 o;
+                if (j >= kWave) {
+                    __syncthreads();
+                    if (tid < size) s.list[tid] = v;
+                    __syncthreads();
+                    o = tid < size ? s.list[tid ^ j] : 0;
+                } else {
+                    if (tid >= size) continue;
+                    o = __shfl_xor(v, j);
+                }
+                const bool larger = ((tid & j) == 0) == ((tid & k) == 0);  // this place keeps the larger one
+                v = (o > v) == larger ? o : v;
+            }
+        __syncthreads();
+        if (tid < size) s.list[tid] = v;
+        __syncthreads();
+        return;
+    }
+    for (int i = n + tid; i < size; i += kThreads) s.list[i] = 0;
     for (int k = 2; k <= size; k *= 2)
         for (int j = k / 2; j > 0; j /= 2) {
             __syncthreads();
-            for (int i = threadIdx.x; i < size / 2; i += kThreads) {
+            for (int i = tid; i < size / 2; i += kThreads) {
                 const int a = 2 * i - (i & (j - 1)), b = a + j;
                 const u64 x = s.list[a], y = s.list[b];
                 if ((x < y) == ((a & k) == 0)) s.list[a] = y, s.list[b] = x;
@@ -392,8 +417,18 @@ __global__ __launch_bounds__(kThreads) void sample_list(SampleArgs a) {
     const int tid = threadIdx.x;
     const Params par(a, r);
     const uint32_t* tops = a.slot_top + r * a.slots;
-    uint32_t best = 0;
-    for (int i = tid; i < a.slots; i += kThreads) best = tops[i] > best ? tops[i] : best;
+    // the threads' maxima, the first kKept a thread in registers (a row of up to 320,000 logits)
+    constexpr int kKept = 8;
+    uint32_t kept_tops[kKept], best = 0;
+#pragma unroll
+    for (int j = 0; j < kKept; ++j) kept_tops[j] = tid + j * kThreads < a.slots ? tops[tid + j * kThreads] : 0;
+    const auto each_top = [&](auto f) {
+#pragma unroll
+        for (int j = 0; j < kKept; ++j)
+            if (j * kThreads < a.slots) f(kept_tops[j], tid + j * kThreads);
+        for (int i = tid + kKept * kThreads; __any(i < a.slots); i += kThreads) f(i < a.slots ? tops[i] : 0, i);
+    };
+    each_top([&](uint32_t t, int) { best = t > best ? t : best; });
     const uint32_t top = static_cast<uint32_t>(block_max(s, best));
     if (tid == 0) a.state[r] = RowState{top, 0, 0};
     if (top <= kKeyLowest) {
@@ -406,7 +441,9 @@ __global__ __launch_bounds__(kThreads) void sample_list(SampleArgs a) {
     if (!par.greedy && !par.by_k(a)) {  // the whole row's weight
         const double* slot_mass = a.slot_mass + r * a.slots;
         u64 v = 0;
-        for (int i = tid; i < a.slots; i += kThreads) v += static_cast<u64>(rint(slot_mass[i] * row.weight(tops[i]) * row.one));
+        each_top([&](uint32_t t, int i) {
+            if (i < a.slots) v += static_cast<u64>(rint(slot_mass[i] * row.weight(t) * row.one));
+        });
         block_scan(s, v, &mass);
     }
     // A bound that `want` of the threads' maxima reach, to 16 bits of the key; two bits a turn.
@@ -416,15 +453,21 @@ __global__ __launch_bounds__(kThreads) void sample_list(SampleArgs a) {
     if (par.greedy) {
         bound = top;
     } else if (!all) {
+        int turn = 0;  // the two halves of s.list take turns, so one barrier a turn is enough
         for (int bit = 30; bit >= 16; bit -= 2) {
-            uint32_t c[3] = {0, 0, 0};
-            for (int i = tid; i < a.slots; i += kThreads) {
-                const uint32_t t = tops[i];
+            uint32_t c[3] = {0, 0, 0};  // the same in every lane
+            each_top([&](uint32_t t, int) {
 #pragma unroll
-                for (int j = 0; j < 3; ++j) c[j] += t >= (bound | static_cast<uint32_t>(j + 1) << bit);
-            }
-            u64 packed = c[0] | static_cast<u64>(c[1]) << 21 | static_cast<u64>(c[2]) << 42, sum;
-            block_scan(s, packed, &sum);
+                for (int j = 0; j < 3; ++j)
+                    c[j] += __builtin_popcountll(__ballot(t >= (bound | static_cast<uint32_t>(j + 1) << bit)));
+            });
+            u64* sums = s.list + turn * kWaves;
+            if (tid % kWave == 0) sums[tid / kWave] = c[0] | static_cast<u64>(c[1]) << 21 | static_cast<u64>(c[2]) << 42;
+            __syncthreads();
+            u64 sum = 0;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) sum += sums[w];
+            turn ^= 1;
             for (int j = 2; j >= 0; --j)
                 if (static_cast<int>(sum >> (21 * j) & 0x1FFFFF) >= want) {
                     bound |= static_cast<uint32_t>(j + 1) << bit;
@@ -438,28 +481,38 @@ __global__ __launch_bounds__(kThreads) void sample_list(SampleArgs a) {
     __syncthreads();
     if (tid == 0) s.n = 0, s.found[2] = 0, s.found[3] = ~0ull;
     __syncthreads();
-    for (int i = tid; i < a.slots; i += kThreads)
-        if (tops[i] >= bound) {
+    each_top([&](uint32_t t, int i) {
+        if (t >= bound && i < a.slots) {
             const uint32_t at = static_cast<uint32_t>(atomicAdd(&s.found[2], 1ull));
             if (at < kSlots) slots[at] = i;
         }
+    });
     __syncthreads();
     const uint32_t named = static_cast<uint32_t>(s.found[2]);
     bool listed = named <= kSlots;
     if (listed || par.greedy) {
         const int64_t work = static_cast<int64_t>(listed ? named : a.slots) * E;
         u64 lowest = ~0ull;
-        for (int64_t w = tid; w < work; w += kThreads) {
-            const int slot = listed ? slots[w / E] : static_cast<int>(w / E);
-            const int64_t i = slot_first(slot, E, static_cast<int>(w % E));
-            const f4 v = load4(row.x, i, row.n, row.wide);
+        constexpr int AHEAD = 4;
+        for (int64_t w0 = tid; w0 < work; w0 += AHEAD * kThreads) {
+            f4 v[AHEAD];
+            int64_t at[AHEAD];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const uint32_t key = key_of(v[c]);
-                if (key < bound || i + c >= row.n) continue;
-                if (par.greedy) lowest = lowest < static_cast<u64>(i + c) ? lowest : static_cast<u64>(i + c);
-                else append(s, key, static_cast<int>(i + c));
+            for (int d = 0; d < AHEAD; ++d) {
+                const int64_t w = w0 + d * kThreads;
+                const int slot = w >= work ? 0 : listed ? slots[w / E] : static_cast<int>(w / E);
+                at[d] = w < work ? slot_first(slot, E, static_cast<int>(w % E)) : row.n;
+                v[d] = load4(row.x, at[d], row.n, row.wide);
             }
+#pragma unroll
+            for (int d = 0; d < AHEAD; ++d)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const uint32_t key = key_of(v[d][c]);
+                    if (key < bound || at[d] + c >= row.n) continue;
+                    if (par.greedy) lowest = lowest < static_cast<u64>(at[d] + c) ? lowest : static_cast<u64>(at[d] + c);
+                    else append(s, key, static_cast<int>(at[d] + c));
+                }
         }
         if (par.greedy) {
             const u64 first = ~block_max(s, ~lowest);
@@ -692,6 +745,45 @@ __device__ __forceinline__ Place locate(Shared& s, const SampleArgs& a, int64_t 
     return p;
 }
 
+// Top-p and the draw at once: wherever in its bin the border of top-p lies,
+// the draw's goal mostly falls into the same bin, and one pass lists both bins.
+// False if it does not, or they are too many.
+__device__ __forceinline__ bool top_p_and_draw(Shared& s, const SampleArgs& a, int64_t r, const Row& row, u64 goal, float u,
+                                               int* index) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < kBins; i += kThreads) {
+        s.mass[i] = a.bin_mass[r * kBins + i];
+        s.count[i] = a.bin_count[r * kBins + i];
+    }
+    __syncthreads();
+    u64 before_p, before_d, count;
+    const int bp = find_bin(s, false, goal, &before_p, &count);
+    const int bd = find_bin(s, false, draw_goal(u, before_p + 1), &before_d, &count);
+    const int bd_last = find_bin(s, false, draw_goal(u, before_p + s.mass[bp]), &before_d, &count);
+    const int nd = static_cast<int>(s.count[bd]), n = nd + (bp == bd ? 0 : static_cast<int>(s.count[bp]));
+    if (bd != bd_last || n > kList) return false;
+    __syncthreads();
+    if (threadIdx.x == 0) s.n = 0;
+    __syncthreads();
+    row.each([&](float x, int i) {
+        const uint32_t key = key_of(x);
+        const int b = row.bin(key);
+        if (b == bp || b == bd) append(s, key, i);
+    });
+    __syncthreads();
+    sort_list(s, n);  // the draw's bin comes first, if they are two
+    const Sums sums(s, row, n);
+    const u64 of_draw = bp == bd ? 0 : sums.at(s, nd - 1);
+    const u64 rest = goal > before_p ? goal - before_p : 1;
+    const int at = sums.reaches(s, rest + of_draw);
+    const u64 kept = before_p + sums.at(s, at) - of_draw;
+    const u64 draw = draw_goal(u, kept);
+    int place = sums.reaches(s, draw > before_d ? draw - before_d : 1);
+    if (place >= nd) place = nd - 1;
+    *index = static_cast<int>(~static_cast<uint32_t>(s.list[place]));
+    return true;
+}
+
 __global__ __launch_bounds__(kThreads) void sample_flat(SampleArgs a) {
     __shared__ Shared s;
     const int64_t r = blockIdx.x;
@@ -708,7 +800,15 @@ __global__ __launch_bounds__(kThreads) void sample_flat(SampleArgs a) {
         block_scan(s, v, &kept);
     }
     if (par.k) kept = locate(s, a, r, row, true, par.k).mass;
-    if (par.use_p()) kept = locate(s, a, r, row, false, top_p_goal(par.top_p, kept)).mass;
+    if (par.use_p()) {
+        const u64 goal = top_p_goal(par.top_p, kept);
+        int index;
+        if (!(par.least > 0.0f) && top_p_and_draw(s, a, r, row, goal, par.u, &index)) {
+            if (threadIdx.x == 0) a.out[r] = index;
+            return;
+        }
+        kept = locate(s, a, r, row, false, goal).mass;
+    }
     if (par.least > 0.0f) {
         // whole bins above the border's, and what weighs enough in the three about it
         const int border = row.bin_of_weight(par.least, par.t);
@@ -737,7 +837,7 @@ int shift_for(int vocab) {
 // float4s a thread of sample_scan takes: fewer while the grid would not fill the GPU.
 int scan_width(int64_t rows, int vocab) {
     const int64_t wide = (static_cast<int64_t>(vocab) + 40 * kScanThreads - 1) / (40 * kScanThreads);
-    return rows * wide < 512 ? 3 : 10;
+    return rows * wide < 512 ? 5 : 10;
 }
 int slots_of(int64_t rows, int vocab) {
     const int64_t per = 4ll * scan_width(rows, vocab) * kScanThreads;
@@ -802,10 +902,10 @@ extern "C" int fence_sample(int32_t* out, const float* logits, int64_t rows, int
         p.slot_top += r0 * slots;
         p.bin_count += r0 * kBins;
         const dim3 scan(slots / kScanThreads, m);
-        int st = width == 3 ? launch(sample_scan<3>, scan, dim3(kScanThreads), 0, stream, p)
+        int st = width == 5 ? launch(sample_scan<5>, scan, dim3(kScanThreads), 0, stream, p)
                             : launch(sample_scan<10>, scan, dim3(kScanThreads), 0, stream, p);
         if (st) return st;
-        st = width == 3 ? launch(sample_list<3>, dim3(m), dim3(kThreads), 0, stream, p)
+        st = width == 5 ? launch(sample_list<5>, dim3(m), dim3(kThreads), 0, stream, p)
                         : launch(sample_list<10>, dim3(m), dim3(kThreads), 0, stream, p);
         if (st) return st;
         if ((st = launch(sample_histogram, dim3(static_cast<unsigned>(parts), m), dim3(kThreads), 0, stream, p, chunk)))
