@@ -34,9 +34,9 @@ constexpr int kThreads = 1024;  // of a workgroup that has a row
 constexpr int kWaves = kThreads / kWave;
 constexpr int kScanThreads = 256;
 constexpr int kListK = 1024;       // largest top-k that the bound from the threads' maxima serves
-constexpr int kTopThreads = 640;   // threads whose maxima bound the list without a top-k
+constexpr int kTopThreads = 320;   // threads whose maxima bound the list without a top-k
 constexpr int kList = 4096;        // elements a list holds
-constexpr int kBins = 2048;        // of the histogram; the last one takes everything further away
+constexpr int kBins = 4096;        // of the histogram; the last one takes everything further away
 constexpr int kMaxVocab = 1 << 26; // so that a row's threads can be counted in 21 bits
 constexpr float kReach = 24.0f;    // how far below the maximum the histogram reaches, in units of T
 typedef unsigned long long u64;
@@ -230,15 +230,27 @@ struct Row {
         const float per = static_cast<float>(kBins) / kReach / t;
         bins_per = per < 3e38f ? per : 3e38f;
     }
-    // f(logit, index) for every one, THREADS of a workgroup from float4 `from` to `to`
+    // f(logit, index) for every one, THREADS of a workgroup from float4 `from` to `to`; AHEAD loads a thread in
+    // flight, which the compiler would not move over what f does.
     template <int THREADS, class F>
     __device__ __forceinline__ void each(int64_t from, int64_t to, F f) const {
-#pragma unroll 4
-        for (int64_t i = from + threadIdx.x; i < to; i += THREADS) {
-            const f4 v = load4(x, 4 * i, n, wide);
+        constexpr int AHEAD = 8;
+        for (int64_t i0 = from + threadIdx.x; i0 < to; i0 += AHEAD * THREADS) {
+            f4 v[AHEAD];
+            if (wide && 4 * (i0 + (AHEAD - 1) * THREADS) + 4 <= n) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (4 * i + j < n) f(v[j], static_cast<int>(4 * i + j));
+                for (int d = 0; d < AHEAD; ++d) v[d] = *reinterpret_cast<const f4*>(x + 4 * (i0 + d * THREADS));
+            } else {
+#pragma unroll
+                for (int d = 0; d < AHEAD; ++d) v[d] = load4(x, 4 * (i0 + d * THREADS), n, wide);
+            }
+#pragma unroll
+            for (int d = 0; d < AHEAD; ++d) {
+                const int64_t i = i0 + d * THREADS;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (i < to && 4 * i + j < n) f(v[d][j], static_cast<int>(4 * i + j));
+            }
         }
     }
     template <class F>
@@ -260,6 +272,14 @@ struct Row {
         if (key == top) return 0;
         const float d = (top_value - of_key(key)) * bins_per;
         return d < static_cast<float>(kBins - 1) ? static_cast<int>(d) : kBins - 1;
+    }
+    // Logits that a bin's elements lie between, with room for the rounding of bin(): two comparisons a logit leave
+    // few for the exact test.  NaN passes.
+    __device__ __forceinline__ void bin_range(int b, float* least, float* most) const {
+        const float room = fabsf(top_value) * 0x1p-20f + 2.0f / bins_per;
+        *most = top_value - static_cast<float>(b) / bins_per + room;
+        *least = b == kBins - 1 ? -__builtin_inff() : top_value - static_cast<float>(b + 1) / bins_per - room;
+        if (top_value == __builtin_inff()) *least = -__builtin_inff(), *most = __builtin_inff();
     }
     // a bin that no element weighing w is more than one away from
     __device__ __forceinline__ int bin_of_weight(float w, float t) const {
@@ -410,6 +430,40 @@ __device__ __forceinline__ u64 top_p_goal(float p, u64 mass) {
 
 // ------------------------------------------------------------------ 2. lists
 
+// The answer from a list of up to 64 logits with the largest k among them: one
+// wave, an entry a lane, without a barrier.
+__device__ __forceinline__ void short_list(Shared& s, const SampleArgs& a, int64_t r, const Row& row, const Params& par, int n) {
+    const int lane = threadIdx.x;
+    u64 v = lane < n ? s.list[lane] : 0;
+#pragma unroll
+    for (int k = 2; k <= kWave; k *= 2)
+#pragma unroll
+        for (int j = k / 2; j > 0; j /= 2) {
+            const u64 o = __shfl_xor(v, j);
+            v = (o > v) == (((lane & j) == 0) == ((lane & k) == 0)) ? o : v;
+        }
+    const double w = lane < par.k ? row.weight(static_cast<uint32_t>(v >> 32)) : 0.0;
+    u64 upto = static_cast<u64>(rint(w * row.one));
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+        const u64 up = __shfl_up(upto, d);
+        if (lane >= d) upto += up;
+    }
+    int keep = par.k;  // at most n
+    if (par.use_p()) {
+        const u64 goal = top_p_goal(par.top_p, __shfl(upto, kWave - 1));
+        keep = __builtin_ctzll(__ballot(upto >= goal)) + 1;
+        if (keep > par.k) keep = par.k;
+    }
+    if (par.least > 0.0f) {
+        const int passing = __builtin_popcountll(__ballot(lane < keep && w >= static_cast<double>(par.least)));
+        keep = passing < 1 ? 1 : passing;
+    }
+    const u64 goal = draw_goal(par.u, __shfl(upto, keep - 1));
+    const int at = __builtin_ctzll(__ballot(upto >= goal));
+    if (lane == at) a.out[r] = static_cast<int>(~static_cast<uint32_t>(v));
+}
+
 template <int E>
 __global__ __launch_bounds__(kThreads) void sample_list(SampleArgs a) {
     __shared__ Shared s;
@@ -453,14 +507,18 @@ __global__ __launch_bounds__(kThreads) void sample_list(SampleArgs a) {
     if (par.greedy) {
         bound = top;
     } else if (!all) {
+        // Where that is enough, out of each thread's largest alone: a somewhat lower bound for an eighth of the work.
+        const bool few = 2 * want <= (a.slots < kThreads ? a.slots : kThreads);
         int turn = 0;  // the two halves of s.list take turns, so one barrier a turn is enough
         for (int bit = 30; bit >= 16; bit -= 2) {
             uint32_t c[3] = {0, 0, 0};  // the same in every lane
-            each_top([&](uint32_t t, int) {
+            const auto count = [&](uint32_t t, int) {
 #pragma unroll
                 for (int j = 0; j < 3; ++j)
                     c[j] += __builtin_popcountll(__ballot(t >= (bound | static_cast<uint32_t>(j + 1) << bit)));
-            });
+            };
+            if (few) count(best, 0);
+            else each_top(count);
             u64* sums = s.list + turn * kWaves;
             if (tid % kWave == 0) sums[tid / kWave] = c[0] | static_cast<u64>(c[1]) << 21 | static_cast<u64>(c[2]) << 42;
             __syncthreads();
@@ -524,6 +582,10 @@ __global__ __launch_bounds__(kThreads) void sample_list(SampleArgs a) {
     }
     if (listed) {
         const int n = static_cast<int>(s.n);
+        if (n <= kWave && par.by_k(a)) {
+            if (tid < kWave) short_list(s, a, r, row, par, n);
+            return;
+        }
         sort_list(s, n);
         const Sums sums(s, row, n);
         const u64 held = sums.at(s, n - 1);
@@ -618,44 +680,59 @@ __global__ __launch_bounds__(kThreads) void sample_histogram(SampleArgs a, int64
 
 // ------------------------------------------------------------------ 4. flat rows
 
-// The bin of s in which the running sum (count) reaches goal; what came before it.
-__device__ __forceinline__ int find_bin(Shared& s, bool by_count, u64 goal, u64* mass_before, u64* count_before) {
-    constexpr int kEach = kBins / kThreads;
-    u64 m[kEach], c[kEach], mm = 0, cc = 0, total;
+// The running sums over s's bins, and the bin in which they reach a goal.
+struct BinSums {
+    static constexpr int kEach = kBins / kThreads;
+    u64 m[kEach], c[kEach], m0, c0;  // of this thread's bins, and of those before them
+
+    __device__ __forceinline__ explicit BinSums(Shared& s) {
+        u64 mm = 0, cc = 0, total;
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-        mm += m[j] = s.mass[threadIdx.x * kEach + j];
-        cc += c[j] = s.count[threadIdx.x * kEach + j];
+        for (int j = 0; j < kEach; ++j) {
+            mm += m[j] = s.mass[threadIdx.x * kEach + j];
+            cc += c[j] = s.count[threadIdx.x * kEach + j];
+        }
+        m0 = block_scan(s, mm, &total) - mm;
+        c0 = block_scan(s, cc, &total) - cc;
     }
-    u64 ms = block_scan(s, mm, &total) - mm;
-    u64 cs = block_scan(s, cc, &total) - cc;
-    __syncthreads();
-    if (threadIdx.x == 0) s.found[0] = ~0ull;
-    __syncthreads();
-    int at = -1;
-    u64 mb = 0, cb = 0;
-    int last = -1;  // this thread's last bin that holds anything, should the sums end below the goal
-    u64 lm = 0, lc = 0;
+    // the last bin that holds anything, should the sums end below the goal
+    __device__ __forceinline__ int find(Shared& s, bool by_count, u64 goal, u64* mass_before, u64* count_before) const {
+        __syncthreads();
+        if (threadIdx.x == 0) s.found[0] = ~0ull;
+        __syncthreads();
+        int at = -1, last = -1;
+        u64 ms = m0, cs = c0, mb = 0, cb = 0, lm = 0, lc = 0;
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-        const int i = threadIdx.x * kEach + j;
-        if (at < 0 && c[j] && (by_count ? cs + c[j] : ms + m[j]) >= goal) at = i, mb = ms, cb = cs;
-        if (c[j]) last = i, lm = ms, lc = cs;
-        ms += m[j];
-        cs += c[j];
+        for (int j = 0; j < kEach; ++j) {
+            const int i = threadIdx.x * kEach + j;
+            if (at < 0 && c[j] && (by_count ? cs + c[j] : ms + m[j]) >= goal) at = i, mb = ms, cb = cs;
+            if (c[j]) last = i, lm = ms, lc = cs;
+            ms += m[j];
+            cs += c[j];
+        }
+        if (at >= 0) atomicMin(&s.found[0], static_cast<u64>(at));
+        __syncthreads();
+        u64 first = s.found[0];
+        if (first == ~0ull) {
+            first = block_max(s, static_cast<u64>(last + 1)) - 1;
+            if (last >= 0 && static_cast<u64>(last) == first) at = last, mb = lm, cb = lc;
+        }
+        if (at >= 0 && static_cast<u64>(at) == first) s.found[1] = mb, s.found[2] = cb;
+        __syncthreads();
+        *mass_before = s.found[1];
+        *count_before = s.found[2];
+        return static_cast<int>(first);
     }
-    if (at >= 0) atomicMin(&s.found[0], static_cast<u64>(at));
+};
+
+// The row's histogram by distance into s.
+__device__ __forceinline__ void load_bins(Shared& s, const SampleArgs& a, int64_t r) {
     __syncthreads();
-    u64 first = s.found[0];
-    if (first == ~0ull) {
-        first = block_max(s, static_cast<u64>(last + 1)) - 1;
-        if (last >= 0 && static_cast<u64>(last) == first) at = last, mb = lm, cb = lc;
+    for (int i = threadIdx.x; i < kBins; i += kThreads) {
+        s.mass[i] = a.bin_mass[r * kBins + i];
+        s.count[i] = a.bin_count[r * kBins + i];
     }
-    if (at >= 0 && static_cast<u64>(at) == first) s.found[1] = mb, s.found[2] = cb;
     __syncthreads();
-    *mass_before = s.found[1];
-    *count_before = s.found[2];
-    return static_cast<int>(first);
 }
 
 // At which element does the row's running sum of weights (or count) reach a
@@ -667,14 +744,9 @@ struct Place {
 
 // For goal >= 1, from the histogram by distance.
 __device__ __forceinline__ Place locate(Shared& s, const SampleArgs& a, int64_t r, const Row& row, bool by_count, u64 goal) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += kThreads) {
-        s.mass[i] = a.bin_mass[r * kBins + i];
-        s.count[i] = a.bin_count[r * kBins + i];
-    }
-    __syncthreads();
+    load_bins(s, a, r);
     u64 mass, count;
-    const int b = find_bin(s, by_count, goal, &mass, &count);
+    const int b = BinSums(s).find(s, by_count, goal, &mass, &count);
     uint32_t lo = 0, hi = ~0u;  // keys that are left, both inclusive
     int left = static_cast<int>(s.count[b]);
     const auto in = [&](uint32_t k) { return k >= lo && k <= hi && row.bin(k) == b; };
@@ -696,7 +768,7 @@ __device__ __forceinline__ Place locate(Shared& s, const SampleArgs& a, int64_t 
         __syncthreads();
         u64 m, c;
         const u64 before = by_count ? count : mass;
-        const int d = find_bin(s, by_count, goal > before ? goal - before : 1, &m, &c);
+        const int d = BinSums(s).find(s, by_count, goal > before ? goal - before : 1, &m, &c);
         mass += m;
         count += c;
         left = static_cast<int>(s.count[d]);
@@ -710,7 +782,10 @@ __device__ __forceinline__ Place locate(Shared& s, const SampleArgs& a, int64_t 
         __syncthreads();
         if (threadIdx.x == 0) s.n = 0;
         __syncthreads();
+        float least, most;
+        row.bin_range(b, &least, &most);
         row.each([&](float x, int i) {
+            if (x < least || x > most) return;
             const uint32_t key = key_of(x);
             if (in(key)) append(s, key, i);
         });
@@ -750,22 +825,22 @@ __device__ __forceinline__ Place locate(Shared& s, const SampleArgs& a, int64_t 
 // False if it does not, or they are too many.
 __device__ __forceinline__ bool top_p_and_draw(Shared& s, const SampleArgs& a, int64_t r, const Row& row, u64 goal, float u,
                                                int* index) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += kThreads) {
-        s.mass[i] = a.bin_mass[r * kBins + i];
-        s.count[i] = a.bin_count[r * kBins + i];
-    }
-    __syncthreads();
+    load_bins(s, a, r);
     u64 before_p, before_d, count;
-    const int bp = find_bin(s, false, goal, &before_p, &count);
-    const int bd = find_bin(s, false, draw_goal(u, before_p + 1), &before_d, &count);
-    const int bd_last = find_bin(s, false, draw_goal(u, before_p + s.mass[bp]), &before_d, &count);
+    const BinSums bins(s);
+    const int bp = bins.find(s, false, goal, &before_p, &count);
+    const int bd = bins.find(s, false, draw_goal(u, before_p + 1), &before_d, &count);
+    const int bd_last = bins.find(s, false, draw_goal(u, before_p + s.mass[bp]), &before_d, &count);
     const int nd = static_cast<int>(s.count[bd]), n = nd + (bp == bd ? 0 : static_cast<int>(s.count[bp]));
     if (bd != bd_last || n > kList) return false;
     __syncthreads();
     if (threadIdx.x == 0) s.n = 0;
     __syncthreads();
+    float least, most, unused;
+    row.bin_range(bp, &least, &unused);
+    row.bin_range(bd, &unused, &most);
     row.each([&](float x, int i) {
+        if (x < least || x > most) return;
         const uint32_t key = key_of(x);
         const int b = row.bin(key);
         if (b == bp || b == bd) append(s, key, i);
@@ -814,7 +889,11 @@ __global__ __launch_bounds__(kThreads) void sample_flat(SampleArgs a) {
         const int border = row.bin_of_weight(par.least, par.t);
         u64 v = 0, total;
         for (int i = threadIdx.x; i < border - 1; i += kThreads) v += a.bin_mass[r * kBins + i];
+        float least, most, unused;
+        row.bin_range(border < kBins - 1 ? border + 1 : border, &least, &unused);
+        row.bin_range(border > 0 ? border - 1 : 0, &unused, &most);
         row.each([&](float x, int) {
+            if (x < least || x > most) return;
             const uint32_t key = key_of(x);
             const int b = row.bin(key);
             if (b >= border - 1 && b <= border + 1 && row.weight(key) >= static_cast<double>(par.least)) v += row.units(key);
@@ -881,8 +960,11 @@ extern "C" int fence_sample(int32_t* out, const float* logits, int64_t rows, int
     a.slot_top = reinterpret_cast<uint32_t*>(a.state + rows);
     a.bin_count = a.slot_top + rows * slots;
     const int64_t n4 = (static_cast<int64_t>(vocab) + 3) / 4;
-    // workgroups a row's histogram takes: enough to fill the GPU, none with fewer than 2048 logits
-    int64_t parts = (1024 + rows - 1) / rows, chunk;
+    // Workgroups a row's histogram takes: one for each CU, but four at least, and none with fewer than 2048 logits.
+    // Each adds its bins to the row's by atomics: 32 rows of 128,256 take 14 us in 8 workgroups a row, 22 in 16 and
+    // 34 in 32; 256 rows of 151,936 take 64 us in one a row and 22 in 4.
+    int64_t parts = (256 + rows - 1) / rows, chunk;
+    if (parts < 4) parts = 4;
     if (parts > (n4 + 511) / 512) parts = (n4 + 511) / 512;
     chunk = (n4 + parts - 1) / parts;
     constexpr int64_t kRows = 32768;  // of a launch: grid.y and the lanes of a grid are bounded
