@@ -8,6 +8,10 @@
 // rows once into registers while it takes their maximum, and writes the codes
 // from there.  Rows of one page follow one another, so a workgroup finds its
 // work by itself: it owns the rows of a window at which a page's rows begin.
+// Where these are several short runs, as with single tokens, a wave each
+// takes them: 512 rows of 512 sequences take 8.6 us and 2,048 take 19.4; with
+// the workgroup on one after the other they take 15.8 and 53.
+//
 // The stream is bound by the bytes in and out; a code costs about 15 VALU
 // operations (an exact rounding of the quotient, kv_q8.hpp), which hides
 // behind them.
@@ -94,35 +98,57 @@ __global__ __launch_bounds__(kThreads) void store_q8_kernel(StoreArgs a) {
     const int per_row = hd / 8;  // groups of 8 values a row
     const int64_t first = static_cast<int64_t>(blockIdx.x) * a.window;
     const int64_t last = first + a.window < a.tokens ? first + a.window : a.tokens;
+    // At which rows of the window a page's rows begin, and how many follow as far as a wave sees at once.
+    const int64_t row = first + lane;
+    const int mine = row < a.tokens ? a.slots[row] : -1;
+    const int before = row < a.tokens && row > 0 ? a.slots[row - 1] : -1;
+    const bool there = mine >= 0 && (mine >> a.page_shift) < a.c.n_pages;
+    const bool goes_on = there && (mine & (page_size - 1)) != 0 && before == mine - 1;
+    const uint64_t on = __ballot(goes_on);
+    const uint64_t begin = __ballot(there && !goes_on && row < last);
+    // Rows that follow the one at lane `at`, itself among them, as far as is seen.
+    const auto run_of = [&](int at) {
+        const uint64_t follow = at == kWave - 1 ? 0 : on >> (at + 1);
+        return 1 + __builtin_ctzll(~follow);  // the bits shifted in are 0
+    };
     int turn = 0;  // the two halves of wave_max take turns, so one barrier a page is enough
-    for (int64_t t = first; t < last; ++t) {
-        const int slot = a.slots[t];
-        if (slot < 0 || (slot >> a.page_shift) >= a.c.n_pages) continue;
+
+    // The rows of one page from the one at lane `at` on, n of them as far as was seen: by the whole workgroup, or
+    // by one wave (SOLO).
+    const auto page_rows = [&](int at, int n, auto solo) {
+        constexpr bool SOLO = decltype(solo)::value;
+        constexpr int T = SOLO ? kWave : kThreads;
+        const int me = SOLO ? lane : tid;
+        const int64_t t = first + at;
+        const int slot = __builtin_amdgcn_readlane(mine, at);
         const int off = slot & (page_size - 1);
-        if (off != 0 && t > 0 && a.slots[t - 1] == slot - 1) continue;  // inside a page's rows
-        // how many rows of this page follow
-        int n = 1;
         const int most = static_cast<int>(a.tokens - t < page_size - off ? a.tokens - t : page_size - off);
-        while (n < most) {
-            const int i = n + lane;
-            const uint64_t differ = __ballot(i >= most || a.slots[t + i] != slot + i);
-            const int same = differ ? __builtin_ctzll(differ) : kWave;
-            n += same;
-            if (same < kWave) break;
+        if (at + n == kWave) {  // to the end of what was seen
+            while (n < most) {
+                const int i = n + lane;
+                const uint64_t differ = __ballot(i >= most || a.slots[t + i] != slot + i);
+                const int same = differ ? __builtin_ctzll(differ) : kWave;
+                n += same;
+                if (same < kWave) break;
+            }
         }
+        n = n < most ? n : most;
         const int groups = n * per_row;
         const int64_t at0 = t * a.ld + static_cast<int64_t>(head) * hd;
+        const int64_t page = slot >> a.page_shift;
+        float* scale_at = (is_v ? a.c.v_scale : a.c.k_scale) + page * a.c.n_kv_heads + head;
+        const float old = off ? *scale_at : 0.0f;
         float x[kHeld][8];
         uint32_t m = 0;
 #pragma unroll
         for (int j = 0; j < kHeld; ++j) {
-            const int g = tid + j * kThreads;
+            const int g = me + j * T;
             if (g < groups) load8<IN, VEC>(src, at0 + (g / per_row) * a.ld + (g % per_row) * 8, x[j]);
         }
 #pragma unroll
         for (int j = 0; j < kHeld; ++j)
-            if (tid + j * kThreads < groups) m = max_bits(m, x[j]);
-        for (int g = tid + kHeld * kThreads; g < groups; g += kThreads) {  // a page of more than kHeld groups a lane
+            if (me + j * T < groups) m = max_bits(m, x[j]);
+        for (int g = me + kHeld * T; g < groups; g += T) {  // a page of more than kHeld groups a lane
             float y[8];
             load8<IN, VEC>(src, at0 + (g / per_row) * a.ld + (g % per_row) * 8, y);
             m = max_bits(m, y);
@@ -132,22 +158,21 @@ __global__ __launch_bounds__(kThreads) void store_q8_kernel(StoreArgs a) {
             const uint32_t o = __shfl_xor(m, d);
             m = m > o ? m : o;
         }
-        if (lane == 0) wave_max[turn][wave] = m;
-        const int64_t page = slot >> a.page_shift;
-        float* scale_at = (is_v ? a.c.v_scale : a.c.k_scale) + page * a.c.n_kv_heads + head;
-        const float old = off ? *scale_at : 0.0f;
-        __syncthreads();
+        if constexpr (!SOLO) {
+            if (lane == 0) wave_max[turn][wave] = m;
+            __syncthreads();
 #pragma unroll
-        for (int w = 0; w < kThreads / kWave; ++w) m = m > wave_max[turn][w] ? m : wave_max[turn][w];
-        turn ^= 1;
-        const float mine = __builtin_bit_cast(float, m) / kCodeTop[TYPE];
-        const float scale = old != old || mine != mine ? __builtin_nanf("") : old > mine ? old : mine;
+            for (int w = 0; w < kThreads / kWave; ++w) m = m > wave_max[turn][w] ? m : wave_max[turn][w];
+            turn ^= 1;
+        }
+        const float now = __builtin_bit_cast(float, m) / kCodeTop[TYPE];
+        const float scale = old != old || now != now ? __builtin_nanf("") : old > now ? old : now;
         const float inv = 1.0f / scale;
         uint8_t* codes = static_cast<uint8_t*>(is_v ? a.c.v : a.c.k) +
                          ((page * a.c.n_kv_heads + head) << a.page_shift) * hd;
         if (scale > old && off) {  // what the page held, at the new scale
             const bool finite = scale < __builtin_inff();
-            for (int g = tid; g < off * per_row; g += kThreads) {
+            for (int g = me; g < off * per_row; g += T) {
                 uint2* p = reinterpret_cast<uint2*>(codes + g * 8);
                 uint2 w = *p;
                 // code * old has 31 bits and its quotient by scale no tie that 53 bits could miss
@@ -164,15 +189,32 @@ __global__ __launch_bounds__(kThreads) void store_q8_kernel(StoreArgs a) {
         codes += static_cast<int64_t>(off) * hd;  // rows of a page are contiguous
 #pragma unroll
         for (int j = 0; j < kHeld; ++j) {
-            const int g = tid + j * kThreads;
+            const int g = me + j * T;
             if (g < groups) put8<TYPE>(codes + g * 8, x[j], scale, inv);
         }
-        for (int g = tid + kHeld * kThreads; g < groups; g += kThreads) {
+        for (int g = me + kHeld * T; g < groups; g += T) {
             float y[8];
             load8<IN, VEC>(src, at0 + (g / per_row) * a.ld + (g % per_row) * 8, y);
             put8<TYPE>(codes + g * 8, y, scale, inv);
         }
-        if (tid == 0) *scale_at = scale;
+        if (me == 0) *scale_at = scale;
+    };
+
+    // Several short runs (single tokens, small pages): a wave each.  The choice is the same in every wave.
+    const int run = run_of(lane);
+    const bool any_long = __any((begin >> lane & 1) && (lane + run == kWave || run * per_row > kHeld * kWave));
+    if (__builtin_popcountll(begin) > 1 && !any_long) {
+        int k = 0;
+        for (uint64_t left = begin; left; left &= left - 1, ++k)
+            if (k % (kThreads / kWave) == wave) {
+                const int at = __builtin_ctzll(left);
+                page_rows(at, run_of(at), std::true_type{});
+            }
+    } else {
+        for (uint64_t left = begin; left; left &= left - 1) {
+            const int at = __builtin_ctzll(left);
+            page_rows(at, run_of(at), std::false_type{});
+        }
     }
 }
 
@@ -197,11 +239,12 @@ extern "C" int fence_store_kv_q8(const fence_kv_pages* cache, const void* k, con
         return FENCE_ERROR_INVALID_VALUE;
     if (tokens == 0) return FENCE_SUCCESS;
     const bool vec = aligned(k, 16) && aligned(v, 16) && ld * size % 16 == 0;
-    // Rows a workgroup looks at: one while the grid is small (single tokens, each on a page of its own), more
-    // when most rows only continue a page and their workgroups would start for nothing.
+    // Rows a workgroup looks at, 64 at most, which a wave sees at once: one while the grid is small (single tokens,
+    // each on a page of its own), more when most rows only continue a page and their workgroups would start for
+    // nothing.  8,001 rows of prompts take 18 us on a grid of 2,048 workgroups, 21 on one of 8,192 and 36 on 32,768.
     const int64_t all = tokens * cache->n_kv_heads * 2;
-    int64_t window = all / 8192;
-    window = window < 1 ? 1 : window > cache->page_size ? cache->page_size : window;
+    int64_t window = all / 2048;
+    window = window < 1 ? 1 : window > kWave ? kWave : window;
     const StoreArgs a{*cache, k, v, slots, ld, tokens, static_cast<int>(window), __builtin_ctz(cache->page_size)};
     const dim3 grid(grid_1d(tokens, window), cache->n_kv_heads, 2);
     if (cache->type == FENCE_KV_INT8)
