@@ -10,6 +10,11 @@
 // no atomics decide an order.  The tokens' rows are filled by the same
 // workgroup while they are few (kOneLaunchTokens), else by a second launch
 // over many workgroups.
+//
+// Bound by latency: a scan is two barriers and 64-bit shuffles, a list item
+// the ten LDS reads of its search, so the searches of kAhead items run side
+// by side, without a branch.  64 single tokens take 8.9 us, 384 prompts of
+// 49,152 rows 13.8 us and another 6.8 for the rows.
 #include "common.hpp"
 
 #include <climits>
@@ -19,13 +24,13 @@ namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kBatchChunk = kThreads;  // one sequence per thread
+constexpr int kAhead = 4;              // items whose loads a thread has in flight
 constexpr int kFillThreads = 256;
-constexpr int kFillTokens = 4 * kFillThreads;  // tokens a workgroup of the second launch fills
-constexpr int kFillLds = 4096;                 // row ends the second launch keeps in LDS
-#ifndef FENCE_PLAN_ONE_LAUNCH_TOKENS
-#define FENCE_PLAN_ONE_LAUNCH_TOKENS 8192
-#endif
-constexpr int64_t kOneLaunchTokens = FENCE_PLAN_ONE_LAUNCH_TOKENS;
+constexpr int kFillTokens = kAhead * kFillThreads;  // tokens a workgroup of the second launch fills
+constexpr int kFillLds = 4096;  // row ends the second launch keeps in LDS
+// Rows that one workgroup fills.  64 sequences, back to back: 4,096 rows take 10.9 us so and 14.7 with the second
+// launch, 8,192 take 13.3 and 15.0, 16,384 take 18.0 and 15.0.
+constexpr int64_t kOneLaunchTokens = 8192;
 
 struct PlanArgs {
     int32_t* lens_out;
@@ -56,14 +61,15 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* waves, int64_t
     }
     if (lane == kWave - 1) waves[wave] = v;
     __syncthreads();
-    int64_t before = 0, sum = 0;
+    int64_t sums = waves[lane % (kThreads / kWave)];  // and their sums, in every wave's first lanes
 #pragma unroll
-    for (int w = 0; w < kThreads / kWave; ++w) {
-        if (w < wave) before += waves[w];
-        sum += waves[w];
+    for (int d = 1; d < kThreads / kWave; d *= 2) {
+        const int64_t up = __shfl_up(sums, d);
+        if (lane >= d) sums += up;
     }
-    *total = sum;
-    return before + v;
+    *total = __shfl(sums, kThreads / kWave - 1);
+    const int64_t before = __shfl(sums, wave > 0 ? wave - 1 : 0);
+    return wave > 0 ? before + v : v;
 }
 
 // The first i with ends[i] > at (ends ascending, at < ends[n - 1]).
@@ -75,6 +81,16 @@ __device__ __forceinline__ int holder(const int* ends, int n, int at) {
         else lo = mid + 1;
     }
     return lo;
+}
+
+// The same among N entries, a power of two, in steps without a branch: several
+// searches of a thread run side by side.
+template <int N>
+__device__ __forceinline__ int holder_of(const int* ends, int at) {
+    int i = 0;
+#pragma unroll
+    for (int step = N / 2; step > 0; step /= 2) i += ends[i + step - 1] <= at ? step : 0;
+    return i;
 }
 
 __device__ __forceinline__ int sat32(int64_t v) { return v > INT_MAX ? INT_MAX : static_cast<int>(v); }
@@ -89,14 +105,16 @@ __device__ __forceinline__ void put_row(const PlanArgs& a, int t, int position, 
 }
 
 __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
-    __shared__ int64_t waves[3][kThreads / kWave];
+    __shared__ int64_t waves[2][kThreads / kWave];
     __shared__ int ends[kBatchChunk];    // ends of a flat list's ranges
     __shared__ int begins[kBatchChunk];  // what a range's items are counted from
     __shared__ int bases[kBatchChunk];   // cached tokens (-1 - them if not admitted)
+    __shared__ int last_taken;           // pages needed up to the last sequence that got one
     const int tid = threadIdx.x;
     const int page = 1 << a.page_shift;
     int64_t count = a.free_count[0];
     count = count < 0 ? 0 : count > a.n_pages ? a.n_pages : count;
+    if (tid == 0) last_taken = 0;
 
     // 1. What ended sequences held, onto the stack.
     for (int b0 = 0; b0 < a.batch; b0 += kBatchChunk) {
@@ -115,8 +133,9 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
         ends[tid] = sat32(end);
         begins[tid] = sat32(end - back);
         __syncthreads();
+#pragma unroll 1
         for (int i = tid; i < total; i += kThreads) {
-            const int s = holder(ends, kBatchChunk, i);
+            const int s = holder_of<kBatchChunk>(ends, i);
             a.free_pages[count + i] = a.table[static_cast<int64_t>(b0 + s) * a.max_blocks + (i - begins[s])];
         }
         count += total;
@@ -132,7 +151,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
         const int len = here && a.lens[b] > 0 ? a.lens[b] : 0;
         const bool ended = given < 0;
         const int64_t add = ended ? 0 : given;
-        int64_t new_rows, new_need, new_taken;
+        int64_t new_rows, new_need;
         const int64_t row_end = rows + block_scan(add, waves[0], &new_rows);
         const int64_t held = (static_cast<int64_t>(len) + page - 1) >> a.page_shift;
         const int64_t after = (len + add + page - 1) >> a.page_shift;
@@ -140,22 +159,34 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
         const int64_t need = fits ? after - held : 0;
         const int64_t need_end = upto + block_scan(need, waves[1], &new_need);
         const bool in = fits && (need == 0 || need_end <= count);
-        const int64_t take = in ? need : 0;
-        const int64_t take_end = block_scan(take, waves[2], &new_taken);
-        ends[tid] = static_cast<int>(take_end);  // at most n_pages
-        begins[tid] = static_cast<int>(take_end - take - held);
+        // A sequence gets pages only if all that were needed before it were there, so the pages taken are the
+        // first ones needed, and the n-th of them is the n-th from the top.
+        if (in && need > 0) atomicMax(&last_taken, static_cast<int>(need_end));  // at most n_pages
+        __syncthreads();
+        const int new_taken = last_taken > upto ? static_cast<int>(last_taken - upto) : 0;
+        const int64_t need_here = need_end - upto;
+        ends[tid] = need_here < new_taken ? static_cast<int>(need_here) : new_taken;
+        begins[tid] = sat32(need_here - need - held);
         if (here) {
             a.lens_out[b] = ended ? 0 : in ? static_cast<int>(len + add) : len;
             a.admitted[b] = in || ended;
             a.q_start[b + 1] = sat32(row_end);
         }
         __syncthreads();
-        // A sequence gets pages only if all that were needed before it were there, so the n-th page taken
-        // is the n-th from the top.
-        for (int i = tid; i < new_taken; i += kThreads) {
-            const int s = holder(ends, kBatchChunk, i);
-            a.table[static_cast<int64_t>(b0 + s) * a.max_blocks + (i - begins[s])] =
-                a.free_pages[count - 1 - taken - i];
+#pragma unroll 1
+        for (int i0 = tid; i0 < new_taken; i0 += kAhead * kThreads) {
+            int id[kAhead], s[kAhead];
+#pragma unroll
+            for (int d = 0; d < kAhead; ++d) {
+                const int i = i0 + d * kThreads;
+                id[d] = i < new_taken ? a.free_pages[count - 1 - taken - i] : 0;
+                s[d] = holder_of<kBatchChunk>(ends, i);
+            }
+#pragma unroll
+            for (int d = 0; d < kAhead; ++d) {
+                const int i = i0 + d * kThreads;
+                if (i < new_taken) a.table[static_cast<int64_t>(b0 + s[d]) * a.max_blocks + (i - begins[s[d]])] = id[d];
+            }
         }
         upto += new_need;
         rows += new_rows;
@@ -175,6 +206,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
 
     // 3. The rows, where they are few.
     __syncthreads();
+#pragma unroll 1
     for (int64_t t64 = tid; t64 < a.max_tokens; t64 += kThreads) {
         const int t = static_cast<int>(t64);
         if (t >= rows) {
@@ -182,7 +214,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
             a.slots[t] = -1;
             continue;
         }
-        const int s = holder(ends, kBatchChunk, t);
+        const int s = holder_of<kBatchChunk>(ends, t);
         const bool in = bases[s] >= 0;
         put_row(a, t, (in ? bases[s] : -1 - bases[s]) + (t - begins[s]), in,
                 a.table + static_cast<int64_t>(s) * a.max_blocks);
@@ -194,26 +226,36 @@ __global__ __launch_bounds__(kFillThreads) void plan_fill_kernel(PlanArgs a) {
     __shared__ int lds[kFillLds];
     const bool near = a.batch <= kFillLds;
     if (near) {
-        for (int i = threadIdx.x; i < a.batch; i += kFillThreads) lds[i] = a.q_start[i + 1];
+        for (int i = threadIdx.x; i < kFillLds; i += kFillThreads) lds[i] = i < a.batch ? a.q_start[i + 1] : INT_MAX;
         __syncthreads();
     }
     const int* ends = near ? lds : a.q_start + 1;
     const int rows = ends[a.batch - 1];
-#pragma unroll 1
-    for (int i = 0; i < kFillTokens / kFillThreads; ++i) {
-        const int64_t at = static_cast<int64_t>(blockIdx.x) * kFillTokens + i * kFillThreads + threadIdx.x;
-        if (at >= a.max_tokens) return;
-        const int t = static_cast<int>(at);
-        if (t >= rows) {
-            a.positions[t] = 0;
-            a.slots[t] = -1;
-            continue;
-        }
-        const int s = holder(ends, a.batch, t);
-        const int start = s ? ends[s - 1] : 0;
-        const bool in = a.admitted[s] != 0;  // a sequence with rows has not ended
-        const int before = in ? a.lens_out[s] - (ends[s] - start) : a.lens_out[s];
-        put_row(a, t, before + (t - start), in, a.table + static_cast<int64_t>(s) * a.max_blocks);
+    int t[kAhead], s[kAhead], slot[kAhead], position[kAhead];
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d) {
+        const int64_t at = static_cast<int64_t>(blockIdx.x) * kFillTokens + d * kFillThreads + threadIdx.x;
+        t[d] = at < a.max_tokens ? static_cast<int>(at) : -1;
+        const int within = t[d] >= 0 && t[d] < rows ? t[d] : 0;
+        s[d] = rows > 0 ? near ? holder_of<kFillLds>(ends, within) : holder(ends, a.batch, within) : 0;
+    }
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d) {
+        const int start = s[d] ? ends[s[d] - 1] : 0;
+        const bool in = a.admitted[s[d]] != 0;  // a sequence with rows has not ended
+        const int len = a.lens_out[s[d]];
+        position[d] = (in ? len - (ends[s[d]] - start) : len) + (t[d] - start);
+        slot[d] = in && t[d] >= 0 && t[d] < rows
+                      ? a.table[static_cast<int64_t>(s[d]) * a.max_blocks + (position[d] >> a.page_shift)]
+                      : -1;
+    }
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d) {
+        if (t[d] < 0) continue;
+        const bool row = t[d] < rows;
+        const bool in = row && a.admitted[s[d]] != 0;
+        a.positions[t[d]] = row ? position[d] : 0;
+        a.slots[t[d]] = in ? (slot[d] << a.page_shift) + (position[d] & ((1 << a.page_shift) - 1)) : -1;
     }
 }
 
