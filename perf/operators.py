@@ -191,7 +191,7 @@ def _prepare_store(case, g, seed):
     at = torch.arange(tokens, device="cuda") - (torch.cumsum(_int(news), 0) - _int(news))[seq] + _int(lens)[seq]
     slots = table[seq, at // page] * page + (at % page).to(torch.int32)
     dtype = torch.float32 if case["dtype"] == "f32" else torch.float16
-    row = 3 * h * d if case["fused_rows"] else h * d
+    row = 6 * h * d if case["fused_rows"] else h * d  # four query heads, a K and a V head of each
     # K has a few channels far larger than the others, as trained models do
     size = torch.ones(row, device="cuda")
     size[::37] = 6.0
