@@ -14,7 +14,7 @@
 // Bound by latency: a scan is two barriers and 64-bit shuffles, a list item
 // the ten LDS reads of its search, so the searches of kAhead items run side
 // by side, without a branch.  64 single tokens take 8.9 us, 384 prompts of
-// 49,152 rows 13.8 us and another 6.8 for the rows.
+// 265,152 rows 13.8 us and another 6.8 for the rows.
 #include "common.hpp"
 
 #include <climits>
