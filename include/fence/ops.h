@@ -347,8 +347,8 @@ enum {
 
 /* One layer's cache pages.  Position j of a sequence lives in page
  * block_table[seq][j / page_size] at offset j % page_size; what it holds is
- * code * scale, with one scale per page and kv head (K and V each).
- * page_size 16, 32, 64, 128 or 256; head_dim a multiple of 16 up to 256;
+ * code * scale, with one scale per page and kv head (K and V each), not
+ * negative.  page_size 16, 32, 64, 128 or 256; head_dim a multiple of 16 up to 256;
  * n_pages * page_size <= INT32_MAX; k and v 16-byte aligned. */
 typedef struct {
     void* k;        /* codes [n_pages][n_kv_heads][page_size][head_dim] */
@@ -383,8 +383,10 @@ typedef struct {
  *      so that a step captured at a fixed number of rows can run padded.
  * The entries of block_table behind a sequence's pages, and those of ended
  * sequences, are left as they were.  Released ids that would not fit the
- * stack are dropped.  page_size as in fence_kv_pages; max_blocks *
- * page_size, n_pages * page_size and max_tokens <= INT32_MAX. */
+ * stack are dropped.  What fence_gqa_attention_q8 gives for the rows of a
+ * sequence that was not admitted means nothing.  page_size as in
+ * fence_kv_pages; max_blocks * page_size, n_pages * page_size and max_tokens
+ * <= INT32_MAX. */
 int fence_kv_plan(int32_t* lens_out, const int32_t* lens, const int32_t* new_lens, int batch,
                   int32_t* block_table, int max_blocks, int page_size, int32_t* free_pages,
                   int32_t* free_count_out, const int32_t* free_count, int n_pages, int32_t* q_start,
@@ -420,7 +422,9 @@ int fence_store_kv_q8(const fence_kv_pages* cache, const void* k, const void* v,
  * page_size, and those in pages with an id outside [0, n_pages), count as not
  * there.  scale = 1/sqrt(head_dim); the softmax and all sums are held in
  * fp32.  FENCE_F32 agrees with fp32 arithmetic to fp32 rounding; FENCE_F16
- * rounds the probabilities to binary16.  n_q_heads % n_kv_heads == 0.
+ * rounds the probabilities to binary16.  n_q_heads % n_kv_heads == 0; batch
+ * <= 65535; ldq and ldo <= 2^32; max_blocks * page_size and max_q_len *
+ * n_q_heads / n_kv_heads at least 128 below INT32_MAX.
  * workspace: fence_gqa_attention_q8_workspace(...) bytes, 16-byte aligned;
  * calls that overlap must not share it. */
 int fence_gqa_attention_q8(void* out, const void* q, int type, int64_t ldq, int64_t ldo,
