@@ -424,7 +424,7 @@ int fence_store_kv_q8(const fence_kv_pages* cache, const void* k, const void* v,
  * fp32.  FENCE_F32 agrees with fp32 arithmetic to fp32 rounding; FENCE_F16
  * rounds the probabilities to binary16.  n_q_heads % n_kv_heads == 0; batch
  * <= 65535; ldq and ldo <= 2^32; max_blocks * page_size and max_q_len *
- * n_q_heads / n_kv_heads at least 128 below INT32_MAX.
+ * n_q_heads / n_kv_heads <= INT32_MAX - 1024.
  * workspace: fence_gqa_attention_q8_workspace(...) bytes, 16-byte aligned;
  * calls that overlap must not share it. */
 int fence_gqa_attention_q8(void* out, const void* q, int type, int64_t ldq, int64_t ldo,
