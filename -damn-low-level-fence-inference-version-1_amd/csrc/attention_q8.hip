@@ -29,7 +29,7 @@ constexpr int kCols = 16;           // few_columns; a sequence with no more of t
 constexpr int kUnit = 32 * kWaves;  // positions its workgroup takes at a time
 constexpr int kPromptCols = 32 * kWaves;  // many_columns
 constexpr int64_t kMaxLd = int64_t(1) << 32;  // elements from row to row: times a row's number they fit 63 bits
-constexpr int kAhead = 1024;  // positions past the last that may be looked up: units loaded turns ahead
+constexpr int kBeyond = 1024;  // positions past the last that may be looked up: units loaded turns ahead
 #ifndef FENCE_ATTN_Q8_ITEM
 #define FENCE_ATTN_Q8_ITEM 384
 #endif
@@ -1272,12 +1272,12 @@ extern "C" int fence_gqa_attention_q8(void* out, const void* q, int type, int64_
     if (batch < 0 || batch > 65535 || max_q_len < 0 || max_blocks < 1 || n_q_heads < 1 ||
         n_q_heads % cache->n_kv_heads)
         return FENCE_ERROR_INVALID_VALUE;
-    if (static_cast<int64_t>(max_blocks) * cache->page_size > INT32_MAX - kAhead) return FENCE_ERROR_INVALID_VALUE;
+    if (static_cast<int64_t>(max_blocks) * cache->page_size > INT32_MAX - kBeyond) return FENCE_ERROR_INVALID_VALUE;
     const int64_t width = static_cast<int64_t>(n_q_heads) * cache->head_dim;
     if (ldq < width || ldo < width || ldq > kMaxLd || ldo > kMaxLd)
         return FENCE_ERROR_INVALID_VALUE;
     const int group = n_q_heads / cache->n_kv_heads;
-    if (static_cast<int64_t>(max_q_len) * group > INT32_MAX - kAhead ||
+    if (static_cast<int64_t>(max_q_len) * group > INT32_MAX - kBeyond ||
         (static_cast<int64_t>(max_q_len) * group / kCols + 1) * cache->n_kv_heads > INT32_MAX)
         return FENCE_ERROR_INVALID_VALUE;
     if (workspace_bytes < fence_gqa_attention_q8_workspace(batch, max_q_len, n_q_heads, cache->n_kv_heads,

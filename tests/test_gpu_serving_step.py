@@ -7,7 +7,7 @@ import pytest
 import fence_ops as F
 import serving_ref as R
 from gpu_util import LIVE, dev, host, stream, torch_mod
-from test_gpu_serving import bound, check_attention, empty, pages_of, run_attention
+from test_gpu_serving import HEADS, bound, check_attention, empty, pages_of, run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -331,3 +331,13 @@ def test_attention_rows_at_odd_distances(heads, kvh, d, half, pad):
     """ldq and ldo that leave rows at their type's alignment and no more."""
     rng = np.random.default_rng(pad * 10 + d + half)
     check_attention(rng, heads, kvh, d, 32, [100, 33, 260], [1, 5, 90], R.INT8, half, pad=pad)
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("heads,kvh,d", HEADS)
+def test_attention_drafts(heads, kvh, d, half):
+    """As many drafted tokens as one tile of columns holds, and one more."""
+    rng = np.random.default_rng(heads + 3 * d + half)
+    most = 16 * kvh // heads
+    for q in ([most, 1, most], [most + 1, 1, most]) if most else ([1, 2],):
+        check_attention(rng, heads, kvh, d, 64, [300, 40, 129][:len(q)], q, R.E4M3, half, pad=16)
