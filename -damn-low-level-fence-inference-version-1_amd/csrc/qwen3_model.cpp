@@ -319,7 +319,10 @@ bool Qwen3Model::load(const std::string& gguf_path, int max_ctx, hipStream_t str
     for (size_t n : f32_sizes) total += align_up(n * 4, kAlign);
     total += align_up(half_n * 2, kAlign) + align_up(FF * 2, kAlign) + kAlign;
     total += align_up(size_t(c.n_heads) * FENCE_ARRIVE_WORDS_PER_HEAD * 4, kAlign);
-    if (hipMalloc(&scratch_arena_, total) != hipSuccess || hipHostMalloc(&host_token_, sizeof(int)) != hipSuccess) {
+    const size_t sample_bytes = fence_sample_workspace(1, c.vocab_size);
+    total += align_up(sizeof(SampleRow), kAlign) + align_up(sample_bytes, kAlign);
+    if (hipMalloc(&scratch_arena_, total) != hipSuccess || hipHostMalloc(&host_token_, sizeof(int)) != hipSuccess ||
+        hipHostMalloc(&host_row_, sizeof(SampleRow)) != hipSuccess) {
         unload();
         return fail("out of memory for scratch buffers", FENCE_ERROR_OUT_OF_MEMORY);
     }
@@ -347,6 +350,8 @@ bool Qwen3Model::load(const std::string& gguf_path, int max_ctx, hipStream_t str
     s.argmax_out = reinterpret_cast<int*>(take(sizeof(int)));
     const size_t arrive_bytes = size_t(c.n_heads) * FENCE_ARRIVE_WORDS_PER_HEAD * 4;
     attn_arrive_ = reinterpret_cast<uint32_t*>(take(arrive_bytes));
+    sample_row_ = reinterpret_cast<SampleRow*>(take(sizeof(SampleRow)));
+    sample_ws_ = take(sample_bytes);
     hipError_t e = hipMemsetAsync(kv_arena_, 0, per_cache * 2 * c.n_layers, stream_);
     if (e == hipSuccess) e = hipMemsetAsync(attn_arrive_, 0, arrive_bytes, stream_);
     if (e == hipSuccess) e = hipStreamSynchronize(stream_);
@@ -363,9 +368,12 @@ void Qwen3Model::unload() {
     if (kv_arena_) (void)hipFree(kv_arena_);
     if (scratch_arena_) (void)hipFree(scratch_arena_);
     if (host_token_) (void)hipHostFree(host_token_);
+    if (host_row_) (void)hipHostFree(host_row_);
     if (own_stream_ && stream_) (void)hipStreamDestroy(stream_);
     weight_arena_ = kv_arena_ = scratch_arena_ = nullptr;
     host_token_ = nullptr;
+    host_row_ = sample_row_ = nullptr;
+    sample_ws_ = nullptr;
     attn_arrive_ = nullptr;
     stream_ = nullptr;
     own_stream_ = false;
@@ -504,6 +512,22 @@ int Qwen3Model::sample_greedy(float* logits) {
     return *host_token_;
 }
 
+int Qwen3Model::sample(const float* logits, float temperature, int top_k, float top_p, float min_p, float u) {
+    if (!weight_arena_ || !logits) return fail("no model loaded or no logits", FENCE_ERROR_INVALID_VALUE), -1;
+    if (!(u >= 0.0f && u < 1.0f)) return fail("u outside [0, 1)", FENCE_ERROR_INVALID_VALUE), -1;
+    *host_row_ = {temperature, top_p, min_p, u, top_k};
+    hipError_t e = hipMemcpyAsync(sample_row_, host_row_, sizeof(SampleRow), hipMemcpyHostToDevice, stream_);
+    if (e != hipSuccess) return fail("sending the sampling parameters failed", hip_status(e)), -1;
+    const int st = fence_sample(scratch.argmax_out, logits, 1, config.vocab_size, config.vocab_size,
+                                &sample_row_->temperature, &sample_row_->top_k, &sample_row_->top_p, &sample_row_->min_p,
+                                &sample_row_->u, sample_ws_, fence_sample_workspace(1, config.vocab_size), stream_);
+    if (st != FENCE_SUCCESS) return fail(std::string("sample: ") + fence_status_string(st), st), -1;
+    e = hipMemcpyAsync(host_token_, scratch.argmax_out, sizeof(int), hipMemcpyDeviceToHost, stream_);
+    if (e == hipSuccess) e = hipStreamSynchronize(stream_);
+    if (e != hipSuccess) return fail("reading the token back failed", hip_status(e)), -1;
+    return *host_token_;
+}
+
 // ------------------------------------------------------------------ C ABI
 
 struct fence_model {
@@ -561,6 +585,15 @@ extern "C" int fence_model_forward(fence_model* h, int token_id, int pos, float*
 extern "C" int fence_model_sample_greedy(fence_model* h, const float* logits, int* token) {
     if (!h || !logits || !token) return FENCE_ERROR_INVALID_VALUE;
     const int t = h->m.sample_greedy(const_cast<float*>(logits));
+    if (t < 0) return h->m.last_status();
+    *token = t;
+    return FENCE_SUCCESS;
+}
+
+extern "C" int fence_model_sample(fence_model* h, const float* logits, float temperature, int top_k, float top_p,
+                                  float min_p, float u, int* token) {
+    if (!h || !logits || !token) return FENCE_ERROR_INVALID_VALUE;
+    const int t = h->m.sample(logits, temperature, top_k, top_p, min_p, u);
     if (t < 0) return h->m.last_status();
     *token = t;
     return FENCE_SUCCESS;

@@ -44,6 +44,7 @@ class ModelConfig(ctypes.Structure):
 _P = ctypes.c_void_p
 _S = ctypes.c_char_p
 _I = ctypes.c_int
+_F = ctypes.c_float
 _U32 = ctypes.c_uint32
 _U64 = ctypes.c_uint64
 _SZ = ctypes.c_size_t
@@ -74,6 +75,7 @@ SIGNATURES = {
     "fence_model_set_sequence": ((_P, _I), _I),
     "fence_model_forward": ((_P, _I, _I, _PP), _I),
     "fence_model_sample_greedy": ((_P, _P, ctypes.POINTER(_I)), _I),
+    "fence_model_sample": ((_P, _P, _F, _I, _F, _F, _F, ctypes.POINTER(_I)), _I),
     "fence_model_read_tensor": ((_P, _S, _P, _U64, ctypes.POINTER(_U64)), _I),
     "fence_model_kv_cache": ((_P, _I, _PP, _PP), _I),
     "fence_model_stream": ((_P,), _P),
@@ -271,6 +273,14 @@ class Model:
     def sample_greedy(self, logits: int) -> int:
         t = _I()
         _check("fence_model_sample_greedy", lib().fence_model_sample_greedy(self._h, logits, ctypes.byref(t)))
+        return t.value
+
+    def sample(self, logits: int, u: float, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+               min_p: float = 0.0) -> int:
+        """A token drawn with the random number u in [0, 1), as fence_ops.sample draws it."""
+        t = _I()
+        _check("fence_model_sample", lib().fence_model_sample(self._h, logits, temperature, top_k, top_p, min_p, u,
+                                                              ctypes.byref(t)))
         return t.value
 
     def logits(self, ptr: int):

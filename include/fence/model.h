@@ -62,6 +62,13 @@ int fence_model_forward(fence_model* m, int token_id, int pos, float** logits);
  * [vocab_size] (the first index of the maximum); synchronises the stream. */
 int fence_model_sample_greedy(fence_model* m, const float* logits, int* token);
 
+/* The next token drawn from device logits [vocab_size] with the random number
+ * u in [0, 1) (EINVAL outside it), as fence_sample in ops.h draws it from one
+ * row; synchronises the stream.  It stands in for the reference's host sampler
+ * (sample_nucleus, src/model/qwen3.cu:350-519). */
+int fence_model_sample(fence_model* m, const float* logits, float temperature, int top_k, float top_p,
+                       float min_p, float u, int* token);
+
 /* Copies the device copy of file tensor `name` into host memory (capacity
  * bytes at dst); *bytes = its size.  NOT_FOUND if the model did not load it,
  * EINVAL if capacity is too small.  Synchronous. */

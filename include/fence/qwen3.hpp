@@ -137,6 +137,13 @@ public:
     /* src/model/qwen3.h:134: argmax of device logits [vocab_size]; -1 on error. */
     int sample_greedy(float* logits);
 
+    /* The next token drawn from device logits [vocab_size] with the random
+     * number u in [0, 1), as fence_sample (include/fence/ops.h) draws it;
+     * -1 on error.  In place of the reference's host sampler
+     * (sample_nucleus, src/model/qwen3.cu:350-519): one number comes back
+     * instead of the logits. */
+    int sample(const float* logits, float temperature, int top_k, float top_p, float min_p, float u);
+
     void set_sequence(Qwen3Sequence s) { sequence_ = s; }
     Qwen3Sequence sequence() const { return sequence_; }
     hipStream_t stream() const { return stream_; }
@@ -153,6 +160,13 @@ private:
     void* kv_arena_ = nullptr;
     void* scratch_arena_ = nullptr;
     int* host_token_ = nullptr;  // pinned
+    struct SampleRow {
+        float temperature, top_p, min_p, u;
+        int top_k;
+    };
+    SampleRow* host_row_ = nullptr;    // pinned
+    SampleRow* sample_row_ = nullptr;  // its device copy
+    void* sample_ws_ = nullptr;        // fence_sample's workspace
     uint32_t* attn_arrive_ = nullptr;  // the one-launch attention's counters, zero between calls
     hipStream_t stream_ = nullptr;
     bool own_stream_ = false;

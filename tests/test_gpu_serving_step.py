@@ -341,3 +341,27 @@ def test_attention_drafts(heads, kvh, d, half):
     most = 16 * kvh // heads
     for q in ([most, 1, most], [most + 1, 1, most]) if most else ([1, 2],):
         check_attention(rng, heads, kvh, d, 64, [300, 40, 129][:len(q)], q, R.E4M3, half, pad=16)
+
+
+def test_model_sample(tmp_path):
+    """A model's decode loop with sampled tokens, against the 64-bit form on its logits; u = 0 at temperature 0 is the greedy
+    token; u outside [0, 1) is refused."""
+    import fence_model as M
+    from model_files import write_tiny_qwen3
+    path = str(tmp_path / "tiny.gguf")
+    write_tiny_qwen3(path)
+    rng = np.random.default_rng(6)
+    with M.Model(path, max_ctx=32) as m:
+        tok = 1
+        for pos in range(12):
+            ptr = m.forward(tok, pos)
+            x = m.logits(ptr)
+            t, k, p, mp = [(0.8, 0, 0.9, 0.0), (1.5, 7, 1.0, 0.0), (1.0, 0, 1.0, 0.05), (0.0, 0, 1.0, 0.0)][pos % 4]
+            u = float(np.float32(rng.random()))
+            tok = m.sample(ptr, u, temperature=t, top_k=k, top_p=p, min_p=mp)
+            assert tok == R.sample(x, t, k, np.float32(p), np.float32(mp), u)
+            if t == 0.0:
+                assert tok == m.sample_greedy(ptr)
+        for u in (-0.1, 1.0, float("nan")):
+            with pytest.raises(F.FenceError):
+                m.sample(ptr, u)
