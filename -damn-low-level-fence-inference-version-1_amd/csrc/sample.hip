@@ -329,6 +329,36 @@ __device__ __forceinline__ void append(Shared& s, uint32_t key, int index) {
     if (at < kList) s.list[at] = static_cast<u64>(key) << 32 | static_cast<uint32_t>(~index);
 }
 
+// The value of lane ^ J, in the vector ALU: within rows of 16 lanes by DPP,
+// across them by the swaps of rows.
+template <int J>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+    if constexpr (J == 1) return __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, true);       // quad_perm 1,0,3,2
+    else if constexpr (J == 2) return __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, true);  // quad_perm 2,3,0,1
+    else if constexpr (J == 4)  // the mirror of 8 lanes (^7), then of 4 (^3)
+        return __builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp(v, 0x141, 0xF, 0xF, true), 0x1B, 0xF, 0xF, true);
+    else if constexpr (J == 8) return __builtin_amdgcn_mov_dpp(v, 0x128, 0xF, 0xF, true);  // row_ror:8
+    else return static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), J));
+}
+template <int J>
+__device__ __forceinline__ u64 lane_xor(u64 v) {
+    return static_cast<u64>(lane_xor<J>(static_cast<uint32_t>(v >> 32))) << 32 | lane_xor<J>(static_cast<uint32_t>(v));
+}
+
+// One step of a bitonic network among a wave's lanes and those below it: `falls`: the part of the network that this
+// place is in puts the larger ones first.
+template <int J>
+__device__ __forceinline__ void lane_steps(u64& v, int at, bool falls) {
+    const u64 o = lane_xor<J>(v);
+    v = (o > v) == (((at & J) == 0) == falls) ? o : v;
+    if constexpr (J > 1) lane_steps<J / 2>(v, at, falls);
+}
+template <int K>
+__device__ __forceinline__ void sort_lanes(u64& v, int at) {
+    if constexpr (K > 2) sort_lanes<K / 2>(v, at);
+    lane_steps<K / 2>(v, at, (at & K) == 0);
+}
+
 // The first n entries of the list in falling order: a bitonic network over the
 // next power of two, filled up with zeros, which come last.  Up to one entry a
 // thread the entries stay in registers and only exchanges across waves go
@@ -339,21 +369,18 @@ __device__ __forceinline__ void sort_list(Shared& s, int n) {
     const int tid = threadIdx.x;
     if (size <= kThreads) {
         u64 v = tid < n ? s.list[tid] : 0;
-        for (int k = 2; k <= size; k *= 2)
-            for (int j = k / 2; j > 0; j /= 2) {
-                u64 o;
-                if (j >= kWave) {
-                    __syncthreads();
-                    if (tid < size) s.list[tid] = v;
-                    __syncthreads();
-                    o = tid < size ? s.list[tid ^ j] : 0;
-                } else {
-                    if (tid >= size) continue;
-                    o = __shfl_xor(v, j);
-                }
-                const bool larger = ((tid & j) == 0) == ((tid & k) == 0);  // this place keeps the larger one
-                v = (o > v) == larger ? o : v;
+        if (tid < size) sort_lanes<kWave>(v, tid);
+        for (int k = 2 * kWave; k <= size; k *= 2) {
+            const bool falls = (tid & k) == 0;
+            for (int j = k / 2; j >= kWave; j /= 2) {
+                __syncthreads();
+                if (tid < size) s.list[tid] = v;
+                __syncthreads();
+                const u64 o = tid < size ? s.list[tid ^ j] : 0;
+                v = (o > v) == (((tid & j) == 0) == falls) ? o : v;  // this place keeps the larger or the smaller one
             }
+            if (tid < size) lane_steps<kWave / 2>(v, tid, falls);
+        }
         __syncthreads();
         if (tid < size) s.list[tid] = v;
         __syncthreads();
@@ -376,6 +403,7 @@ __device__ __forceinline__ void sort_list(Shared& s, int n) {
 constexpr int kPer = kList / kThreads;
 struct Sums {
     u64 upto[kPer];  // inclusive
+    u64 before;      // this thread's first
     int per, n;
     __device__ __forceinline__ Sums(Shared& s, const Row& row, int count) : n(count) {
         per = (n + kThreads - 1) / kThreads;
@@ -387,7 +415,7 @@ struct Sums {
             upto[j] = mine;
         }
         u64 total;
-        const u64 before = block_scan(s, mine, &total) - mine;
+        before = block_scan(s, mine, &total) - mine;
 #pragma unroll
         for (int j = 0; j < kPer; ++j) upto[j] += before;
     }
@@ -406,9 +434,9 @@ struct Sums {
         if (threadIdx.x == 0) s.found[0] = n - 1;
         __syncthreads();
 #pragma unroll
-        for (int j = kPer - 1; j >= 0; --j) {
+        for (int j = 0; j < kPer; ++j) {  // one place at most: sums never fall
             const int i = threadIdx.x * per + j;
-            if (j < per && i < n && upto[j] >= goal) atomicMin(&s.found[0], static_cast<u64>(i));
+            if (j < per && i < n && upto[j] >= goal && (j ? upto[j - 1] : before) < goal) s.found[0] = i;
         }
         __syncthreads();
         return static_cast<int>(s.found[0]);
@@ -435,13 +463,7 @@ __device__ __forceinline__ u64 top_p_goal(float p, u64 mass) {
 __device__ __forceinline__ void short_list(Shared& s, const SampleArgs& a, int64_t r, const Row& row, const Params& par, int n) {
     const int lane = threadIdx.x;
     u64 v = lane < n ? s.list[lane] : 0;
-#pragma unroll
-    for (int k = 2; k <= kWave; k *= 2)
-#pragma unroll
-        for (int j = k / 2; j > 0; j /= 2) {
-            const u64 o = __shfl_xor(v, j);
-            v = (o > v) == (((lane & j) == 0) == ((lane & k) == 0)) ? o : v;
-        }
+    sort_lanes<kWave>(v, lane);
     const double w = lane < par.k ? row.weight(static_cast<uint32_t>(v >> 32)) : 0.0;
     u64 upto = static_cast<u64>(rint(w * row.one));
 #pragma unroll
@@ -507,30 +529,44 @@ __global__ __launch_bounds__(kThreads) void sample_list(SampleArgs a) {
     if (par.greedy) {
         bound = top;
     } else if (!all) {
-        // Where that is enough, out of each thread's largest alone: a somewhat lower bound for an eighth of the work.
-        const bool few = 2 * want <= (a.slots < kThreads ? a.slots : kThreads);
-        int turn = 0;  // the two halves of s.list take turns, so one barrier a turn is enough
-        for (int bit = 30; bit >= 16; bit -= 2) {
-            uint32_t c[3] = {0, 0, 0};  // the same in every lane
-            const auto count = [&](uint32_t t, int) {
-#pragma unroll
-                for (int j = 0; j < 3; ++j)
-                    c[j] += __builtin_popcountll(__ballot(t >= (bound | static_cast<uint32_t>(j + 1) << bit)));
-            };
-            if (few) count(best, 0);
-            else each_top(count);
-            u64* sums = s.list + turn * kWaves;
-            if (tid % kWave == 0) sums[tid / kWave] = c[0] | static_cast<u64>(c[1]) << 21 | static_cast<u64>(c[2]) << 42;
+        const auto narrow = [&](auto count) {  // count(bound): how many reach it, the same in every thread
+            for (int bit = 31; bit >= 16; --bit)
+                if (count(bound | 1u << bit) >= want) bound |= 1u << bit;
+        };
+        if (2 * want <= (a.slots < kThreads ? a.slots : kThreads)) {
+            // Out of each thread's largest alone, a somewhat lower bound for a fraction of the work: by one wave, that
+            // keeps all of them in registers and needs no barrier, 2 us where the whole workgroup takes 6.
+            uint32_t* bests = reinterpret_cast<uint32_t*>(s.list);
+            bests[tid] = best;
             __syncthreads();
-            u64 sum = 0;
+            if (tid < kWave) {
+                uint32_t t[kWaves];
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) sum += sums[w];
-            turn ^= 1;
-            for (int j = 2; j >= 0; --j)
-                if (static_cast<int>(sum >> (21 * j) & 0x1FFFFF) >= want) {
-                    bound |= static_cast<uint32_t>(j + 1) << bit;
-                    break;
-                }
+                for (int w = 0; w < kWaves; ++w) t[w] = bests[w * kWave + tid];
+                narrow([&](uint32_t least) {
+                    int n = 0;
+#pragma unroll
+                    for (int w = 0; w < kWaves; ++w) n += __builtin_popcountll(__ballot(t[w] >= least));
+                    return n;
+                });
+                if (tid == 0) s.n = bound;
+            }
+            __syncthreads();
+            bound = s.n;
+        } else {
+            int turn = 0;  // the two halves of s.list take turns, so one barrier a turn is enough
+            narrow([&](uint32_t least) {
+                uint32_t n = 0;  // the same in every lane
+                each_top([&](uint32_t t, int) { n += __builtin_popcountll(__ballot(t >= least)); });
+                u64* sums = s.list + turn * kWaves;
+                if (tid % kWave == 0) sums[tid / kWave] = n;
+                __syncthreads();
+                int sum = 0;
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) sum += static_cast<int>(sums[w]);
+                turn ^= 1;
+                return sum;
+            });
         }
     }
     // The logits above it, out of the threads' that have one; s.mass holds those threads' numbers meanwhile.
@@ -684,44 +720,41 @@ __global__ __launch_bounds__(kThreads) void sample_histogram(SampleArgs a, int64
 struct BinSums {
     static constexpr int kEach = kBins / kThreads;
     u64 m[kEach], c[kEach], m0, c0;  // of this thread's bins, and of those before them
+    u64 masses, counts;              // of all
 
     __device__ __forceinline__ explicit BinSums(Shared& s) {
-        u64 mm = 0, cc = 0, total;
+        u64 mm = 0, cc = 0;
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
             mm += m[j] = s.mass[threadIdx.x * kEach + j];
             cc += c[j] = s.count[threadIdx.x * kEach + j];
         }
-        m0 = block_scan(s, mm, &total) - mm;
-        c0 = block_scan(s, cc, &total) - cc;
+        m0 = block_scan(s, mm, &masses) - mm;
+        c0 = block_scan(s, cc, &counts) - cc;
     }
-    // the last bin that holds anything, should the sums end below the goal
+    // A goal past the last sum counts as the last one.
     __device__ __forceinline__ int find(Shared& s, bool by_count, u64 goal, u64* mass_before, u64* count_before) const {
+        const u64 all = by_count ? counts : masses;
+        goal = goal < all ? goal : all;
+        u64 ms = m0, cs = c0;
         __syncthreads();
-        if (threadIdx.x == 0) s.found[0] = ~0ull;
+        if (threadIdx.x == 0) s.found[0] = s.found[1] = s.found[2] = 0;
         __syncthreads();
-        int at = -1, last = -1;
-        u64 ms = m0, cs = c0, mb = 0, cb = 0, lm = 0, lc = 0;
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
-            const int i = threadIdx.x * kEach + j;
-            if (at < 0 && c[j] && (by_count ? cs + c[j] : ms + m[j]) >= goal) at = i, mb = ms, cb = cs;
-            if (c[j]) last = i, lm = ms, lc = cs;
+            const u64 before = by_count ? cs : ms, here = by_count ? c[j] : m[j];
+            if (before < goal && before + here >= goal) {  // one bin at most: sums never fall
+                s.found[0] = threadIdx.x * kEach + j;
+                s.found[1] = ms;
+                s.found[2] = cs;
+            }
             ms += m[j];
             cs += c[j];
         }
-        if (at >= 0) atomicMin(&s.found[0], static_cast<u64>(at));
-        __syncthreads();
-        u64 first = s.found[0];
-        if (first == ~0ull) {
-            first = block_max(s, static_cast<u64>(last + 1)) - 1;
-            if (last >= 0 && static_cast<u64>(last) == first) at = last, mb = lm, cb = lc;
-        }
-        if (at >= 0 && static_cast<u64>(at) == first) s.found[1] = mb, s.found[2] = cb;
         __syncthreads();
         *mass_before = s.found[1];
         *count_before = s.found[2];
-        return static_cast<int>(first);
+        return static_cast<int>(s.found[0]);
     }
 };
 
