@@ -22,9 +22,17 @@
 //      kListK end here, having read the row once.
 //   3. sample_histogram, for the rows that are left (flat ones): weights and
 //      counts by distance from the maximum.
-//   4. sample_flat, a workgroup a row: from there to one bin for each question;
-//      its elements are listed, or, if they are too many for that as well,
-//      divided by the digits of their keys.
+//   4. sample_flat: the bins in which the borders of the filters and the draw
+//      can lie; their elements are listed by all of a row's workgroups, and
+//      the last to come sorts and answers.  If they are too many for a list,
+//      one workgroup takes one question after the other, to one bin and, where
+//      that is too many as well, by the digits of its elements' keys.
+//
+// Bound by the latency of these steps, not by bytes: one row of 151,936 with
+// top-k 20 takes 2.9 + 10.4 us (scan, list) and 9 of the two launches that
+// find nothing to do; 32 rows of 128,256 with top-p take 8.8 + 22.7 + 13.4 +
+// 32.5 us; 256 rows of 151,936 with mixed filters 35 (4.4 TB/s) + 25.6 + 23 +
+// 42.
 #include "common.hpp"
 
 namespace fence {
@@ -45,6 +53,7 @@ struct RowState {  // from sample_list to the launches behind it
     uint32_t top;  // the maximum's key
     uint32_t flat; // whether anything is left to do
     u64 mass;      // the whole row's weight
+    uint32_t n, arrived;  // sample_flat: what its workgroups have listed, and how many have
 };
 
 struct SampleArgs {
@@ -61,6 +70,7 @@ struct SampleArgs {
     // workspace, per row
     double* slot_mass;    // [slots]
     u64* bin_mass;        // [kBins]
+    u64* list;            // [kList]
     RowState* state;
     uint32_t* slot_top;   // [slots]
     uint32_t* bin_count;  // [kBins]
@@ -203,8 +213,9 @@ struct Shared {
     uint32_t count[kBins];
     u64 list[kList];  // key << 32 | ~index: larger comes first
     double table[kTable];
-    u64 wave[kWaves];
+    u64 wave[kWaves], wave2[kWaves];
     u64 found[4];
+    int bin[8];  // a place for each of the bins that Borders looks for
     uint32_t n;
 };
 
@@ -287,6 +298,29 @@ struct Row {
         return d < static_cast<float>(kBins - 1) ? static_cast<int>(d) : kBins - 1;
     }
 };
+
+// Inclusive sums of two numbers over the workgroup's threads, and their totals.
+__device__ __forceinline__ void block_scan2(Shared& s, u64& v, u64& w, u64* v_total, u64* w_total) {
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+        const u64 v_up = __shfl_up(v, d), w_up = __shfl_up(w, d);
+        if (lane >= d) v += v_up, w += w_up;
+    }
+    __syncthreads();
+    if (lane == kWave - 1) s.wave[wave] = v, s.wave2[wave] = w;
+    __syncthreads();
+    u64 v_before = 0, w_before = 0;
+    *v_total = *w_total = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        if (i < wave) v_before += s.wave[i], w_before += s.wave2[i];
+        *v_total += s.wave[i];
+        *w_total += s.wave2[i];
+    }
+    v += v_before;
+    w += w_before;
+}
 
 // Inclusive sum over the workgroup's threads and its total.
 __device__ __forceinline__ u64 block_scan(Shared& s, u64 v, u64* total) {
@@ -506,7 +540,7 @@ __global__ __launch_bounds__(kThreads) void sample_list(SampleArgs a) {
     };
     each_top([&](uint32_t t, int) { best = t > best ? t : best; });
     const uint32_t top = static_cast<uint32_t>(block_max(s, best));
-    if (tid == 0) a.state[r] = RowState{top, 0, 0};
+    if (tid == 0) a.state[r] = RowState{top, 0, 0, 0, 0};
     if (top <= kKeyLowest) {
         if (tid == 0) a.out[r] = 0;
         return;
@@ -666,7 +700,7 @@ __global__ __launch_bounds__(kThreads) void sample_list(SampleArgs a) {
         }
     }
     // Not here: a histogram, from zero.
-    if (tid == 0) a.state[r] = RowState{top, 1, mass};
+    if (tid == 0) a.state[r] = RowState{top, 1, mass, 0, 0};
     for (int i = tid; i < kBins; i += kThreads) a.bin_mass[r * kBins + i] = 0, a.bin_count[r * kBins + i] = 0;
 }
 
@@ -729,8 +763,21 @@ struct BinSums {
             mm += m[j] = s.mass[threadIdx.x * kEach + j];
             cc += c[j] = s.count[threadIdx.x * kEach + j];
         }
-        m0 = block_scan(s, mm, &masses) - mm;
-        c0 = block_scan(s, cc, &counts) - cc;
+        m0 = mm, c0 = cc;
+        block_scan2(s, m0, c0, &masses, &counts);
+        m0 -= mm, c0 -= cc;
+    }
+    // The bin in which a running sum reaches a goal, in s.bin[slot] behind the next barrier.
+    __device__ __forceinline__ void leave(Shared& s, int slot, bool by_count, u64 goal) const {
+        const u64 all = by_count ? counts : masses;
+        goal = goal < all ? goal : all;
+        u64 before = by_count ? c0 : m0;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+            const u64 here = by_count ? c[j] : m[j];
+            if (before < goal && before + here >= goal) s.bin[slot] = threadIdx.x * kEach + j;  // one bin: sums never fall
+            before += here;
+        }
     }
     // A goal past the last sum counts as the last one.
     __device__ __forceinline__ int find(Shared& s, bool by_count, u64 goal, u64* mass_before, u64* count_before) const {
@@ -853,54 +900,213 @@ __device__ __forceinline__ Place locate(Shared& s, const SampleArgs& a, int64_t 
     return p;
 }
 
-// Top-p and the draw at once: wherever in its bin the border of top-p lies,
-// the draw's goal mostly falls into the same bin, and one pass lists both bins.
-// False if it does not, or they are too many.
-__device__ __forceinline__ bool top_p_and_draw(Shared& s, const SampleArgs& a, int64_t r, const Row& row, u64 goal, float u,
-                                               int* index) {
-    load_bins(s, a, r);
-    u64 before_p, before_d, count;
-    const BinSums bins(s);
-    const int bp = bins.find(s, false, goal, &before_p, &count);
-    const int bd = bins.find(s, false, draw_goal(u, before_p + 1), &before_d, &count);
-    const int bd_last = bins.find(s, false, draw_goal(u, before_p + s.mass[bp]), &before_d, &count);
-    const int nd = static_cast<int>(s.count[bd]), n = nd + (bp == bd ? 0 : static_cast<int>(s.count[bp]));
-    if (bd != bd_last || n > kList) return false;
-    __syncthreads();
-    if (threadIdx.x == 0) s.n = 0;
-    __syncthreads();
-    float least, most, unused;
-    row.bin_range(bp, &least, &unused);
-    row.bin_range(bd, &unused, &most);
-    row.each([&](float x, int i) {
-        if (x < least || x > most) return;
-        const uint32_t key = key_of(x);
-        const int b = row.bin(key);
-        if (b == bp || b == bd) append(s, key, i);
-    });
-    __syncthreads();
-    sort_list(s, n);  // the draw's bin comes first, if they are two
-    const Sums sums(s, row, n);
-    const u64 of_draw = bp == bd ? 0 : sums.at(s, nd - 1);
-    const u64 rest = goal > before_p ? goal - before_p : 1;
-    const int at = sums.reaches(s, rest + of_draw);
-    const u64 kept = before_p + sums.at(s, at) - of_draw;
-    const u64 draw = draw_goal(u, kept);
-    int place = sums.reaches(s, draw > before_d ? draw - before_d : 1);
-    if (place >= nd) place = nd - 1;
-    *index = static_cast<int>(~static_cast<uint32_t>(s.list[place]));
-    return true;
+// A row's answer from one list.  The histogram says in which bins every
+// border can lie: top-k's in one; top-p's in those that its goal falls into
+// for the least and the most weight that top-k may leave; min-p's in three;
+// the draw's in those for the least and the most weight that is left then.
+// These bins' elements are listed, few as a rule, and with the sums of the
+// bins between them every border and the draw come out of one sort.
+struct Borders {
+    static constexpr int kRanges = 4;
+    int from[kRanges], to[kRanges];  // bins, apart from one another and rising; from > to: none
+    int min_from, min_to;            // min-p's, none if it cannot matter
+    u64 mass;                        // what top-k and the others start from
+    bool fits;                       // the list holds all
+
+    // Leaves s.mass and s.count as sums before each bin.
+    __device__ __forceinline__ Borders(Shared& s, const SampleArgs& a, int64_t r, const Row& row, const Params& par,
+                                       u64 row_mass) {
+        load_bins(s, a, r);
+        const BinSums bins(s);
+        mass = par.by_k(a) ? bins.masses : row_mass;  // sample_scan summed nothing then: its list was too long for ties
+        __syncthreads();
+        u64 ms = bins.m0, cs = bins.c0;
+#pragma unroll
+        for (int j = 0; j < BinSums::kEach; ++j) {
+            s.mass[threadIdx.x * BinSums::kEach + j] = ms;
+            s.count[threadIdx.x * BinSums::kEach + j] = static_cast<uint32_t>(cs);
+            ms += bins.m[j];
+            cs += bins.c[j];
+        }
+        __syncthreads();
+        const auto end = [&](int b) { return b == kBins - 1 ? bins.masses : s.mass[b + 1]; };
+        const auto count_end = [&](int b) { return b == kBins - 1 ? bins.counts : s.count[b + 1]; };
+        const u64 slack = (mass >> 28) + 1;  // weights in bins are off by 2^-31 of themselves
+        const auto less = [&](u64 v) { return v > slack ? v - slack : 1; };
+#pragma unroll
+        for (int i = 0; i < kRanges; ++i) from[i] = kBins, to[i] = -1;
+        u64 lo = mass, hi = mass;
+        if (par.k) {
+            bins.leave(s, 0, true, par.k);
+            __syncthreads();
+            from[0] = to[0] = s.bin[0];
+            lo = s.mass[from[0]] + 1, hi = end(to[0]);
+        }
+        if (par.use_p()) {
+            bins.leave(s, 1, false, less(top_p_goal(par.top_p, lo)));
+            bins.leave(s, 2, false, top_p_goal(par.top_p, hi) + slack);
+            __syncthreads();
+            from[1] = s.bin[1], to[1] = s.bin[2];
+            const u64 most = end(to[1]);
+            lo = s.mass[from[1]] + 1 < lo ? s.mass[from[1]] + 1 : lo;
+            hi = most < hi ? most : hi;
+        }
+        min_from = kBins, min_to = -1;
+        if (par.least > 0.0f) {
+            const int border = row.bin_of_weight(par.least, par.t);
+            const int b0 = border > 0 ? border - 1 : 0, b1 = border < kBins - 1 ? border + 1 : border;
+            if (s.mass[b0] < hi + slack) {
+                from[2] = min_from = b0, to[2] = min_to = b1;
+                const u64 before = s.mass[b0] + 1, most = end(b1);
+                lo = before < lo ? before : lo;
+                hi = most < hi ? most : hi;
+            }
+        }
+        bins.leave(s, 3, false, less(draw_goal(par.u, lo)));
+        bins.leave(s, 4, false, draw_goal(par.u, hi) + slack);
+        __syncthreads();
+        from[3] = s.bin[3], to[3] = s.bin[4];
+        // in order, joined where they touch
+#pragma unroll
+        for (int i = 1; i < kRanges; ++i)
+#pragma unroll
+            for (int j = i; j > 0; --j)
+                if (from[j] < from[j - 1]) {
+                    const int f = from[j], t = to[j];
+                    from[j] = from[j - 1], to[j] = to[j - 1];
+                    from[j - 1] = f, to[j - 1] = t;
+                }
+#pragma unroll
+        for (int i = 1; i < kRanges; ++i)
+            if (to[i] >= 0 && from[i] <= to[i - 1] + 1) {
+                from[i] = from[i - 1];
+                to[i] = to[i] > to[i - 1] ? to[i] : to[i - 1];
+                from[i - 1] = kBins, to[i - 1] = -1;
+            }
+        u64 n = 0;
+#pragma unroll
+        for (int i = 0; i < kRanges; ++i)
+            if (to[i] >= 0) n += count_end(to[i]) - s.count[from[i]];
+        fits = n <= kList;
+    }
+    __device__ __forceinline__ bool holds(int b) const {
+        bool in = false;
+#pragma unroll
+        for (int i = 0; i < kRanges; ++i) in = in || (b >= from[i] && b <= to[i]);
+        return in;
+    }
+};
+
+// The answer from the listed elements, n of them in s.list.
+__device__ __forceinline__ int from_borders(Shared& s, const Row& row, const Params& par, const Borders& borders, int n) {
+    sort_list(s, n);
+    // Running sums of weights and numbers, the bins between included.
+    const int per = (n + kThreads - 1) / kThreads;
+    u64 upto[kPer], place[kPer], mine = 0, places = 0, light = 0, total, unused;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        const int i = threadIdx.x * per + j;
+        if (j < per && i < n) {
+            const uint32_t key = static_cast<uint32_t>(s.list[i] >> 32);
+            const int b = row.bin(key), last = i ? row.bin(static_cast<uint32_t>(s.list[i - 1] >> 32)) : -1;
+            const double w = row.weight(key);
+            const u64 units = static_cast<u64>(rint(w * row.one));
+            if (b > last + 1) {  // between the bins: from the end of the one to the start of the other
+                mine += s.mass[b] - s.mass[last + 1];
+                places += s.count[b] - s.count[last + 1];
+            }
+            mine += units;
+            ++places;
+            if (b >= borders.min_from && b <= borders.min_to && w >= static_cast<double>(par.least)) light += units;
+        }
+        upto[j] = mine;
+        place[j] = places;
+    }
+    u64 before = mine, placed = places;
+    block_scan2(s, before, placed, &total, &unused);
+    before -= mine, placed -= places;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) upto[j] += before, place[j] += placed;
+    // the first element whose sum (or place) reaches goal, or the last: its index, and *sum
+    const auto reaches = [&](const u64* sums, u64 first, u64 goal, u64* sum) {
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {  // one at most reaches it first: sums never fall
+            const int i = threadIdx.x * per + j;
+            if (j < per && i < n && (j ? sums[j - 1] : first) < goal && (sums[j] >= goal || i == n - 1))
+                s.found[0] = i, s.found[1] = upto[j];
+        }
+        __syncthreads();
+        *sum = s.found[1];
+        return static_cast<int>(s.found[0]);
+    };
+    u64 kept = borders.mass;
+    if (par.k) reaches(place, placed, par.k, &kept);
+    if (par.use_p()) reaches(upto, before, top_p_goal(par.top_p, kept), &kept);
+    if (borders.min_to >= 0) {
+        block_scan(s, light, &total);
+        total += s.mass[borders.min_from];
+        kept = total < kept ? total : kept;
+    }
+    const int at = reaches(upto, before, draw_goal(par.u, kept), &unused);
+    return static_cast<int>(~static_cast<uint32_t>(s.list[at]));
 }
 
-__global__ __launch_bounds__(kThreads) void sample_flat(SampleArgs a) {
+__global__ __launch_bounds__(kThreads) void sample_flat(SampleArgs a, int64_t chunk) {
     __shared__ Shared s;
-    const int64_t r = blockIdx.x;
+    const int64_t r = blockIdx.y;
     const RowState state = a.state[r];
     if (!state.flat) return;
     const Params par(a, r);
     const Row row(a, r, par.t, state.top);
     fill_table(s.table);
     __syncthreads();
+    {
+        const Borders borders(s, a, r, row, par, state.mass);
+        if (borders.fits) {
+            // A row's workgroups list their parts of it; the last to come answers.
+            if (threadIdx.x == 0) s.n = 0;
+            __syncthreads();
+            const int64_t n4 = (static_cast<int64_t>(row.n) + 3) / 4;
+            const int64_t from = blockIdx.x * chunk, to = from + chunk < n4 ? from + chunk : n4;
+            row.each<kThreads>(from, to, [&](float x, int i) {
+                const uint32_t key = key_of(x);
+                if (borders.holds(row.bin(key))) append(s, key, i);
+            });
+            __syncthreads();
+            int n = s.n < kList ? static_cast<int>(s.n) : kList;  // as the histogram counted them, never more
+            if (gridDim.x > 1) {
+                if (threadIdx.x == 0 && n)
+                    s.found[2] = __hip_atomic_fetch_add(&a.state[r].n, static_cast<uint32_t>(n), __ATOMIC_RELAXED,
+                                                        __HIP_MEMORY_SCOPE_AGENT);
+                __syncthreads();
+                u64* list = a.list + r * kList;
+                for (int i = threadIdx.x; i < n; i += kThreads)
+                    if (s.found[2] + i < kList)
+                        __hip_atomic_store(list + s.found[2] + i, s.list[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                // every wave's stores have completed before the one arrival
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __syncthreads();
+                if (threadIdx.x == 0) {
+                    const uint32_t before = __hip_atomic_fetch_add(&a.state[r].arrived, 1u, __ATOMIC_RELAXED,
+                                                                   __HIP_MEMORY_SCOPE_AGENT);
+                    s.found[3] = before + 1 == gridDim.x;
+                    s.n = __hip_atomic_load(&a.state[r].n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+                __syncthreads();
+                if (!s.found[3]) return;
+                n = s.n < kList ? static_cast<int>(s.n) : kList;
+                for (int i = threadIdx.x; i < n; i += kThreads)
+                    s.list[i] = __hip_atomic_load(list + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __syncthreads();
+            }
+            const int index = from_borders(s, row, par, borders, n);
+            if (threadIdx.x == 0) a.out[r] = index;
+            return;
+        }
+    }
+    // Lists too long for that: one question after the other, by one workgroup.
+    if (blockIdx.x) return;
     u64 kept = state.mass;
     if (par.by_k(a)) {  // sample_scan summed nothing: its list was too long for ties
         u64 v = 0;
@@ -910,11 +1116,6 @@ __global__ __launch_bounds__(kThreads) void sample_flat(SampleArgs a) {
     if (par.k) kept = locate(s, a, r, row, true, par.k).mass;
     if (par.use_p()) {
         const u64 goal = top_p_goal(par.top_p, kept);
-        int index;
-        if (!(par.least > 0.0f) && top_p_and_draw(s, a, r, row, goal, par.u, &index)) {
-            if (threadIdx.x == 0) a.out[r] = index;
-            return;
-        }
         kept = locate(s, a, r, row, false, goal).mass;
     }
     if (par.least > 0.0f) {
@@ -958,7 +1159,8 @@ int slots_of(int64_t rows, int vocab) {
 
 int64_t row_bytes(int slots) {
     return slots * static_cast<int64_t>(sizeof(double) + sizeof(uint32_t)) +
-           kBins * static_cast<int64_t>(sizeof(u64) + sizeof(uint32_t)) + static_cast<int64_t>(sizeof(RowState));
+           kBins * static_cast<int64_t>(sizeof(u64) + sizeof(uint32_t)) + kList * static_cast<int64_t>(sizeof(u64)) +
+           static_cast<int64_t>(sizeof(RowState));
 }
 
 }  // namespace
@@ -986,16 +1188,18 @@ extern "C" int fence_sample(int32_t* out, const float* logits, int64_t rows, int
     if (rows == 0) return FENCE_SUCCESS;
     const int slots = slots_of(rows, vocab), width = scan_width(rows, vocab);
     SampleArgs a{out, logits, ld, vocab, shift_for(vocab), slots, temperature, top_k, top_p, min_p, u,
-                 nullptr, nullptr, nullptr, nullptr, nullptr};
+                 nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
     a.slot_mass = static_cast<double*>(workspace);
     a.bin_mass = reinterpret_cast<u64*>(a.slot_mass + rows * slots);
-    a.state = reinterpret_cast<RowState*>(a.bin_mass + rows * kBins);
+    a.list = a.bin_mass + rows * kBins;
+    a.state = reinterpret_cast<RowState*>(a.list + rows * kList);
     a.slot_top = reinterpret_cast<uint32_t*>(a.state + rows);
     a.bin_count = a.slot_top + rows * slots;
     const int64_t n4 = (static_cast<int64_t>(vocab) + 3) / 4;
-    // Workgroups a row's histogram takes: one for each CU, but four at least, and none with fewer than 2048 logits.
-    // Each adds its bins to the row's by atomics: 32 rows of 128,256 take 14 us in 8 workgroups a row, 22 in 16 and
-    // 34 in 32; 256 rows of 151,936 take 64 us in one a row and 22 in 4.
+    // Workgroups that share a flat row: one for each CU, but four at least, and none with fewer than 2048 logits.
+    // Each adds its bins to the row's by atomics: the histograms of 32 rows of 128,256 take 14 us in 8 workgroups a
+    // row, 22 in 16 and 34 in 32; those of 256 rows of 151,936 take 64 us in one a row and 22 in 4.  Listing, they
+    // all begin with the whole histogram: 38 us in 8 a row and 62 in 32; 83 us in one a row, 60 in 2 and 47 in 4.
     int64_t parts = (256 + rows - 1) / rows, chunk;
     if (parts < 4) parts = 4;
     if (parts > (n4 + 511) / 512) parts = (n4 + 511) / 512;
@@ -1013,6 +1217,7 @@ extern "C" int fence_sample(int32_t* out, const float* logits, int64_t rows, int
         p.u += r0;
         p.slot_mass += r0 * slots;
         p.bin_mass += r0 * kBins;
+        p.list += r0 * kList;
         p.state += r0;
         p.slot_top += r0 * slots;
         p.bin_count += r0 * kBins;
@@ -1025,7 +1230,7 @@ extern "C" int fence_sample(int32_t* out, const float* logits, int64_t rows, int
         if (st) return st;
         if ((st = launch(sample_histogram, dim3(static_cast<unsigned>(parts), m), dim3(kThreads), 0, stream, p, chunk)))
             return st;
-        if ((st = launch(sample_flat, dim3(m), dim3(kThreads), 0, stream, p))) return st;
+        if ((st = launch(sample_flat, dim3(static_cast<unsigned>(parts), m), dim3(kThreads), 0, stream, p, chunk))) return st;
     }
     return FENCE_SUCCESS;
 }

@@ -498,3 +498,18 @@ def test_sample_distribution():
     p = np.exp(x[0].astype(np.float64))
     p /= p.sum()
     assert (np.abs(got - 20000 * p) <= 5 * np.sqrt(20000 * p * (1 - p))).all()
+
+
+def test_sample_many_flat_rows():
+    """Rows that need the whole histogram, more than one workgroup each, beside peaked ones; every filter and none."""
+    rng = np.random.default_rng(77)
+    rows, vocab = 300, 20011
+    x = logits(rng, rows, vocab, [0.3, 1.0, 2.0, 5.0])
+    t = rng.uniform(0.5, 2.0, rows).astype(np.float32)
+    t[::17] = 0
+    k = np.where(rng.random(rows) < 0.4, rng.integers(1, vocab, rows), 0).astype(np.int32)
+    p = np.where(rng.random(rows) < 0.6, rng.uniform(0.2, 1.0, rows), 1.0).astype(np.float32)
+    m = np.where(rng.random(rows) < 0.4, 10.0 ** rng.uniform(-4, 0, rows), 0.0).astype(np.float32)
+    u = rng.random(rows).astype(np.float32)
+    u[::13], u[5::13] = 0.0, np.float32(1 - 2.0 ** -24)
+    check_sample(x, t, k, p, m, u)
