@@ -43,6 +43,14 @@ constexpr int kGrid = FENCE_ATTN_Q8_GRID;
 #endif
 constexpr int kBigGrid = FENCE_ATTN_Q8_BIG_GRID;
 
+// Where a workgroup begins, as it leaves it for the join.
+struct Border {
+    int64_t item, cost, total;  // where the item begins in the work, what it costs, and all work
+    int seq, tile, head, unit, units;
+    int grid;  // workgroups that share the work; 0: nothing to do for this one
+};
+static_assert(sizeof(Border) == 48);
+
 struct Q8Args {
     void* out;
     const void* q;
@@ -55,6 +63,7 @@ struct Q8Args {
     const int32_t* kv_lens;
     const int32_t* q_start;
     float* ws;
+    Border* borders;  // in the workspace, one for each workgroup
     int n_pages, page_shift, n_kv_heads, head_dim, group;
     int max_blocks, batch, max_q_len;
     int part_cols;  // columns of a part in the workspace
@@ -284,9 +293,14 @@ struct Share {
                 if (i == 0) return cut(me, n, g);
                 to_end = me + 1 == g;
                 return to_end ? n - 1 : cut(me + 1, n, g);
-            }))
+            })) {
+            if (threadIdx.x == 0) a.borders[me].grid = 0;
             return false;
+        }
         p = ends[0];
+        if (threadIdx.x == 0)
+            a.borders[me] = Border{p.item, p.cost, total, p.seq, p.tile, p.head, p.unit, p.units, grid};
+        __builtin_amdgcn_sched_barrier(0);  // or its values stay in registers that the products then lack
         end_seq = ends[1].seq;
         end_tile = ends[1].tile;
         end_head = ends[1].head;
@@ -1104,84 +1118,110 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void mixed_q8_kernel(Q
     else few_columns<TYPE, QT, HD>(few, reinterpret_cast<float*>(buf), wg - many_grid, gridDim.x - many_grid);
 }
 
+// Workgroups that join an item of many columns.  24 sequences of 35 columns take 9.2 us with 4, 13.6 with 2 and 10.4
+// with 8; 3,000 rows in six prompts 18.0, 23.2 and 16.4 us; a prompt of 8,192 rows 19.9, 18.5 and 20.1.
+constexpr int kJoinWide = 4;
+
 // Joins the parts of the items that more than one workgroup took, in workgroup
 // order.  Workgroup x looks at the border between workgroups x and x + 1 of
 // the other kernel: if it is the first border inside an item, the item's
 // columns are its to join, together with the other workgroups of the same x,
 // a run of 4 dimensions a thread.
 template <int QT, int HD, class KIND>
-__device__ __forceinline__ void join_at(const Q8Args& a, int w0, int grid) {
-    int64_t total;
-    Place p[1];
-    if (!find<KIND, 1>(a, &grid, &total, p, [&](int, int64_t n, int g) -> int64_t {
-            return w0 + 1 < g ? cut(w0 + 1, n, g) : -1;
-        }))
-        return;
-    if (p[0].unit == 0) return;
-    const int64_t off0 = cut(w0, total, grid) - p[0].item;  // the border before
-    if (off0 > 0 && (KIND::MANY ? quotient(off0 * p[0].units, p[0].cost) : off0) > 0) return;
+__device__ __forceinline__ void join_at(const Q8Args& a, int w0, int y, int ys) {
+    struct Raw {
+        u4 w[sizeof(Border) / 16];
+    } raw;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(Border) / 16); ++i)
+        raw.w[i] = uniform_load(reinterpret_cast<const u4*>(a.borders + w0 + 1), i);
+    const Border p = __builtin_bit_cast(Border, raw);
+    const int grid = p.grid;
+    const int64_t total = p.total;
+    if (grid == 0 || p.unit == 0) return;
+    const int64_t off0 = cut(w0, total, grid) - p.item;  // the border before
+    if (off0 > 0 && (KIND::MANY ? quotient(off0 * p.units, p.cost) : off0) > 0) return;
     // the workgroup whose share holds the item's end
-    const int64_t end = p[0].item + p[0].cost;
+    const int64_t end = p.item + p.cost;
     int w_end = static_cast<int>(quotient(end * grid - 1, total));
     while (w_end + 1 < grid && cut(w_end + 1, total, grid) < end) ++w_end;
     while (w_end > w0 + 1 && cut(w_end, total, grid) >= end) --w_end;
     w_end = __builtin_amdgcn_readfirstlane(w_end);
-    const Seq<KIND> s = Seq<KIND>::uniform(a, p[0].seq);
-    const int col0 = p[0].tile * Seq<KIND>::COLS;
+    const Seq<KIND> s = Seq<KIND>::uniform(a, p.seq);
+    const int col0 = p.tile * Seq<KIND>::COLS;
     const int left = s.rows * a.group - col0;
     const int cols = left < Seq<KIND>::COLS ? left : Seq<KIND>::COLS;
     const int hd = a.head_dim;
-    constexpr int AHEAD = 8;  // parts whose loads are in flight together
-    for (int x = blockIdx.y * kThreads + threadIdx.x; x < cols * (HD / 4); x += gridDim.y * kThreads) {
-        const int c = x / (HD / 4), d = x % (HD / 4) * 4;
-        float top = -__builtin_inff(), sum = 0.0f;
-        f4 val = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int w = w0; w <= w_end; w += AHEAD) {
-            float m[AHEAD], l[AHEAD];
-            f4 v[AHEAD];
+    const int step = ys * kThreads, all = cols * (HD / 4);
+    // RUNS runs of this thread at once and AHEAD parts of each, whose loads are in flight together.
+    const auto join = [&](auto runs, auto ahead) {
+        constexpr int RUNS = decltype(runs)::value, AHEAD = decltype(ahead)::value;
+        for (int x0 = y * kThreads + threadIdx.x; x0 < all; x0 += RUNS * step) {
+            float top[RUNS], sum[RUNS];
+            f4 val[RUNS];
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) {
-                const int ww = w + i <= w_end ? w + i : w_end;
-                float* part = part_at(a, ww, ww == w0, HD);
-                const float* ml = part_sums(a, part, HD) + 2 * c;
-                m[i] = ml[0];
-                l[i] = ml[1];
-                v[i] = *reinterpret_cast<const f4*>(part + c * HD + d);
-            }
-            float most = top;
+            for (int r = 0; r < RUNS; ++r) top[r] = -__builtin_inff(), sum[r] = 0.0f, val[r] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int w = w0; w <= w_end; w += AHEAD) {
+                float m[RUNS][AHEAD], l[RUNS][AHEAD];
+                f4 v[RUNS][AHEAD];
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) most = fmaxf(most, m[i]);
-            const float ref = most == -__builtin_inff() ? 0.0f : most;
-            const float f0 = __builtin_amdgcn_exp2f(top - ref);
-            sum *= f0;
-            val *= f0;
+                for (int r = 0; r < RUNS; ++r) {
+                    const int x = x0 + r * step < all ? x0 + r * step : x0;
+                    const int c = x / (HD / 4), d = x % (HD / 4) * 4;
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) {
-                // a sum of 0: nothing seen, or a share without units, which leaves no output
-                if (w + i <= w_end && l[i] != 0.0f) {
-                    const float f = __builtin_amdgcn_exp2f(m[i] - ref);
-                    sum += f * l[i];
-                    val += v[i] * f;
+                    for (int i = 0; i < AHEAD; ++i) {
+                        const int ww = w + i <= w_end ? w + i : w_end;
+                        float* part = part_at(a, ww, ww == w0, HD);
+                        const float* ml = part_sums(a, part, HD) + 2 * c;
+                        m[r][i] = ml[0];
+                        l[r][i] = ml[1];
+                        v[r][i] = *reinterpret_cast<const f4*>(part + c * HD + d);
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < RUNS; ++r) {
+                    float most = top[r];
+#pragma unroll
+                    for (int i = 0; i < AHEAD; ++i) most = fmaxf(most, m[r][i]);
+                    const float ref = most == -__builtin_inff() ? 0.0f : most;
+                    const float f0 = __builtin_amdgcn_exp2f(top[r] - ref);
+                    sum[r] *= f0;
+                    val[r] *= f0;
+#pragma unroll
+                    for (int i = 0; i < AHEAD; ++i) {
+                        // a sum of 0: nothing seen, or a share without units, which leaves no output
+                        if (w + i <= w_end && l[r][i] != 0.0f) {
+                            const float f = __builtin_amdgcn_exp2f(m[r][i] - ref);
+                            sum[r] += f * l[r][i];
+                            val[r] += v[r][i] * f;
+                        }
+                    }
+                    top[r] = most;
                 }
             }
-            top = most;
-        }
-        if (d < hd) {
-            const int cc = col0 + c;
-            const int64_t to = static_cast<int64_t>(s.row0 + cc / a.group) * a.ldo +
-                               static_cast<int64_t>(p[0].head * a.group + cc % a.group) * hd + d;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) put<QT>(a.out, to + i, sum != 0.0f ? val[i] / sum : 0.0f);
+            for (int r = 0; r < RUNS; ++r) {
+                const int x = x0 + r * step, d = x % (HD / 4) * 4;
+                if (x >= all || d >= hd) continue;
+                const int cc = col0 + x / (HD / 4);
+                const int64_t to = static_cast<int64_t>(s.row0 + cc / a.group) * a.ldo +
+                                   static_cast<int64_t>(p.head * a.group + cc % a.group) * hd + d;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) put<QT>(a.out, to + i, sum[r] != 0.0f ? val[r][i] / sum[r] : 0.0f);
+            }
         }
-    }
+    };
+    const int parts = w_end - w0 + 1;
+    if (parts <= 2) join(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{});
+    else join(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
 }
 
 // The borders of both kernels in one launch: first those of the prompts.
 template <int QT, int HD>
-__global__ __launch_bounds__(kThreads) void join_q8_kernel(Q8Args many, int many_grid, Q8Args few, int few_grid) {
-    const int border = blockIdx.x;
-    if (border < many_grid - 1) join_at<QT, HD, Prompt>(many, border, many_grid);
-    else join_at<QT, HD, Few>(few, border - (many_grid > 1 ? many_grid - 1 : 0), few_grid);
+__global__ __launch_bounds__(kThreads) void join_q8_kernel(Q8Args many, int many_grid, Q8Args few) {
+    const int of_many = many_grid > 1 ? (many_grid - 1) * kJoinWide : 0, x = blockIdx.x;
+    if (x < of_many) join_at<QT, HD, Prompt>(many, x / kJoinWide, x % kJoinWide, kJoinWide);
+    else join_at<QT, HD, Few>(few, x - of_many, 0, 1);
 }
 
 int padded(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
@@ -1211,6 +1251,9 @@ int attention_launch(const Q8Args& a, hipStream_t s) {
     const int64_t columns = static_cast<int64_t>(a.max_q_len) * a.group;
     const int64_t positions = static_cast<int64_t>(a.max_blocks) << a.page_shift;
     Q8Args many = a, few = a;
+    few.borders = reinterpret_cast<Border*>(a.ws);
+    many.borders = few.borders + kGrid;
+    many.ws = few.ws = reinterpret_cast<float*>(many.borders + kBigGrid);
     few.part_cols = part_cols(a.max_q_len, a.group, false);
     const unsigned few_grid = grid_for(1, a.n_kv_heads, positions, kUnit, a.batch, kGrid);
     unsigned many_grid = 0;
@@ -1227,10 +1270,9 @@ int attention_launch(const Q8Args& a, hipStream_t s) {
         if (const int st = launch(attention_q8_kernel<TYPE, QT, HD>, dim3(few_grid), dim3(kThreads), shmem, s, few))
             return st;
     }
-    const unsigned borders = (many_grid > 1 ? many_grid - 1 : 0) + few_grid - 1;
+    const unsigned borders = (many_grid > 1 ? (many_grid - 1) * kJoinWide : 0) + few_grid - 1;
     if (borders == 0) return FENCE_SUCCESS;
-    return launch(join_q8_kernel<QT, HD>, dim3(borders, many_grid > 1 ? 2 : 1), dim3(kThreads), 0, s, many,
-                  static_cast<int>(many_grid), few, static_cast<int>(few_grid));
+    return launch(join_q8_kernel<QT, HD>, dim3(borders), dim3(kThreads), 0, s, many, static_cast<int>(many_grid), few);
 }
 
 template <int TYPE, int QT>
@@ -1252,7 +1294,7 @@ extern "C" int64_t fence_gqa_attention_q8_workspace(int batch, int max_q_len, in
         head_dim > 256 || head_dim % 16)
         return 0;
     const int group = n_q_heads / n_kv_heads;
-    int64_t bytes = 4 * part_floats(max_q_len, group, head_dim, false);
+    int64_t bytes = 4 * part_floats(max_q_len, group, head_dim, false) + (kGrid + kBigGrid) * int64_t(sizeof(Border));
     if (big(max_q_len, group)) bytes += 4 * part_floats(max_q_len, group, head_dim, true);
     return bytes < 16 ? 16 : bytes;
 }
@@ -1286,7 +1328,7 @@ extern "C" int fence_gqa_attention_q8(void* out, const void* q, int type, int64_
     if (batch == 0 || max_q_len == 0) return FENCE_SUCCESS;
     const float scale = 1.0f / sqrtf(static_cast<float>(cache->head_dim));
     const Q8Args a{out, q, ldq, ldo, static_cast<const uint8_t*>(cache->k), static_cast<const uint8_t*>(cache->v),
-                   cache->k_scale, cache->v_scale, block_table, kv_lens, q_start, static_cast<float*>(workspace),
+                   cache->k_scale, cache->v_scale, block_table, kv_lens, q_start, static_cast<float*>(workspace), nullptr,
                    cache->n_pages, __builtin_ctz(cache->page_size), cache->n_kv_heads, cache->head_dim, group,
                    max_blocks, batch, max_q_len, 0,
                    static_cast<float>(scale * 1.4426950408889634), aligned(out, 16) && ldo * size % 16 == 0};
