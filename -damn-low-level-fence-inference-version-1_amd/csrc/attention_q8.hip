@@ -883,30 +883,35 @@ __device__ __forceinline__ void many_columns(const Q8Args& a, h8* buf, int me, i
         {
             const int64_t from = mine ? static_cast<int64_t>(s.row0 + row) * a.ldq + static_cast<int64_t>(qhead) * hd : 0;
             if constexpr (F32) {
-                float biggest = 0.0f;
+                float x[KS][8], biggest = 0.0f;
 #pragma unroll
-                for (int k = 0; k < KS; ++k)
+                for (int k = 0; k < KS; ++k) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[k][i] = 0.0f;
                     if (mine && k * 16 < hd) {
                         const float* src = static_cast<const float*>(a.q) + from + k * 16 + g * 8;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) biggest = fmaxf(biggest, fabsf(src[i]));
+                        for (int i = 0; i < 8; ++i) x[k][i] = src[i];
                     }
+                }
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) biggest = fmaxf(biggest, fabsf(x[k][i]));
                 biggest = fmaxf(biggest, __shfl_xor(biggest, 32));
                 uint32_t e = __builtin_bit_cast(uint32_t, biggest) >> 23;
                 e = e < 15 ? 15 : e > 254 ? 254 : e;
                 const float up = __builtin_bit_cast(float, (268 - e) << 23);
                 unscale *= __builtin_bit_cast(float, (e - 14) << 23);
 #pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    const float* src = static_cast<const float*>(a.q) + from + k * 16 + g * 8;
+                for (int k = 0; k < KS; ++k)
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         _Float16 hi, lo;
-                        split(mine && k * 16 < hd ? src[i] * up : 0.0f, &hi, &lo);
+                        split(x[k][i] * up, &hi, &lo);
                         qf[0][k][i] = hi;
                         qf[1][k][i] = lo;
                     }
-                }
             } else {
 #pragma unroll
                 for (int k = 0; k < KS; ++k) {
