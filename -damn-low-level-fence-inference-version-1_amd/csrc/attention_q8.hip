@@ -30,13 +30,14 @@ constexpr int kUnit = 32 * kWaves;  // positions its workgroup takes at a time
 constexpr int kPromptCols = 32 * kWaves;  // many_columns
 constexpr int64_t kMaxLd = int64_t(1) << 32;  // elements from row to row: times a row's number they fit 63 bits
 constexpr int kBeyond = 1024;  // positions past the last that may be looked up: units loaded turns ahead
-// What an item of many columns costs besides its positions, in positions.  Six prompt chunks of 500 rows in fp32 take
-// 161 us with 384, 183 with 192 and 164 with 768; one prompt of 8,192 rows 828, 823 and 840.
+// What an item of many columns costs besides its positions, in positions.  One prompt of 8,192 rows takes
+// 730 us with 384, 736 with 192 and 747 with 128; six prompt chunks of 500 rows in fp32 130, 126 and 130.
 constexpr int kBigItem = 384;
 // Workgroups that share the work: with few columns four a CU (64 single tokens at up to 32k positions take 307 us, 302
 // with two a CU and 320 with eight), with many the two that fit (a prompt of 8,192 rows: 828 us, with one 1,140).
 constexpr int kGrid = 1024;
 constexpr int kBigGrid = 512;
+constexpr int kXcds = 8;
 
 // Where a workgroup begins, as it leaves it for the join.
 struct Border {
@@ -171,7 +172,7 @@ __device__ __forceinline__ int sharers(int64_t total, int grid) {
 // Where workgroup w begins, when `grid` of them share `total`.
 __device__ __forceinline__ int64_t cut(int w, int64_t total, int grid) { return quotient(w * total, grid); }
 
-// A place in the work, in the order of sequences, tiles, kv heads and units.
+// A place in the work, in the order of sequences, kv heads, tiles and units.
 // An item is a sequence's tile of one kv head.
 struct Place {
     int seq, tile, head, unit, units;
@@ -252,18 +253,19 @@ __device__ __forceinline__ bool find(const Q8Args& a, int* grid, int64_t* total,
         p[i].seq = __builtin_amdgcn_readfirstlane(p[i].seq);
         const Seq<KIND> s = Seq<KIND>::uniform(a, p[i].seq);
         const int64_t rest = point[i] - uniform64(before[i]);
+        const int64_t per_head = s.before(s.tiles());
+        p[i].head = __builtin_amdgcn_readfirstlane(static_cast<int>(quotient(rest, per_head)));
+        const int64_t in_head = rest - p[i].head * per_head;
         int lo = 0, hi = s.tiles() - 1;  // the last tile that begins at or before it
         while (lo < hi) {
             const int mid = (lo + hi + 1) / 2;
-            if (s.before(mid) * a.n_kv_heads <= rest) lo = mid;
+            if (s.before(mid) <= in_head) lo = mid;
             else hi = mid - 1;
         }
         p[i].tile = __builtin_amdgcn_readfirstlane(lo);
         p[i].units = s.units(p[i].tile);
         p[i].cost = s.cost(p[i].tile);
-        const int64_t in_tile = rest - s.before(p[i].tile) * a.n_kv_heads;
-        p[i].head = __builtin_amdgcn_readfirstlane(static_cast<int>(quotient(in_tile, p[i].cost)));
-        const int64_t off = in_tile - p[i].head * p[i].cost;
+        const int64_t off = in_head - s.before(p[i].tile);
         p[i].item = point[i] - off;
         const int unit = KIND::MANY ? static_cast<int>(quotient(off * p[i].units, p[i].cost)) : static_cast<int>(off);
         p[i].unit = __builtin_amdgcn_readfirstlane(unit);
@@ -311,13 +313,14 @@ struct Share {
     __device__ __forceinline__ bool next(const Q8Args& a) {
         if (in_last()) return false;
         p.unit = 0;
-        if (++p.head < a.n_kv_heads) return true;
-        p.head = 0;
         Seq<KIND> s = Seq<KIND>::uniform(a, p.seq);
         if (++p.tile == s.tiles()) {
             p.tile = 0;
-            do s = Seq<KIND>::uniform(a, ++p.seq);
-            while (s.rows == 0);  // the end lies in a sequence behind
+            if (++p.head == a.n_kv_heads) {
+                p.head = 0;
+                do s = Seq<KIND>::uniform(a, ++p.seq);
+                while (s.rows == 0);  // the end lies in a sequence behind
+            }
         }
         p.units = s.units(p.tile);
         return true;
@@ -722,15 +725,21 @@ __device__ __forceinline__ void few_columns(const Q8Args& a, float* lds, int me,
 // conversions and LDS reads, but take all registers of a SIMD for one wave:
 // 8,192 rows in 1,130 us against 868.)
 //
+// Two waves share a SIMD, and of two that are ready the older one goes first,
+// so one workgroup of a CU would run a quarter faster and leave the other
+// alone at the end.  With the second half of a turn at the higher priority
+// both keep the same pace and one's products stand beside the other's
+// exponentials: 746 us for 8,192 rows against 782.
+//
 // binary16 (QT = FENCE_F16): with the page's V scale in the exponent, one
 // fused multiply-add and one exponential make the probability that the
 // product takes, and its sum comes from the rounded values by dot products.
 // The running maximum and the largest V scale are only moved when a value
 // would grow past 2^15 (kSlack), so O is rarely rescaled.
 //
-// 8,192 rows of 32 heads over 8 by 128 dimensions take 790 us in binary16,
-// 696 TFLOP/s, with the MFMA pipes busy for a third of it and the vector pipe
-// for most of the rest; 3,000 rows in fp32 (twice the products) 157 us, 252
+// 8,192 rows of 32 heads over 8 by 128 dimensions take 746 us in binary16,
+// 737 TFLOP/s, with the MFMA pipes busy for a third of it and the vector pipe
+// for most of the rest; 3,000 rows in fp32 (twice the products) 133 us, 297
 // TFLOP/s of the result's.
 template <int HD>
 struct PromptLds {
@@ -940,6 +949,7 @@ __device__ __forceinline__ void many_columns(const Q8Args& a, h8* buf, int me, i
         __syncthreads();
 
         const auto turn = [&](int un, auto masked) {
+            __builtin_amdgcn_s_setprio(0);
             const h8* half = buf + (un & 1) * HALF;
             const int pos0 = un * Prompt::UNIT;
             trim(un + 1);
@@ -973,6 +983,7 @@ __device__ __forceinline__ void many_columns(const Q8Args& a, h8* buf, int me, i
                 __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(1);
             load(un + 2, id_next);
             // Scalar loads here, where no LDS read is waited for: with one in flight such a wait is for all.
             scales(id_next);
@@ -1123,7 +1134,11 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void mixed_q8_kernel(Q
     __shared__ h8 buf[2 * PromptLds<HD>::HALF];
     static_assert(sizeof(buf) >= kWaves * kCols * (HD + 2) * sizeof(float), "the other kernel's LDS");
     const int wg = blockIdx.x;
-    if (wg < many_grid) many_columns<TYPE, QT, HD>(many, buf, wg, many_grid);
+    // Workgroups go to the XCDs in turn; shares that follow one another, mostly tiles of one kv head, to one XCD's L2:
+    // 775 us for 8,192 rows against 786, 28 against 31 for 24 x 5 drafted rows, 135 against 131 for six chunks of 500.
+    const int each = many_grid / kXcds;
+    const int share = each * kXcds == many_grid ? wg % kXcds * each + wg / kXcds : wg;
+    if (wg < many_grid) many_columns<TYPE, QT, HD>(many, buf, share, many_grid);
     else few_columns<TYPE, QT, HD>(few, reinterpret_cast<float*>(buf), wg - many_grid, gridDim.x - many_grid);
 }
 
