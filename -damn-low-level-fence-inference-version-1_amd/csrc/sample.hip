@@ -556,17 +556,13 @@ __global__ __launch_bounds__(kThreads) void sample_list(SampleArgs a) {
         });
         block_scan(s, v, &mass);
     }
-    // A bound that `want` of the threads' maxima reach, to 16 bits of the key; two bits a turn.
+    // A bound that `want` of the threads' maxima reach, to 16 bits of the key.
     uint32_t bound = 0;
     const bool all = a.vocab <= kList && !par.greedy;
     const int want = par.by_k(a) ? par.k : kTopThreads < a.slots / 2 ? kTopThreads : a.slots / 2;
     if (par.greedy) {
         bound = top;
     } else if (!all) {
-        const auto narrow = [&](auto count) {  // count(bound): how many reach it, the same in every thread
-            for (int bit = 31; bit >= 16; --bit)
-                if (count(bound | 1u << bit) >= want) bound |= 1u << bit;
-        };
         if (2 * want <= (a.slots < kThreads ? a.slots : kThreads)) {
             // Out of each thread's largest alone, a somewhat lower bound for a fraction of the work: by one wave, that
             // keeps all of them in registers and needs no barrier, 2 us where the whole workgroup takes 6.
@@ -577,30 +573,39 @@ __global__ __launch_bounds__(kThreads) void sample_list(SampleArgs a) {
                 uint32_t t[kWaves];
 #pragma unroll
                 for (int w = 0; w < kWaves; ++w) t[w] = bests[w * kWave + tid];
-                narrow([&](uint32_t least) {
-                    int n = 0;
+                for (int bit = 31; bit >= 16; --bit) {
+                    const uint32_t least = bound | 1u << bit;
+                    int n = 0;  // the same in every lane
 #pragma unroll
                     for (int w = 0; w < kWaves; ++w) n += __builtin_popcountll(__ballot(t[w] >= least));
-                    return n;
-                });
+                    if (n >= want) bound = least;
+                }
                 if (tid == 0) s.n = bound;
             }
             __syncthreads();
             bound = s.n;
         } else {
             int turn = 0;  // the two halves of s.list take turns, so one barrier a turn is enough
-            narrow([&](uint32_t least) {
-                uint32_t n = 0;  // the same in every lane
-                each_top([&](uint32_t t, int) { n += __builtin_popcountll(__ballot(t >= least)); });
-                u64* sums = s.list + turn * kWaves;
-                if (tid % kWave == 0) sums[tid / kWave] = n;
-                __syncthreads();
-                int sum = 0;
+            for (int bit = 30; bit >= 16; bit -= 2) {  // two bits a turn
+                uint32_t c[3] = {0, 0, 0};             // the same in every lane
+                each_top([&](uint32_t t, int) {
 #pragma unroll
-                for (int w = 0; w < kWaves; ++w) sum += static_cast<int>(sums[w]);
+                    for (int j = 0; j < 3; ++j)
+                        c[j] += __builtin_popcountll(__ballot(t >= (bound | static_cast<uint32_t>(j + 1) << bit)));
+                });
+                u64* sums = s.list + turn * kWaves;
+                if (tid % kWave == 0) sums[tid / kWave] = c[0] | static_cast<u64>(c[1]) << 21 | static_cast<u64>(c[2]) << 42;
+                __syncthreads();
+                u64 sum = 0;
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) sum += sums[w];
                 turn ^= 1;
-                return sum;
-            });
+                for (int j = 2; j >= 0; --j)
+                    if (static_cast<int>(sum >> (21 * j) & 0x1FFFFF) >= want) {
+                        bound |= static_cast<uint32_t>(j + 1) << bit;
+                        break;
+                    }
+            }
         }
     }
     // The logits above it, out of the threads' that have one; s.mass holds those threads' numbers meanwhile.

@@ -513,3 +513,12 @@ def test_sample_many_flat_rows():
     u = rng.random(rows).astype(np.float32)
     u[::13], u[5::13] = 0.0, np.float32(1 - 2.0 ** -24)
     check_sample(x, t, k, p, m, u)
+
+
+def test_sample_more_rows_than_a_launch_takes():
+    rng = np.random.default_rng(19)
+    rows, vocab = 33001, 70
+    x = (rng.standard_normal((rows, vocab)) * 2).astype(np.float32)
+    k = rng.integers(0, 12, rows).astype(np.int32)
+    p = rng.uniform(0.3, 1.1, rows).astype(np.float32)
+    check_sample(x, np.float32(0.9), k, p, None, rng.random(rows).astype(np.float32))
