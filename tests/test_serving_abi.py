@@ -120,3 +120,11 @@ def test_reference_sample():
     assert {R.sample(x, top_k=2, u=u) for u in (0.1, 0.5, 0.9)} == {1, 3}
     assert {R.sample(x, top_p=0.65, u=u) for u in (0.1, 0.5, 0.9)} == {1, 3}
     assert {R.sample(x, min_p=0.6, u=u) for u in (0.1, 0.5, 0.9)} == {1, 3}
+
+
+def test_model_sample_refuses():
+    import ctypes
+    import fence_model as M
+    token = ctypes.c_int(-5)
+    assert M.lib().fence_model_sample(None, P[0], 1.0, 0, 1.0, 0.0, 0.5, ctypes.byref(token)) == E
+    assert token.value == -5
