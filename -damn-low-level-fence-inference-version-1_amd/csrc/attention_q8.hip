@@ -330,7 +330,9 @@ struct Share {
 // Where a workgroup leaves its part of an item that it shares: the one that
 // it ends (or passes through) and the one that it begins.  A part: per column
 // the unnormalised output, then per column the running maximum and the sum.
-__host__ __device__ __forceinline__ int64_t part_size(int cols, int hd) { return (static_cast<int64_t>(cols) * (hd + 2) + 3) / 4 * 4; }
+__host__ __device__ __forceinline__ int64_t part_size(int cols, int hd) {
+    return (static_cast<int64_t>(cols) * (hd + 2) + 3) / 4 * 4;
+}
 __device__ __forceinline__ float* part_at(const Q8Args& a, int wg, bool begins, int hd) {
     return a.ws + (wg * 2 + (begins ? 1 : 0)) * part_size(a.part_cols, hd);
 }

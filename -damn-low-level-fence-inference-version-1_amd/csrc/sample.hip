@@ -29,7 +29,7 @@
 //      that is too many as well, by the digits of its elements' keys.
 //
 // Bound by the latency of these steps, not by bytes: one row of 151,936 with
-// top-k 20 takes 2.9 + 10.4 us (scan, list) and 9 of the two launches that
+// top-k 20 takes 2.9 + 10.4 us (scan, list) and 3 to 6 of the two launches that
 // find nothing to do; 32 rows of 128,256 with top-p take 8.8 + 22.7 + 13.4 +
 // 32.5 us; 256 rows of 151,936 with mixed filters 35 (4.4 TB/s) + 25.6 + 23 +
 // 42.
