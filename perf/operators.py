@@ -39,8 +39,9 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 def _fence():
     """The framework's binding."""
-    if "fence_ops" not in sys.modules:
-        sys.path.insert(0, glob.glob(os.path.join(glob.escape(ROOT), "*_amd"))[0])
+    pkg = glob.glob(os.path.join(glob.escape(ROOT), "*_amd"))[0]
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
     import fence_ops
 
     return fence_ops
@@ -191,7 +192,7 @@ def _prepare_store(case, g, seed):
     at = torch.arange(tokens, device="cuda") - (torch.cumsum(_int(news), 0) - _int(news))[seq] + _int(lens)[seq]
     slots = table[seq, at // page] * page + (at % page).to(torch.int32)
     dtype = torch.float32 if case["dtype"] == "f32" else torch.float16
-    row = 6 * h * d if case["fused_rows"] else h * d  # four query heads, a K and a V head of each
+    row = 3 * h * d if case["fused_rows"] else h * d
     # K has a few channels far larger than the others, as trained models do
     size = torch.ones(row, device="cuda")
     size[::37] = 6.0
