@@ -1011,6 +1011,16 @@ __device__ __forceinline__ void many_columns(const Q8Args& a, h8* buf, int me, i
                     for (int i = 0; i < 16; ++i)
                         if (!seen(h, i)) st[h][i] = -__builtin_inff();
             }
+            // In place of a page that is not there page 0's codes were multiplied: a NaN among them (e4m3), or a q that
+            // is not finite, would pass the weight of 0.  The same branch in every lane.
+            if (__any(!(in[0] && in[1] && in[2] && in[3]))) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (!in[q]) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) st[q / 2][(q % 2) * 8 + i] = 0.0f;
+                    }
+            }
             float top = -__builtin_inff();
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
