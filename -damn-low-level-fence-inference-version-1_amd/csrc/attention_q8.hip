@@ -735,7 +735,9 @@ __device__ __forceinline__ void few_columns(const Q8Args& a, float* lds, int me,
 //
 // binary16 (QT = FENCE_F16): with the page's V scale in the exponent, one
 // fused multiply-add and one exponential make the probability that the
-// product takes, and its sum comes from the rounded values by dot products.
+// product takes.  The sum takes it before it is rounded, in fp32, and with the
+// V scale taken out again: rounded, a page's weight would be lost where its
+// V scale is small beside another's.
 // The running maximum and the largest V scale are only moved when a value
 // would grow past 2^15 (kSlack), so O is rarely rescaled.
 //
@@ -746,8 +748,8 @@ __device__ __forceinline__ void few_columns(const Q8Args& a, float* lds, int me,
 template <int HD>
 struct PromptLds {
     // A half in 16-byte pieces: K fragments [2][HD / 16][64 lanes], V fragments [4][HD / 32][64 lanes], per 16
-    // positions K scale (-1 if the page is not there), V scale, its log2 and inverse, and a place for each lane to
-    // write what nobody reads.
+    // positions K scale (-1 if the page is not there), V scale and its log2, and a place for each lane to write what
+    // nobody reads.
     static constexpr int V0 = HD / 8 * kWave, S0 = V0 + HD / 8 * kWave, X0 = S0 + 4, HALF = X0 + kWave;
 };
 
@@ -881,7 +883,7 @@ __device__ __forceinline__ void many_columns(const Q8Args& a, h8* buf, int me, i
                 for (int i = 0; i < 4; ++i)
                     half[vto[i] < 0 ? X0 + lane : vto[i] + j * 32] = join(x[0][i], x[1][i], x[2][i], x[3][i]);
             }
-            *reinterpret_cast<f4*>(half + sto) = f4{ks, vs, __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs)};
+            *reinterpret_cast<f4*>(half + sto) = f4{ks, vs, __builtin_amdgcn_logf(vs), 0.0f};
         };
 
         int id_next = page_of(first);
@@ -1061,25 +1063,20 @@ __device__ __forceinline__ void many_columns(const Q8Args& a, h8* buf, int me, i
                         pf[PARTS - 1][i] = lo;
                     }
                 } else {
-                    // V codes under a scale of 0 are zero: any weight will do that can be taken back
-                    const bool none = sc[q][1] == 0.0f;
-                    const float shift = in[q] ? (none ? 0.0f : sc[q][2] - vlog) + (kBase - ref) : -__builtin_inff();
+                    // The page's V scale in units of the largest, as a power of two.  Below 2^-60 none of it is left in
+                    // binary16, but the weight has to stay; V codes under a scale of 0 are zero.  NaN stays NaN.
+                    float rel = sc[q][2] - vlog;
+                    rel = rel < -60.0f ? -60.0f : rel;
+                    const float shift = in[q] ? rel + (kBase - ref) : -__builtin_inff();
                     float p[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[q / 2][(q % 2) * 8 + i], fk, shift));
                         if (masked && !seen(q / 2, (q % 2) * 8 + i)) p[i] = 0.0f;
+                        pf[0][i] = static_cast<_Float16>(p[i]);
                     }
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 8; i += 2) {
-                        const h2 y = {static_cast<_Float16>(p[i]), static_cast<_Float16>(p[i + 1])};
-                        pf[0][i] = y[0];
-                        pf[0][i + 1] = y[1];
-                        const h2 ones = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
-                        sum = __builtin_amdgcn_fdot2(y, ones, sum, false);
-                    }
-                    l += sum * (none ? 0x1p-10f : 0x1p-10f * (vnow * sc[q][3]));
+                    const float sum = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+                    l += sum * __builtin_amdgcn_exp2f(-kBase - rel);
                 }
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import serving_ref as R
-from test_gpu_serving import check_attention
+from test_gpu_serving import bound, check_attention, random_cache, run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +37,69 @@ def test_rows_that_are_not_finite_and_see_no_page(cache, half):
 
     got = check_attention(rng, 8, 2, 64, 16, [95, 70], [90, 30], cache, half, change=bad)
     assert (got[:90] == 0).all()
+
+
+# ------------------------------------------------------------------ V scales of any size
+
+# What binary16 prompts add to test_gpu_serving's bound: they hold p times its page's V scale as a share of 2^10 of the
+# largest V scale so far, not 2^14, so what lies below binary16's smallest step 2^-24 is rounded by up to 2^-25, 2^-35 of
+# the largest |v|, for each of the n positions (the sum of the weights is 1 at least: the largest of them).
+def check_scales(rng, kv_lens, q_lens, cache, half, v_scale, q_size=2.0, heads=8, kvh=2, d=128, page=16, tiny=1e-30):
+    """v_scale(page's place in its sequence) -> the V scale of it; tiny: in place of the bound's 1e-30."""
+    blocks = [-(-n // page) for n in kv_lens]
+    ids = rng.permutation(sum(blocks)).astype(np.int32)
+    table, at = np.full((len(kv_lens), max(blocks)), -1, np.int32), 0
+    codes, scale = random_cache(rng, len(ids), kvh, page, d, cache)
+    for b, n in enumerate(blocks):
+        table[b, :n] = ids[at:at + n]
+        at += n
+        scale[1, table[b, :n]] = np.array([v_scale(j) for j in range(n)], np.float32)[:, None]
+    q_start = np.concatenate([[0], np.cumsum(q_lens)])
+    q = (rng.standard_normal((int(q_start[-1]), heads, d)) * q_size).astype(np.float16 if half else np.float32)
+    got = run_attention(q, codes, scale, table, kv_lens, q_start, cache, half, max(q_lens))
+    want, spread, big = R.attention(q, codes, scale, table, kv_lens, q_start, cache)
+    vmax = R.TOP[cache] * scale[1].astype(np.float64).max()
+    most = bound(want, spread, big, d, max(kv_lens), half, vmax) - 1e-30 + tiny + (max(kv_lens) * 2.0 ** -35 * vmax if half else 0)
+    off = np.abs(got - want)
+    assert (off <= most).all(), f"{np.nanmax(off):.3g}, {np.nanmax(off / most):.3g} of what it may be"
+    return got, want
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("q", [1, 6, 70])
+@pytest.mark.parametrize("down", [6, 10, 17, 24, 30, 36, 45, 61, 100])
+def test_attention_weight_under_small_v_scales(down, q, half):
+    """Half of the pages have a V scale far below the others': they add nothing to speak of to the output, and all of
+    their weight to the sum that divides it.  Flat scores over thousands of positions, and ordinary ones."""
+    rng = np.random.default_rng(down * 10 + q)
+    small = float(np.float32(1.5 * 2.0 ** -down))
+    for q_size in (0.01, 2.0):
+        check_scales(rng, [4100, 260], [q, q], R.INT8, half, lambda j: small if j % 2 else 1.0, q_size)
+        check_scales(rng, [1500], [q], R.E4M3, half, lambda j: 1.0 if j < 2 else small, q_size)
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("q", [1, 18])
+def test_attention_light_positions_under_small_v_scales(q, half):
+    """One heavy position on the page with the large V scale; thousands of light ones, whose weights together are as
+    much, under V scales 2^-17 of it.  As many copies of the sequence as let one workgroup meet all of one's positions."""
+    rng = np.random.default_rng(q)
+    heads, kvh, d, page, n, batch = 8, 8, 64, 64, 8256, 64
+    table = rng.permutation(n // page).astype(np.int32)[None]
+    codes, scale = random_cache(rng, n // page, kvh, page, d, R.INT8)
+    scale[1] = 2.0 ** -17
+    scale[1, table[0, 0]] = 1.0
+    # K of position 7 is 1 in dimension 0 and every other K is 0: one weight of e^9 among ones.  V of the first page's
+    # other positions is 0.
+    codes[0], codes[1, table[0, 0]] = 0, 0
+    codes[0, table[0, 0], :, 7, 0] = 127
+    codes[1, table[0, 0], :, 7] = np.arange(1, d + 1, dtype=np.uint8)
+    scale[0] = 1.0 / 127
+    rows = np.zeros((q, heads, d), np.float16 if half else np.float32)
+    rows[:, :, 0] = 9.0 * np.sqrt(d)
+    got = run_attention(np.tile(rows, (batch, 1, 1)), codes, scale, np.tile(table, (batch, 1)), [n] * batch,
+                        np.arange(batch + 1) * q, R.INT8, half, q).reshape(batch, q, heads, d)
+    want, spread, big = R.attention(rows, codes, scale, table, [n], [0, q], R.INT8)
+    assert (np.abs(want[-1, 0] / np.arange(1, d + 1) - 0.5) < 0.05).all()  # half of the weight is the heavy one's
+    most = bound(want, spread, big, d, n, half, 127.0) + (n * 2.0 ** -35 * 127 if half else 0)
+    assert (np.abs(got - want) <= most).all(), np.abs(got - want).max()
