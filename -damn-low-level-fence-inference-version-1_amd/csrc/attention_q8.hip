@@ -338,6 +338,10 @@ __device__ __forceinline__ float* part_at(const Q8Args& a, int wg, bool begins, 
 }
 __device__ __forceinline__ float* part_sums(const Q8Args& a, float* part, int hd) { return part + a.part_cols * hd; }
 
+// The least that a V scale counts as when it becomes the unit of an output: the inverse of a subnormal number may be
+// infinite.
+constexpr float kLeastUnit = 0x1p-126f;
+
 // y as the sum of two binary16 numbers, 22 bits of it.  The empty asm makes y
 // one fp32 value: otherwise the product that it came from may be rounded to
 // binary16 a second time, unrounded, and next to a tie that gives another
@@ -587,7 +591,7 @@ __device__ __forceinline__ void few_columns(const Q8Args& a, float* lds, int me,
             float vtop = vref;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
-                if (c.vs[t] > vtop && c.vs[t] < __builtin_inff()) vtop = c.vs[t];
+                if (c.vs[t] > vtop && c.vs[t] < __builtin_inff()) vtop = fmaxf(c.vs[t], kLeastUnit);
             if (__any(top > m) || vtop > vref) {
                 const float alpha = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(m - top);
                 const float beta = vtop > 0.0f ? alpha * (vref * __builtin_amdgcn_rcpf(vtop)) : 0.0f;
@@ -598,11 +602,11 @@ __device__ __forceinline__ void few_columns(const Q8Args& a, float* lds, int me,
                 for (int i = 0; i < DT; ++i) o[i] *= beta;
             }
             const float ref = m == -__builtin_inff() ? 0.0f : m;
-            const float to_v = vref > 0.0f ? 16384.0f * __builtin_amdgcn_rcpf(vref) : 0.0f;
+            const float to_v = vref > 0.0f ? __builtin_amdgcn_rcpf(vref) : 0.0f;
             h8 pf[PARTS];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const float f = c.vs[t] * to_v;
+                const float f = c.vs[t] * to_v * 16384.0f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float p = __builtin_amdgcn_exp2f(st[t][i] - ref);
@@ -662,7 +666,7 @@ __device__ __forceinline__ void few_columns(const Q8Args& a, float* lds, int me,
             for (int i = 0; i < DT; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    mo[(wave * pc + r) * HD + (4 * g + j) * DT + i] = o[i][j] * (vref * 0x1p-14f);
+                    mo[(wave * pc + r) * HD + (4 * g + j) * DT + i] = o[i][j] * 0x1p-14f * vref;
             if (g == 0) {
                 ml[(wave * pc + r) * 2] = m;
                 ml[(wave * pc + r) * 2 + 1] = l;
@@ -998,7 +1002,7 @@ __device__ __forceinline__ void many_columns(const Q8Args& a, h8* buf, int me, i
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 in[q] = !(sc[q][0] < 0.0f);
-                if (sc[q][1] > vtop && sc[q][1] < __builtin_inff()) vtop = sc[q][1];
+                if (sc[q][1] > vtop && sc[q][1] < __builtin_inff()) vtop = fmaxf(sc[q][1], kLeastUnit);
             }
             const bool grow_v = vtop > (F32 ? vref : 2.0f * vref);
             const float vnow = grow_v ? vtop : vref;
@@ -1097,10 +1101,10 @@ __device__ __forceinline__ void many_columns(const Q8Args& a, h8* buf, int me, i
 
         // o[t][i] is dimension (8 (i / 4) + 4 g + i % 4) * NT + t of this lane's column: runs of 4 NT.
         const float sum = l + __shfl_xor(l, 32);
-        const float unit_v = vref * (F32 ? 0x1p-14f : 0x1p-10f);
         if (mine) {
             const bool whole = first == 0 && last == units;
-            const float f = whole ? (sum != 0.0f ? unit_v / sum : 0.0f) : unit_v;
+            const float one = F32 ? 0x1p-14f : 0x1p-10f;  // o is in units of vref times this; vref last, it may be tiny
+            const float f = whole ? (sum != 0.0f ? one / sum : 0.0f) : one;
             float* part = part_at(a, me, first == 0, HD);
             const int64_t to = static_cast<int64_t>(s.row0 + row) * a.ldo + static_cast<int64_t>(qhead) * hd;
             if (!whole && g == 0) {
@@ -1116,7 +1120,7 @@ __device__ __forceinline__ void many_columns(const Q8Args& a, h8* buf, int me, i
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const int j = (z + i) / NT, t = (z + i) % NT;
-                        y[i] = whole && sum == 0.0f ? 0.0f : o[t][4 * q + j] * f;
+                        y[i] = whole && sum == 0.0f ? 0.0f : o[t][4 * q + j] * f * vref;
                     }
                     if (whole) {
                         if (d < hd) put8<QT>(a, to + d, y);

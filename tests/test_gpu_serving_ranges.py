@@ -103,3 +103,20 @@ def test_attention_light_positions_under_small_v_scales(q, half):
     assert (np.abs(want[-1, 0] / np.arange(1, d + 1) - 0.5) < 0.05).all()  # half of the weight is the heavy one's
     most = bound(want, spread, big, d, n, half, 127.0) + (n * 2.0 ** -35 * 127 if half else 0)
     assert (np.abs(got - want) <= most).all(), np.abs(got - want).max()
+
+
+@pytest.mark.parametrize("cache", [R.INT8, R.E4M3])
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("q", [1, 6, 70])
+@pytest.mark.parametrize("first,then", [(1e-40, 0.02), (3e-45, 0.02), (0.02, 1e-40), (1e-40, 1e-40), (3e-45, 1e-40),
+                                        (2e-36, 2e-36), (1.2e-38, 2e-37), (1e-40, 20.0)])
+def test_attention_subnormal_v_scales(first, then, q, half, cache):
+    """V scales that the store makes from tiny values: on a sequence's first pages, behind others, and on all.  Where all
+    are tiny, 1e-30 says nothing.  In its place: V scales count as 2^-126 at the least where they are the unit of the
+    output, so the share of a position that binary16 does not hold is 2^-39 of that times a code; and each wave of each
+    workgroup rounds its part to multiples of 2^-149 once, nine workgroups of four waves here, and the result is too."""
+    rng = np.random.default_rng(q)
+    for lens in ([300, 40], [1100]):
+        lens = [max(n, q) for n in lens]
+        check_scales(rng, lens, [q] * len(lens), cache, half, lambda j: first if j < 2 else then,
+                     tiny=max(lens) * 2.0 ** -39 * R.TOP[cache] * 2.0 ** -126 + 37 * 2.0 ** -150)
