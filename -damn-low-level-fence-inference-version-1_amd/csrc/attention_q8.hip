@@ -90,24 +90,24 @@ template <class KIND>
 struct Seq {
     static constexpr bool BIG = KIND::MANY;
     static constexpr int COLS = KIND::COLS, UNIT = KIND::UNIT;
-    int row0, rows, q_len, kv, group;  // first row, rows computed, rows there are, positions
+    int row0, rows, q_len, kv, cap, group;  // first row, rows computed, rows there are, positions, those the table has room for
 
     __device__ __forceinline__ Seq(const Q8Args& a, int row, int row_end, int len) : row0(row), group(a.group) {
         q_len = row_end > row ? row_end - row : 0;
         rows = q_len < a.max_q_len ? q_len : a.max_q_len;
         if ((rows * group > kCols) != BIG) rows = 0;
-        const int cap = a.max_blocks << a.page_shift;
-        kv = len < 0 ? 0 : len > cap ? cap : len;
+        cap = a.max_blocks << a.page_shift;
+        kv = len < 0 ? 0 : len;
     }
     // of the same index in every lane
     static __device__ __forceinline__ Seq uniform(const Q8Args& a, int b) {
         return Seq(a, uniform_load(a.q_start, b), uniform_load(a.q_start, b + 1), uniform_load(a.kv_lens, b));
     }
     __device__ __forceinline__ int tiles() const { return (rows * group + COLS - 1) / COLS; }
-    // positions that row i sees, i at most q_len - 1
+    // Positions that row i sees: the last row the last one, whether the table reaches it or not.
     __device__ __forceinline__ int row_sees(int i) const {
-        const int n = kv - q_len + i + 1;
-        return n < 0 ? 0 : n;
+        const int64_t n = static_cast<int64_t>(kv) - q_len + i + 1;
+        return n < 0 ? 0 : n > cap ? cap : static_cast<int>(n);
     }
     // positions that the last column of a tile sees
     __device__ __forceinline__ int sees(int tile) const {
@@ -124,7 +124,7 @@ struct Seq {
     // times the group; a linear function of the tile, so that the sum needs no loop over the tiles.
     __device__ __forceinline__ int64_t slope() const {
         const int64_t n = static_cast<int64_t>(kv) - q_len + 1;
-        return ((n < 1 ? 1 : n) + kBigItem) * group - 1;
+        return ((n < 1 ? 1 : n > cap ? cap : n) + kBigItem) * group - 1;
     }
     __device__ __forceinline__ int64_t cost(int tile) const {
         if constexpr (!BIG) return units(tile);

@@ -120,3 +120,28 @@ def test_attention_subnormal_v_scales(first, then, q, half, cache):
         lens = [max(n, q) for n in lens]
         check_scales(rng, lens, [q] * len(lens), cache, half, lambda j: first if j < 2 else then,
                      tiny=max(lens) * 2.0 ** -39 * R.TOP[cache] * 2.0 ** -126 + 37 * 2.0 ** -150)
+
+
+# ------------------------------------------------------------------ lengths past the table
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("q", [1, 6, 90])
+def test_attention_lengths_past_the_table(q, half):
+    """A row sees the positions below kv_len - q_len + i + 1; those that the table has no room for are not there, and
+    leave the others where they are.  The reference gets a table with room for all, whose further pages are not there."""
+    rng = np.random.default_rng(q + half)
+    heads, kvh, d, page, blocks = 8, 2, 64, 16, 7
+    table = rng.permutation(3 * blocks).astype(np.int32).reshape(3, blocks)
+    codes, scale = random_cache(rng, 3 * blocks, kvh, page, d, R.INT8)
+    rows = (rng.standard_normal((3 * q, heads, d)) * 2).astype(np.float16 if half else np.float32)
+    kv_lens, q_start = [blocks * page + 1, blocks * page + q // 2, blocks * page + q + 30], [0, q, 2 * q, 3 * q]
+    got = run_attention(rows, codes, scale, table, kv_lens, q_start, R.INT8, half, q)
+    room = np.concatenate([table, np.full((3, 20), -1, np.int32)], 1)
+    want, spread, big = R.attention(rows, codes, scale, room, kv_lens, q_start, R.INT8)
+    off, most = np.abs(got - want), bound(want, spread, big, d, max(kv_lens), half, 127 * scale[1].max())
+    assert (off <= most).all(), f"{off.max():.3g}, {(off / most).max():.3g} of what it may be"
+    # the largest length there is, with a last row far past the table: every row sees the whole table
+    got = run_attention(rows, codes, scale, table, [2 ** 31 - 1] * 3, q_start, R.INT8, half, q)
+    want, spread, big = R.attention(rows, codes, scale, room, [blocks * page + q] * 3, q_start, R.INT8)
+    most = bound(want, spread, big, d, blocks * page, half, 127 * scale[1].max())
+    assert (np.abs(got - want) <= most).all()
