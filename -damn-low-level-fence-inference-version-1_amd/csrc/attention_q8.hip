@@ -164,6 +164,12 @@ __device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
     return static_cast<int64_t>(static_cast<double>(x) / static_cast<double>(y));
 }
 
+// The unit of a tile of many columns that a point `off` into its cost lies in.  The product passes 64 bits where a group
+// of 256 heads meets 2^31 positions, so it is taken in 64-bit floating point, where it is as exact as the quotient.
+__device__ __forceinline__ int unit_at(int64_t off, int units, int64_t cost) {
+    return static_cast<int>(static_cast<double>(off) * units / static_cast<double>(cost));
+}
+
 // Workgroups that share the work: none without any.
 __device__ __forceinline__ int sharers(int64_t total, int grid) {
     return total < grid ? static_cast<int>(total) : grid;
@@ -267,7 +273,7 @@ __device__ __forceinline__ bool find(const Q8Args& a, int* grid, int64_t* total,
         p[i].cost = s.cost(p[i].tile);
         const int64_t off = in_head - s.before(p[i].tile);
         p[i].item = point[i] - off;
-        const int unit = KIND::MANY ? static_cast<int>(quotient(off * p[i].units, p[i].cost)) : static_cast<int>(off);
+        const int unit = KIND::MANY ? unit_at(off, p[i].units, p[i].cost) : static_cast<int>(off);
         p[i].unit = __builtin_amdgcn_readfirstlane(unit);
     }
     return true;
@@ -1177,7 +1183,7 @@ __device__ __forceinline__ void join_at(const Q8Args& a, int w0, int y, int ys) 
     const int64_t total = p.total;
     if (grid == 0 || p.unit == 0) return;
     const int64_t off0 = cut(w0, total, grid) - p.item;  // the border before
-    if (off0 > 0 && (KIND::MANY ? quotient(off0 * p.units, p.cost) : off0) > 0) return;
+    if (off0 > 0 && (KIND::MANY ? unit_at(off0, p.units, p.cost) : off0) > 0) return;
     // the workgroup whose share holds the item's end
     const int64_t end = p.item + p.cost;
     int w_end = static_cast<int>(quotient(end * grid - 1, total));

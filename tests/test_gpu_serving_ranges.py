@@ -145,3 +145,34 @@ def test_attention_lengths_past_the_table(q, half):
     want, spread, big = R.attention(rows, codes, scale, room, [blocks * page + q] * 3, q_start, R.INT8)
     most = bound(want, spread, big, d, blocks * page, half, 127 * scale[1].max())
     assert (np.abs(got - want) <= most).all()
+
+
+# ------------------------------------------------------------------ the longest cache
+
+@pytest.mark.parametrize("half", [False, True])
+def test_attention_longest_cache_and_wide_group(half):
+    """As many positions as a table may have room for, nearly 2^31, under 256 heads of one kv head: the product of a
+    place in the work and a number of units passes 64 bits.  Seven pages again and again, so the reference is a softmax
+    over theirs, each as often as it comes.
+
+    Weights and V codes are positive, so a running sum of n numbers is off by n 2^-24 of itself at the most, however they
+    come.  256 workgroups share the positions of a tile, and a lane adds up 32 of 64, one after the other: 2^22 sums, 2^-2.
+    Its products add 16 positions at a time, 2^19 of them, 2^-5; the join's 256 parts and the probabilities' rounding are
+    far below 2^-5 more."""
+    rng = np.random.default_rng(5)
+    page, d, heads, n_pages = 256, 16, 256, 7
+    blocks = (2 ** 31 - 1 - 1024) // page
+    table = (np.arange(blocks) % n_pages).astype(np.int32)[None]
+    codes, scale = random_cache(rng, n_pages, 1, page, d, R.INT8)
+    codes[1] = rng.integers(1, 128, codes[1].shape).astype(np.uint8)
+    q = rng.standard_normal((1, heads, d)).astype(np.float16 if half else np.float32)
+    n = blocks * page
+    got = run_attention(q, codes, scale, table, [n], [0, 1], R.INT8, half, 1)
+    times = np.repeat(np.bincount(table[0], minlength=n_pages), page).astype(np.float64)
+    k, v = ((R.decode(codes[i, :, 0], R.INT8) * scale[i, :, 0].astype(np.float64)[:, None, None]).reshape(-1, d)
+            for i in range(2))
+    s = q[0].astype(np.float64) @ k.T / np.sqrt(d)
+    w = np.exp(s - s.max(1, keepdims=True)) * times
+    want = (w @ v) / w.sum(1, keepdims=True)
+    assert (np.abs(got[0] - want) <= (2.0 ** -2 + 2.0 ** -4) * want).all(), np.abs(got[0] / want - 1).max()
+    print("relative to the reference:", np.abs(got[0] / want - 1).max())
