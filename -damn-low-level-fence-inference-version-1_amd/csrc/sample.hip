@@ -1153,10 +1153,8 @@ int shift_for(int vocab) {
 }
 
 // float4s a thread of sample_scan takes: fewer while the grid would not fill the GPU.
-int scan_width(int64_t rows, int vocab) {
-    const int64_t wide = (static_cast<int64_t>(vocab) + 40 * kScanThreads - 1) / (40 * kScanThreads);
-    return rows * wide < 512 ? 5 : 10;
-}
+int64_t wide_groups(int vocab) { return (static_cast<int64_t>(vocab) + 40 * kScanThreads - 1) / (40 * kScanThreads); }
+int scan_width(int64_t rows, int vocab) { return rows * wide_groups(vocab) < 512 ? 5 : 10; }
 int slots_of(int64_t rows, int vocab) {
     const int64_t per = 4ll * scan_width(rows, vocab) * kScanThreads;
     return static_cast<int>((vocab + per - 1) / per) * kScanThreads;
@@ -1174,8 +1172,11 @@ int64_t row_bytes(int slots) {
 extern "C" int64_t fence_sample_workspace(int64_t rows, int vocab) {
     using namespace fence;
     if (rows < 0 || rows > INT32_MAX || vocab < 1 || vocab > kMaxVocab) return 0;
-    const int64_t n = rows * row_bytes(slots_of(rows, vocab));
-    return n < 16 ? 16 : n;
+    // Rows that are few have twice the slots, so 34 rows of 151,936 need more than 46: what the most such rows need is
+    // the least, and a workspace serves every smaller number of rows.
+    const int64_t few = 511 / wide_groups(vocab) < rows ? 511 / wide_groups(vocab) : rows;
+    const int64_t n = rows * row_bytes(slots_of(rows, vocab)), m = few * row_bytes(slots_of(few, vocab));
+    return n > m ? n : m < 16 ? 16 : m;
 }
 
 extern "C" int fence_sample(int32_t* out, const float* logits, int64_t rows, int vocab, int64_t ld,

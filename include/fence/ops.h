@@ -455,7 +455,8 @@ int fence_sample(int32_t* out, const float* logits, int64_t rows, int vocab, int
                  const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
                  const float* u, void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
-/* Workspace bytes of fence_sample (host; 0 for bad arguments). */
+/* Workspace bytes of fence_sample (host; 0 for bad arguments).  A workspace for
+ * a number of rows serves every smaller number of the same vocab. */
 int64_t fence_sample_workspace(int64_t rows, int vocab);
 
 /* ---------------------------------------------------------------------------

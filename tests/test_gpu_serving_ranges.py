@@ -3,8 +3,10 @@ forms of serving_ref.py, within test_gpu_serving's bound unless one is derived h
 import numpy as np
 import pytest
 
+import fence_ops as F
 import serving_ref as R
-from test_gpu_serving import bound, check_attention, random_cache, run_attention
+from gpu_util import dev, host, stream, torch_mod
+from test_gpu_serving import bound, check_attention, empty, logits, random_cache, run_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -176,3 +178,23 @@ def test_attention_longest_cache_and_wide_group(half):
     want = (w @ v) / w.sum(1, keepdims=True)
     assert (np.abs(got[0] - want) <= (2.0 ** -2 + 2.0 ** -4) * want).all(), np.abs(got[0] / want - 1).max()
     print("relative to the reference:", np.abs(got[0] / want - 1).max())
+
+
+# ------------------------------------------------------------------ a sampling workspace for the largest batch
+
+def test_sample_batches_in_one_workspace():
+    """Batches of every size in the workspace of the largest, as a server holds it; nothing is written behind it."""
+    torch = torch_mod()
+    rng = np.random.default_rng(17)
+    vocab, most = 128256, 42
+    x = logits(rng, most, vocab, [0.05, 1.0, 3.0])
+    u, p = rng.random(most).astype(np.float32), np.full(most, 0.95, np.float32)
+    want = [R.sample(x[r], top_p=0.95, u=u[r]) for r in range(most)]
+    size = F.sample_workspace(most, vocab)
+    ws, d_x, d_u, d_p = empty((size + 64,), torch.uint8, 255), dev(x), dev(u), dev(p)
+    for rows in (1, 2, 5, 30, 37, 38, 39, 40, 41, 42):
+        out = empty((most,), torch.int32, -9)
+        F.sample(out.data_ptr(), d_x.data_ptr(), rows, vocab, vocab, 0, 0, d_p.data_ptr(), 0, d_u.data_ptr(), ws.data_ptr(), size,
+                 stream())
+        assert host(out).tolist() == want[:rows] + [-9] * (most - rows)
+    assert (host(ws)[size:] == 255).all()
