@@ -198,3 +198,15 @@ def test_sample_batches_in_one_workspace():
                  stream())
         assert host(out).tolist() == want[:rows] + [-9] * (most - rows)
     assert (host(ws)[size:] == 255).all()
+
+
+# ------------------------------------------------------------------ full tiles
+
+@pytest.mark.parametrize("cache", [R.INT8, R.E4M3])
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("heads,kvh,d,q", [(16, 1, 256, 1), (8, 2, 256, 4), (16, 2, 256, 2), (16, 1, 208, 1), (8, 2, 128, 4),
+                                           (4, 1, 256, 4)])
+def test_attention_exactly_sixteen_columns(heads, kvh, d, q, half, cache):
+    """As many columns as the kernel of few columns takes, at the widest heads as well: 66,048 bytes of LDS."""
+    rng = np.random.default_rng(heads + d + q)
+    check_attention(rng, heads, kvh, d, 32, [300, 17, 1100, q], [q] * 4, cache, half)
