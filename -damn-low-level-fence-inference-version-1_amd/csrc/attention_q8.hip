@@ -30,12 +30,15 @@ constexpr int kUnit = 32 * kWaves;  // positions its workgroup takes at a time
 constexpr int kPromptCols = 32 * kWaves;  // many_columns
 constexpr int64_t kMaxLd = int64_t(1) << 32;  // elements from row to row: times a row's number they fit 63 bits
 constexpr int kBeyond = 1024;  // positions past the last that may be looked up: units loaded turns ahead
-// What an item of many columns costs besides its positions, in positions.  One prompt of 8,192 rows takes
-// 730 us with 384, 736 with 192 and 747 with 128; six prompt chunks of 500 rows in fp32 130, 126 and 130.
+// What an item of many columns costs besides its positions, in positions.  With 384, 192 and 128: 24 x 5 drafted rows
+// in groups of seven 28.7, 30.1 and 28.5 us, one prompt of 8,192 rows 736, 730 and 734, six prompt chunks of 500 rows
+// in fp32 131, 126 and 131, in binary16 151, 147 and 152.
 constexpr int kBigItem = 384;
-// Workgroups that share the work: with few columns four a CU (64 single tokens at up to 32k positions take 307 us, 302
-// with two a CU and 320 with eight), with many the two that fit (a prompt of 8,192 rows: 828 us, with one 1,140).
-constexpr int kGrid = 1024;
+// Workgroups that share the work, two a CU.  With few columns, where more fit (two, four and eight a CU): one token at
+// 32,768 positions takes 33, 51 and 80 us, as each part that an item is cut into has to be joined; 64 tokens at up to
+// 4,096 60, 66 and 78, and at up to 32,768 302, 305 and 320.  With many columns two fit: a prompt of 8,192 rows takes
+// 736 us, with one a CU 1,162.
+constexpr int kGrid = 512;
 constexpr int kBigGrid = 512;
 constexpr int kXcds = 8;
 
@@ -735,13 +738,14 @@ __device__ __forceinline__ void few_columns(const Q8Args& a, float* lds, int me,
 // before; the scheduling groups keep the compiler to that and its LDS reads
 // ahead.  (Two column tiles a wave would halve what a column pays for
 // conversions and LDS reads, but take all registers of a SIMD for one wave:
-// 8,192 rows in 1,130 us against 868.)
+// 8,192 rows in 1,130 us where this form, in an earlier state, took 868.)
 //
 // Two waves share a SIMD, and of two that are ready the older one goes first,
 // so one workgroup of a CU would run a quarter faster and leave the other
 // alone at the end.  With the second half of a turn at the higher priority
 // both keep the same pace and one's products stand beside the other's
-// exponentials: 746 us for 8,192 rows against 782.
+// exponentials: 736 us for 8,192 rows against 770, and 742 with the first half
+// at the higher one.
 //
 // binary16 (QT = FENCE_F16): with the page's V scale in the exponent, one
 // fused multiply-add and one exponential make the probability that the
@@ -751,10 +755,10 @@ __device__ __forceinline__ void few_columns(const Q8Args& a, float* lds, int me,
 // The running maximum and the largest V scale are only moved when a value
 // would grow past 2^15 (kSlack), so O is rarely rescaled.
 //
-// 8,192 rows of 32 heads over 8 by 128 dimensions take 746 us in binary16,
-// 737 TFLOP/s, with the MFMA pipes busy for a third of it and the vector pipe
-// for most of the rest; 3,000 rows in fp32 (twice the products) 133 us, 297
-// TFLOP/s of the result's.
+// 8,192 rows of 32 heads over 8 by 128 dimensions take 736 us in binary16 (716
+// to 757 from machine to machine), 747 TFLOP/s, with the MFMA pipes busy for a
+// third of it and the vector pipe for most of the rest; 3,000 rows in fp32
+// (twice the products) 131 us, 302 TFLOP/s of the result's.
 template <int HD>
 struct PromptLds {
     // A half in 16-byte pieces: K fragments [2][HD / 16][64 lanes], V fragments [4][HD / 32][64 lanes], per 16
@@ -1154,7 +1158,8 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void mixed_q8_kernel(Q
     static_assert(sizeof(buf) >= kWaves * kCols * (HD + 2) * sizeof(float), "the other kernel's LDS");
     const int wg = blockIdx.x;
     // Workgroups go to the XCDs in turn; shares that follow one another, mostly tiles of one kv head, to one XCD's L2:
-    // 775 us for 8,192 rows against 786, 28 against 31 for 24 x 5 drafted rows, 135 against 131 for six chunks of 500.
+    // 736 us for 8,192 rows against 780, 28.7 against 31.5 for 24 x 5 drafted rows; six chunks of 500 rows take 151 both
+    // ways in binary16, 131 against 128 in fp32.
     const int each = many_grid / kXcds;
     const int share = each * kXcds == many_grid ? wg % kXcds * each + wg / kXcds : wg;
     if (wg < many_grid) many_columns<TYPE, QT, HD>(many, buf, share, many_grid);
