@@ -348,8 +348,11 @@ enum {
 /* One layer's cache pages.  Position j of a sequence lives in page
  * block_table[seq][j / page_size] at offset j % page_size; what it holds is
  * code * scale, with one scale per page and kv head (K and V each), not
- * negative.  page_size 16, 32, 64, 128 or 256; head_dim a multiple of 16 up to 256;
- * n_pages * page_size <= INT32_MAX; k and v 16-byte aligned. */
+ * negative.  The codes of a sequence's positions are numbers, as the store
+ * writes them: one that is e4m3's NaN would reach rows that do not see it.
+ * Codes behind a sequence's last position, and pages of no sequence, may hold
+ * anything.  page_size 16, 32, 64, 128 or 256; head_dim a multiple of 16 up to
+ * 256; n_pages * page_size <= INT32_MAX; k and v 16-byte aligned. */
 typedef struct {
     void* k;        /* codes [n_pages][n_kv_heads][page_size][head_dim] */
     void* v;        /* the same */
@@ -377,10 +380,13 @@ typedef struct {
  *   3. lens_out[b]: the new length (the old one if not admitted);
  *      free_count_out[0]: pages left.  Both may equal their inputs.
  *   4. q_start[0..batch]: the first row of each sequence's tokens, in batch
- *      order, admitted or not.  For row t of them positions[t] is its
- *      position and slots[t] = page * page_size + offset, -1 if it was not
- *      admitted.  Rows behind the last, up to max_tokens: position 0, slot -1,
- *      so that a step captured at a fixed number of rows can run padded.
+ *      order, admitted or not, so that it passes max_tokens where the new
+ *      tokens of all sequences do: arrays whose rows are taken by q_start, as
+ *      fence_gqa_attention_q8's, need q_start[batch] rows then.  For row t of
+ *      them, up to max_tokens, positions[t] is its position and slots[t] =
+ *      page * page_size + offset, -1 if it was not admitted.  Rows behind the
+ *      last, up to max_tokens: position 0, slot -1, so that a step captured at
+ *      a fixed number of rows can run padded.
  * The entries of block_table behind a sequence's pages, and those of ended
  * sequences, are left as they were.  Released ids that would not fit the
  * stack are dropped.  What fence_gqa_attention_q8 gives for the rows of a
@@ -413,16 +419,21 @@ int fence_store_kv_q8(const fence_kv_pages* cache, const void* k, const void* v,
 /* Attention of a batch over an 8-bit cache: the batched, paged form of
  * fence_gqa_attention, for single tokens, drafted tokens and prompts alike.
  * Sequence b has the rows q_start[b] .. q_start[b+1] of q and out
- * [rows][n_q_heads][head_dim] (`type` FENCE_F32 or FENCE_F16 for both, ldq and
- * ldo elements from row to row, at least n_q_heads * head_dim); its last row
- * is position kv_lens[b] - 1, so row i sees the positions below kv_lens[b] -
- * (q_start[b+1] - q_start[b]) + i + 1.  A row that sees none is zeros; rows
- * that are no sequence's are left as they were.  max_q_len bounds the rows of
- * a sequence; rows past it are not computed.  Positions past max_blocks *
- * page_size, and those in pages with an id outside [0, n_pages), count as not
- * there.  scale = 1/sqrt(head_dim); the softmax and all sums are held in
- * fp32.  FENCE_F32 agrees with fp32 arithmetic to fp32 rounding; FENCE_F16
- * rounds the probabilities to binary16.  n_q_heads % n_kv_heads == 0; batch
+ * [q_start[batch]][n_q_heads][head_dim] (`type` FENCE_F32 or FENCE_F16 for
+ * both, ldq and ldo elements from row to row, at least n_q_heads * head_dim);
+ * its last row is position kv_lens[b] - 1, so row i sees the positions below
+ * kv_lens[b] - (q_start[b+1] - q_start[b]) + i + 1.  A row that sees none is
+ * zeros; rows that are no sequence's are left as they were.  max_q_len bounds
+ * the rows of a sequence; rows past it are not computed.  Positions past
+ * max_blocks * page_size, and those in pages with an id outside [0, n_pages),
+ * count as not there and leave the border of the others where it is.  scale =
+ * 1/sqrt(head_dim); the softmax's statistics and all sums are held in fp32.
+ * What the products take is rounded: FENCE_F32 holds q, and each probability
+ * times its page's V scale, in 22 bits, about fp32's rounding; FENCE_F16 holds
+ * the latter in binary16's 11.  A probability times V scale is held to 2^-35
+ * of the largest V scale that the sequence has met (2^-39 in FENCE_F32, and
+ * for up to 16 rows times heads of a group), so what is smaller adds nothing
+ * to the output; its weight still counts.  n_q_heads % n_kv_heads == 0; batch
  * <= 65535; ldq and ldo <= 2^32; max_blocks * page_size and max_q_len *
  * n_q_heads / n_kv_heads <= INT32_MAX - 1024.
  * workspace: fence_gqa_attention_q8_workspace(...) bytes, 16-byte aligned;
@@ -443,7 +454,8 @@ int64_t fence_gqa_attention_q8_workspace(int batch, int max_q_len, int n_q_heads
  * shortest beginning that holds at least top_p of their weight; of these the
  * ones whose weight is at least min_p (the first one's is 1).  out[row] is the
  * first kept token at which the running sum of weights passes u times the
- * kept weight.  Sums are held in 64 bits.  temperature, top_k, top_p, min_p
+ * kept weight.  Weights are held to 3e-10 of themselves, and their sums in 64
+ * bits.  temperature, top_k, top_p, min_p
  * and u are device arrays of one entry per row; NULL temperature: 1, NULL or
  * out-of-range filters (top_k outside 1..vocab-1, top_p not below 1, min_p
  * not above 0): off.  temperature <= 0: the largest logit, the lowest index
