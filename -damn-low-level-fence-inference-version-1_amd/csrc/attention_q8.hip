@@ -435,8 +435,8 @@ __device__ __forceinline__ float across_rows(float v, Op op) {
 // position.  The next positions' codes are loaded before these are used.
 //
 // Bound by HBM where the batch is large: 64 tokens over 1.6 GB of int8 pages
-// take 303 us, 5.4 TB/s.  One token at 2,916 positions takes 8.8 us and the
-// join 5.6: the chain of place, page ids, codes, products and merge.
+// take 302 us, 5.4 TB/s.  One token at 2,916 positions takes 9 us and the join
+// 6: the chain of place, page ids, codes, products and merge.
 template <int TYPE, int QT, int HD>
 __device__ __forceinline__ void few_columns(const Q8Args& a, float* lds, int me, int grid) {
     constexpr int PIECES = HD / 64;       // 64 dimensions of K: 16 a lane
