@@ -1090,7 +1090,8 @@ __device__ __forceinline__ void many_columns(const Q8Args& a, h8* buf, int me, i
                         pf[0][i] = static_cast<_Float16>(p[i]);
                     }
                     const float sum = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-                    l += sum * __builtin_amdgcn_exp2f(-kBase - rel);
+                    // no weight under a scale that is NaN: none of the page's positions is seen
+                    if (!(masked && sum == 0.0f)) l += sum * __builtin_amdgcn_exp2f(-kBase - rel);
                 }
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {

@@ -210,3 +210,25 @@ def test_attention_exactly_sixteen_columns(heads, kvh, d, q, half, cache):
     """As many columns as the kernel of few columns takes, at the widest heads as well: 66,048 bytes of LDS."""
     rng = np.random.default_rng(heads + d + q)
     check_attention(rng, heads, kvh, d, 32, [300, 17, 1100, q], [q] * 4, cache, half)
+
+
+# ------------------------------------------------------------------ scales that are not finite
+
+@pytest.mark.parametrize("cache", [R.INT8, R.E4M3])
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("q", [1, 6, 90])
+def test_attention_scales_that_are_not_finite(q, half, cache):
+    """They reach the rows that see their page, and no other."""
+    rng = np.random.default_rng(19)
+
+    def broken(codes, scale, table, q):
+        scale[0, table[0, 10]] = np.nan
+        scale[1, table[1, 7]] = np.inf
+        codes[1, table[1, 7]] = 0  # times infinity: NaN, as what it is multiplied with
+        scale[1, table[2, 6]] = np.nan
+
+    got = check_attention(rng, 8, 2, 128, 16, [200, 130, 120], [q, q, q], cache, half, change=broken)
+    for last in (q - 1, 2 * q - 1, 3 * q - 1):
+        assert np.isnan(got[last]).all()
+    if q > 40:
+        assert np.isfinite(got[:40]).all() and np.isfinite(got[90:160]).all() and np.isfinite(got[180:240]).all()
